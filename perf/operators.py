@@ -82,7 +82,7 @@ def draw(rng):
     vocab = _log_int(rng, 1000, 160000)
     return {"op": op, "rows": _log_int(rng, 1, min(400, (192 * 128256) // vocab)), "vocab": vocab,
             "dtype": rng.choice(("bf16", "f32")), "bias": rng.choice((0, 1, 40, 300)),
-            "allowed": rng.choice((0.0, 0.01, 0.3, 1.0))}
+            "allowed": rng.choice((0.01, 0.1, 0.3, 1.0))}
 
 
 def _lengths(case):
@@ -160,6 +160,7 @@ def prepare(case, seed):
     mask = (bits.to(torch.int64) << torch.arange(32, device="cuda")).sum(-1)
     mask = torch.where(mask >= 1 << 31, mask - (1 << 32), mask).to(torch.int32)
     mask[1::2] = -1                       # every other row is free of the grammar
+    mask[2::16] = 0                       # and a grammar may leave a row nothing
     return {"case": case, "logits": logits, "counts": counts,
             "count_row": torch.randperm(slots, generator=g, device="cuda")[:n].to(torch.int32),
             "repetition": 1.0 + 0.3 * _rand(g, n), "frequency": 0.5 * _rand(g, n), "presence": _rand(g, n) - 0.3,
