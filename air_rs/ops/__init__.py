@@ -370,3 +370,7 @@ def gated_delta(q, k, v, alpha, beta, state=None):
     require_ext().gated_delta(f(q), f(k), f(v), f(alpha), f(beta), state, out)
     count_launch()
     return out, state
+
+
+from .recurrent import (add_rmsnorm_fp8, bias_lists, linear_attention,  # noqa: E402
+                        linear_attention_step, logit_rules)

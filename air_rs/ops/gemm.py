@@ -137,16 +137,27 @@ def linear_fp8(x: torch.Tensor, w: QWeight, out: torch.Tensor, *, residual: bool
     src/w8a8.rs:40-160)."""
     if w.fmt != FMT_FP8 or w.scales is None:
         raise ValueError("linear_fp8 needs block-scaled FP8 weights")
-    ext = require_ext()
-    T = x.shape[0]
     xq, xs = quant_fp8_rows(x)
+    return linear_fp8_rows(xq, xs, w, out, residual=residual, splits=splits, err=err)
+
+
+def linear_fp8_rows(xq: torch.Tensor, xs: torch.Tensor, w: QWeight, out: torch.Tensor, *, residual: bool = False,
+                    splits: int | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`linear_fp8` of rows that are already E4M3 codes [T, K] + one f32 scale per row
+    (``quant_fp8_rows`` or ``add_rmsnorm_fp8``)."""
+    if w.fmt != FMT_FP8 or w.scales is None:
+        raise ValueError("linear_fp8_rows needs block-scaled FP8 weights")
+    ext = require_ext()
+    T = xq.shape[0]
+    if T == 0:
+        return out
     mode = GEMM_RESIDUAL if residual else (GEMM_STORE_BF16 if out.dtype == torch.bfloat16 else GEMM_STORE_F32)
     s = splits if splits is not None else ext.gemm_fp8_splits(w.N, w.K, T)
     ws = cnt = None
     if s > 1:
-        ws, cnt = workspace(x.device).ensure(ext.gemm_fp8_workspace(w.N, T, s), ext.gemm_fp8_counters(w.N, T))
+        ws, cnt = workspace(xq.device).ensure(ext.gemm_fp8_workspace(w.N, T, s), ext.gemm_fp8_counters(w.N, T))
     if err is None:
-        err = workspace(x.device).err
+        err = workspace(xq.device).err
     ext.gemm_fp8(w.data, w.scales, w.row_bytes, w.N, w.K, xq, xs, out, mode, s, ws, cnt, err)
     count_launch()
     return out

@@ -19,6 +19,7 @@ void register_comm(pybind11::module_& m);
 void register_gds(pybind11::module_& m);
 void register_kv_push(pybind11::module_& m);
 void register_ssm(pybind11::module_& m);
+void register_recurrent(pybind11::module_& m);
 air::PeerPush peer_push_from_meta(const at::Tensor& meta);
 
 using at::Tensor;
@@ -397,6 +398,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_gemm_tc(m);
   register_kv_push(m);
   register_ssm(m);
+  register_recurrent(m);
   register_comm(m);
   register_gds(m);
 }
