@@ -120,7 +120,18 @@ void linear_attention(Tensor q, Tensor k, Tensor v, Tensor decay, optional<Tenso
   TORCH_CHECK(!a.state || a.slots || N <= a.S, "linear_attention: ", str(N), " sequences, ", str(a.S), " state rows");
   if (N == 0) return;
   const bool f32 = q.scalar_type() == at::kFloat;
-  air::launch_linear_scan(a, f32, at::cuda::getCurrentCUDAStream());
+  auto st = at::cuda::getCurrentCUDAStream();
+  if (air::linear_blocks_supported(a, f32)) {
+    const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    // scratch of the split over the length, from the allocator's pool of this stream
+    Tensor ws;
+    const int64_t n = air::linear_blocks_workspace(a, sms);
+    if (n) ws = at::empty({n}, q.options().dtype(at::kFloat));
+    const char* e = air::launch_linear_blocks(a, n ? ws.data_ptr<float>() : nullptr, sms, st);
+    TORCH_CHECK(e == nullptr, e ? e : "");
+  } else {
+    air::launch_linear_scan(a, f32, st);
+  }
   post("linear_attention");
 }
 
