@@ -10,7 +10,7 @@
 // dk = dv = 128.
 //
 // Roundings: P and the copy of S that Q S reads are bf16 (the outputs are bf16 too; the other operands
-// are exact). S itself stays f32: the keys times their f32 decay factors are split into three bf16
+// are exact). S itself stays f32: the keys times their f32 decay factors are split into four bf16
 // parts that add up to all 24 bits, each block's update is accumulated on its own and added to S in
 // registers, because adding it to a long-lived accumulator inside the tensor core would round the
 // whole state 24 times a block.
@@ -111,7 +111,7 @@ AIR_DEVICE Pos snap(const LinAttnArgs& a, int64_t p, int64_t total, int longest,
   return locate(a, at, total, len);
 }
 
-AIR_DEVICE Range make_range(const LinAttnArgs& a, int r, int R) {
+__device__ __noinline__ Range make_range(const LinAttnArgs& a, int r, int R) {
   const int lane = threadIdx.x & 31;
   int64_t total = 0;
   int most = 0;
@@ -165,18 +165,30 @@ struct Walk {
 };
 
 // ---------------------------------------------------------------- descriptors
-// N-contiguous (MN-major) operand in the 128-byte swizzle layout: rows of K are 128 B (64 bf16 of N),
-// 8-row atoms 1024 B apart along K (SBO), the next 64 columns of N one panel further (LBO).
-AIR_DEVICE uint64_t mn_desc(const void* p, uint32_t panel_bytes) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_u32(p) & 0x3FFFF) >> 4);
-  d |= (uint64_t)(panel_bytes >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
+// Both operands use the 128-byte swizzle layout (8 rows of 128 B an atom, atoms 1024 B apart); the
+// descriptors' high words are equal: stride 1024, version 1, SWIZZLE_128B.
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+// K-contiguous operand, low word.
+AIR_DEVICE uint32_t k_desc(uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); }
+// N-contiguous (MN-major) operand: rows of K hold 64 bf16 of N, the next 64 columns of N are one panel
+// further (the leading byte offset).
+AIR_DEVICE uint32_t mn_desc(uint32_t addr, uint32_t panel_bytes) { return ((addr & 0x3FFFF) >> 4) | (panel_bytes >> 4) << 16; }
+constexpr uint32_t kBMn = 1u << 16;      // instruction descriptor: B is N-contiguous
+
+AIR_DEVICE void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi) : "memory");
 }
-constexpr uint32_t kBMn = 1u << 16;      // B is N-contiguous
+AIR_DEVICE void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+      "mov.b64 y, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi) : "memory");
+}
 
 AIR_DEVICE void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
@@ -192,62 +204,176 @@ AIR_DEVICE void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-AIR_DEVICE void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
+// The same for two times 32 columns, waiting once.
+AIR_DEVICE void tmem_ld32x2(uint32_t taddr, float (&v)[32], float (&w)[32]) {
+  uint32_t r[32], q[32];
+#define AIR_LD32(R, A)                                                                                               \
+  asm volatile(                                                                                                      \
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"               \
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                                     \
+      : "=r"(R[0]), "=r"(R[1]), "=r"(R[2]), "=r"(R[3]), "=r"(R[4]), "=r"(R[5]), "=r"(R[6]), "=r"(R[7]), "=r"(R[8]),  \
+        "=r"(R[9]), "=r"(R[10]), "=r"(R[11]), "=r"(R[12]), "=r"(R[13]), "=r"(R[14]), "=r"(R[15]), "=r"(R[16]),       \
+        "=r"(R[17]), "=r"(R[18]), "=r"(R[19]), "=r"(R[20]), "=r"(R[21]), "=r"(R[22]), "=r"(R[23]), "=r"(R[24]),      \
+        "=r"(R[25]), "=r"(R[26]), "=r"(R[27]), "=r"(R[28]), "=r"(R[29]), "=r"(R[30]), "=r"(R[31])                    \
+      : "r"(A))
+  AIR_LD32(r, taddr);
+  AIR_LD32(q, taddr + 32);
+#undef AIR_LD32
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]), w[i] = __uint_as_float(q[i]);
+}
+AIR_DEVICE void tma_load_3d(uint32_t dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      ::"r"(dst), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
+}
+AIR_DEVICE void tma_store_3d(const void* tmap, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(tmap), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until the stores of this thread have read shared memory (READ) or are complete.
+template <bool READ> AIR_DEVICE void tma_store_wait() {
+  if constexpr (READ) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  else asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+AIR_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Bounded wait: gives up after about a quarter of a second, or when another role of the CTA has, and
+// leaves word of it in *abort_flag. The loop is a call, so that the many waits stay small: the code of
+// all roles together has to stay in the instruction cache.
+__device__ __noinline__ void bar_wait_slow(uint64_t* bar, uint32_t parity, int* abort_flag) {
+  const long long t0 = clock64();
+#pragma unroll 1
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return;
+    if (*(volatile int*)abort_flag != 0) return;
+    if (clock64() - t0 > (1ll << 29)) {
+      *(volatile int*)abort_flag = 1;
+      return;
+    }
+  }
+}
+// After an abort the roles leave at their next block; until then they work on whatever is there, all of
+// it inside the CTA's own memory.
+AIR_DEVICE void bar_wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
+  if (!mbar_try_wait(bar, parity & 1)) bar_wait_slow(bar, parity & 1, abort_flag);
+}
+// For copies in flight at the end: waits on whatever happened, for a shorter time.
+__device__ __noinline__ void bar_drain(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity & 1) && clock64() - t0 < (1ll << 27)) {}
+}
+// Two f32 operations in one instruction.
+AIR_DEVICE uint64_t f2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+AIR_DEVICE void unf2(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+AIR_DEVICE uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+AIR_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+AIR_DEVICE uint32_t bf2_mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+AIR_DEVICE uint32_t bf2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+AIR_DEVICE uint32_t bf2_neg(uint32_t a) {
+  uint32_t r;
+  asm("neg.bf16x2 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+AIR_DEVICE void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+AIR_DEVICE void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 AIR_DEVICE uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-AIR_DEVICE float lo_f(uint32_t u) { return __uint_as_float(u << 16); }
-AIR_DEVICE float hi_f(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
-
 // ---------------------------------------------------------------- shared memory
 template <int DK, int DV>
 struct Smem {
   static constexpr int kKTile = C * DK * 2, kVTile = C * DV * 2, kSTile = DK * DV * 2;
   static constexpr int kK = 0, kV = 2 * kKTile, kQ = kV + 2 * kVTile, kS = kQ + kKTile, kBars = kS + kSTile;
 };
-struct alignas(16) Block {         // one block's decays, all from sums within 32 tokens
+constexpr int kRing = 4;           // blocks whose decays and descriptions are in shared memory
+struct alignas(16) Block {
+  // decays, all from sums within 32 tokens
   float gl[C];                     // log2 of exp(g_1 + ... + g_i) over the token's own 32
   float e[C];                      // exp(g_{j+1} + ... ) up to the end of the token's 32
-  float w[C];                      // exp(g_{j+1} + ... + g_128); 0 past the sequence's end
+  uint32_t w[3][C / 2];            // exp(g_{j+1} + ... + g_128) as three bf16 parts, two tokens a word
   float t2[4];                     // log2 of the 32s' total decays
-  float f;                         // the block's total decay: exp(total), or expm1(total) when slow
-  int slow;
+  // S <- exp(total) S + U as one S + (f S + U): f = expm1(total), one = 1 where the decay is slow, so
+  // that a slow head does not drift by a factor that is rounded the same way every block
+  float f, one;
+  int tok, nt;                     // first token, tokens
+  int h, hq, hk, hv;               // head, and the ones it reads
+  int in;                          // the block has an incoming state
+  int first;                       // first block of a piece: S comes from src (null: zeros)
+  const float* src;
+  float* dst;                      // where S goes after the block (null: nowhere)
 };
 struct Bars {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], gfull[2], gempty[2];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], gfull[kRing], gempty[kRing];
   uint64_t qfull, qempty;
-  uint64_t sc_done, qs_done, o_done, u_done, p_ready, o_scaled, o_free, s_ready, kt_ready[2], kt_free[2], u_free;
+  uint64_t sc_done, qs_done, o_done, u_done, p_ready, o_scaled, o_free, s_ready, kt_ready[3], kt_free[3], u_free, drain;
   uint32_t tmem;
   int abort;
   Range range;
-  Block blk[2];
+  Block blk[kRing];
 };
 
-constexpr int kThreads = 512;      // 4 service warps, 4 output warps, 8 state warps
-// TMEM columns
-constexpr uint32_t kSC = 0, kO = 128, kU = 256;
-// the three parts of the transposed keys; buffer 0 shares the upper half of the scores' columns
-// (free once P is written), buffer 1 exists in the state-only kernel
-__device__ constexpr uint32_t kKT[2][3] = {{384, 448, 64}, {0, 128, 192}};
+constexpr int kThreads = 512;      // 16 warps: 4 of service (copies, products, decays, empty sequences), 4 of output, 8 of state
+AIR_DEVICE bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// TMEM columns. The scores and the update U take turns in one region: U is read before the next
+// block's scores are formed, and these are read (into P) before the next update. The decayed keys go
+// through a ring of three quarter blocks (32 tokens: four parts of 16 columns).
+constexpr uint32_t kP = 0, kO = 128, kSC = 256, kU = 256;
+AIR_DEVICE uint32_t kt_cols(int n) { return n == 0 ? 64 : n == 1 ? 384 : 448; }
+// The state-only kernel has neither P nor O and takes two regions for U in turn.
+template <bool STATE> AIR_DEVICE uint32_t u_cols(int i) { return STATE && (i & 1) ? kO : kU; }
 
 // STATE: the state-only pass over each range's cut-off last piece.
 template <int DK, int DV, bool STATE>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ LinAttnArgs a,
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
+                     const __grid_constant__ LinAttnArgs a,
                      float* __restrict__ ws_state, int4* __restrict__ ws_meta) {
   using M = Smem<DK, DV>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);   // an offset, so that accesses stay shared-space
   Bars* b = reinterpret_cast<Bars*>(smem + M::kBars);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kKt = STATE ? 2 : 1;     // buffers of the transposed keys
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == 2) {
     const Range g = make_range(a, blockIdx.x, gridDim.x);
@@ -256,13 +382,17 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b->kfull[i], 1);
-      mbar_init(&b->kempty[i], 8);
+      mbar_init(&b->kempty[i], STATE ? 8 : 9);
       mbar_init(&b->vfull[i], 1);
-      mbar_init(&b->vempty[i], 1);
-      mbar_init(&b->gfull[i], 1);
-      mbar_init(&b->gempty[i], STATE ? 8 : 12);
+      mbar_init(&b->vempty[i], STATE ? 1 : 4);
+    }
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&b->kt_ready[i], 8);
       mbar_init(&b->kt_free[i], 1);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&b->gfull[i], 1);
+      mbar_init(&b->gempty[i], STATE ? 10 : 14);
     }
     mbar_init(&b->qfull, 1);
     mbar_init(&b->qempty, 1);
@@ -275,6 +405,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     mbar_init(&b->o_free, 4);
     mbar_init(&b->s_ready, 8);
     mbar_init(&b->u_free, 8);
+    mbar_init(&b->drain, 1);
     b->abort = 0;
     fence_mbar_init();
   }
@@ -282,328 +413,419 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = b->tmem;
-  const Range rg = b->range;
-  Pos begin = rg.begin;
-  int nblk = rg.blocks;
-  if constexpr (STATE) {
-    nblk = rg.tail;
-    begin = Pos{rg.end.n, rg.end.h, rg.end.c - rg.tail};
-    if (threadIdx.x == 0) ws_meta[blockIdx.x * 2].x = rg.cut_end;
-  }
-  // a block has an incoming state unless it opens a fresh sequence
-  auto incoming = [&](const Walk& w, int i) {
-    if constexpr (STATE) return i > 0;
-    return w.p.c > 0 || (seq_init(a, w.p.n) && seq_slot(a, w.p.n) >= 0);
-  };
-  bool ok = true;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {    // one thread
-    if (ok && !mbar_wait(bar, parity & 1, &b->abort)) {
-      ok = false;
-      set_error(a.err, kErrTimeout);
-      b->abort = 1;
-    }
-    return ok;
-  };
-  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {   // all lanes give up together
-    wait(bar, parity);
-    return ok = __all_sync(0xffffffffu, ok);
-  };
+  const uint32_t tmem = __shfl_sync(0xffffffffu, b->tmem, 0);
+  const int nblk = __shfl_sync(0xffffffffu, STATE ? b->range.tail : b->range.blocks, 0);
+  auto wait = [&](uint64_t* bar, int parity) { bar_wait(bar, parity, &b->abort); };
+  auto aborted = [&] { return *(volatile int*)&b->abort != 0; };
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA producer
-    if (lane == 0) {
-      Walk w(a, begin);
-      int issued = 0;
-      for (int i = 0; i < nblk; ++i, w.next()) {
-        const int s = i & 1, u = i >> 1;
-        const int z = w.token();
-        if (i >= 2 && !wait(&b->kempty[s], u - 1)) break;
-        mbar_expect_tx(&b->kfull[s], M::kKTile);
-#pragma unroll
-        for (int p = 0; p < DK / 64; ++p)
-          tma_load_3d(smem + M::kK + s * M::kKTile + p * C * 128, &tm_k, &b->kfull[s], 64 * p, w.p.h / a.k_div, z);
-        if constexpr (!STATE) {
-          if (i >= 1 && !wait(&b->qempty, i - 1)) {
-            mbar_wait(&b->kfull[s], u & 1, nullptr, 50ull * 1000 * 1000);
-            break;
+  if (warp < 4) {
+    if (warp == 0) {
+      // -------------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        const uint32_t sm = smem_u32(smem);
+        int issued = 0, q_issued = 0;
+#pragma unroll 1
+        for (int i = 0; i < nblk; ++i) {
+          const int s = i & 1, u = i >> 1, r = i % kRing;
+          wait(&b->gfull[r], i / kRing);
+          if (i >= 2) {
+            wait(&b->kempty[s], u - 1);
+            wait(&b->vempty[s], u - 1);
           }
-          mbar_expect_tx(&b->qfull, M::kKTile);
+          if (aborted()) break;
+          const int z = b->blk[r].tok, hq = b->blk[r].hq, hk = b->blk[r].hk, hv = b->blk[r].hv;
+          mbar_arrive(&b->gempty[r]);
+          mbar_expect_tx(&b->kfull[s], M::kKTile);
+          mbar_expect_tx(&b->vfull[s], M::kVTile);
 #pragma unroll
           for (int p = 0; p < DK / 64; ++p)
-            tma_load_3d(smem + M::kQ + p * C * 128, &tm_q, &b->qfull, 64 * p, w.p.h / a.q_div, z);
-        }
-        if (i >= 2 && !wait(&b->vempty[s], u - 1)) {
-          mbar_wait(&b->kfull[s], u & 1, nullptr, 50ull * 1000 * 1000);
-          if (!STATE) mbar_wait(&b->qfull, i & 1, nullptr, 50ull * 1000 * 1000);
-          break;
-        }
-        mbar_expect_tx(&b->vfull[s], M::kVTile);
+            tma_load_3d(sm + M::kK + s * M::kKTile + p * C * 128, &tm_k, &b->kfull[s], 64 * p, hk, z);
 #pragma unroll
-        for (int p = 0; p < DV / 64; ++p)
-          tma_load_3d(smem + M::kV + s * M::kVTile + p * C * 128, &tm_v, &b->vfull[s], 64 * p, w.p.h / a.v_div, z);
-        issued = i + 1;
+          for (int p = 0; p < DV / 64; ++p)
+            tma_load_3d(sm + M::kV + s * M::kVTile + p * C * 128, &tm_v, &b->vfull[s], 64 * p, hv, z);
+          issued = i + 1;
+          if constexpr (!STATE) {
+            if (i >= 1) wait(&b->qempty, i - 1);
+            if (aborted()) break;
+            mbar_expect_tx(&b->qfull, M::kKTile);
+#pragma unroll
+            for (int p = 0; p < DK / 64; ++p) tma_load_3d(sm + M::kQ + p * C * 128, &tm_q, &b->qfull, 64 * p, hq, z);
+            ++q_issued;
+          }
+        }
+        // never leave the CTA with copies in flight into its shared memory
+        for (int i = max(0, issued - 2); i < issued; ++i) {
+          bar_drain(&b->kfull[i & 1], i >> 1);
+          bar_drain(&b->vfull[i & 1], i >> 1);
+        }
+        if (q_issued) bar_drain(&b->qfull, q_issued - 1);
       }
-      // never leave the CTA with copies in flight into its shared memory
-      for (int i = max(0, issued - 2); i < issued; ++i) {
-        mbar_wait(&b->kfull[i & 1], (i >> 1) & 1, nullptr, 50ull * 1000 * 1000);
-        mbar_wait(&b->vfull[i & 1], (i >> 1) & 1, nullptr, 50ull * 1000 * 1000);
-        if (!STATE && i == issued - 1) mbar_wait(&b->qfull, i & 1, nullptr, 50ull * 1000 * 1000);
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    } else if (warp == 1) {
+      // -------------------------------------------------------------- MMA issuer
+      // the whole warp walks and waits, so that operands stay in uniform registers; one lane issues
       constexpr uint32_t id_qk = idesc_bf16_f32(128, C);
       constexpr uint32_t id_mn = idesc_bf16_f32(128, DV) | kBMn;
-      Walk w(a, begin);
-      int n_in = 0;                      // blocks with an incoming state so far
-      for (int i = 0; i < nblk; ++i, w.next()) {
-        const int s = i & 1, u = i >> 1;
-        const uint8_t* sk = smem + M::kK + s * M::kKTile;
-        const uint8_t* sv = smem + M::kV + s * M::kVTile;
+      int n_in = 0;                        // blocks with an incoming state so far
+      int kt = 0, kt_round = 0;            // place in the ring of quarter blocks
+      const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      const uint32_t dq = k_desc(sm + M::kQ), ds = mn_desc(sm + M::kS, DK * 128);
+#pragma unroll 1
+      for (int i = 0; i < nblk; ++i) {
+        const int s = i & 1, u = i >> 1, r = i % kRing;
+        const uint32_t dks = k_desc(sm + M::kK + s * M::kKTile), dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
+        wait(&b->gfull[r], i / kRing);
+        const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
+        const int quarters = __shfl_sync(0xffffffffu, (b->blk[r].nt + 31) / 32, 0);
+        if (aborted()) break;
+        if (lane == 0) mbar_arrive(&b->gempty[r]);
         if constexpr (!STATE) {
-          const bool in = incoming(w, i);
-          // scores = Q K^T (their columns also hold the third key part of the block before)
-          if (!wait(&b->kfull[s], u) || !wait(&b->qfull, i)) break;
-          if (i >= 1 && !wait(&b->u_done, i - 1)) break;
+          // scores = Q K^T
+          wait(&b->kfull[s], u);
+          wait(&b->qfull, i);
+          if (i >= 1) wait(&b->u_free, i - 1);
           tc_fence_after();
-#pragma unroll
-          for (int ks = 0; ks < DK / 16; ++ks) {
-            const int off = (ks / 4) * C * 128;
-            mma_bf16(tmem + kSC, sw128_desc(smem + M::kQ + off) + 2 * (ks & 3), sw128_desc(sk + off) + 2 * (ks & 3),
-                     id_qk, ks > 0);
-          }
-          mma_commit(&b->sc_done);
-          if (in) {
-            // O = Q S
-            if (!wait(&b->s_ready, n_in)) break;
-            if (i >= 1 && !wait(&b->o_free, i - 1)) break;
-            tc_fence_after();
+          if (elect()) {
 #pragma unroll
             for (int ks = 0; ks < DK / 16; ++ks) {
-              const int off = (ks / 4) * C * 128;
-              mma_bf16(tmem + kO, sw128_desc(smem + M::kQ + off) + 2 * (ks & 3),
-                       mn_desc(smem + M::kS + ks * 2048, DK * 128), id_mn, ks > 0);
+              const int off = (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3);
+              mma_ss(tmem + kSC, dq + off, dks + off, id_qk, ks > 0);
             }
-            mma_commit(&b->qs_done);
+            mma_commit(&b->sc_done);
+            mma_commit(&b->kempty[s]);
           }
-          mma_commit(&b->qempty);
-          // O (+)= P V
-          if (!wait(&b->p_ready, i) || !wait(&b->vfull[s], u)) break;
-          if (in ? !wait(&b->o_scaled, n_in) : (i >= 1 && !wait(&b->o_free, i - 1))) break;
-          if (in) ++n_in;
-          tc_fence_after();
+          __syncwarp();
+          if (in) {
+            // O = Q S
+            wait(&b->s_ready, n_in);
+            if (i >= 1) wait(&b->o_free, i - 1);
+            tc_fence_after();
+            if (elect()) {
 #pragma unroll
-          for (int ks = 0; ks < C / 16; ++ks)
-            mma_bf16_ts(tmem + kO, tmem + kSC + 8 * ks, mn_desc(sv + ks * 2048, C * 128), id_mn, in || ks > 0);
-          mma_commit(&b->o_done);
+              for (int ks = 0; ks < DK / 16; ++ks)
+                mma_ss(tmem + kO, dq + (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3), ds + ks * (2048 >> 4), id_mn, ks > 0);
+              mma_commit(&b->qs_done);
+            }
+            __syncwarp();
+          }
+          if (elect()) mma_commit(&b->qempty);
+          __syncwarp();
+          wait(&b->p_ready, i);            // the scores are read
         } else {
-          if (!wait(&b->vfull[s], u)) break;
+          if (i >= 2) wait(&b->u_free, i - 2);
         }
-        // U = W V, the smallest parts first
-        const int kb = i % kKt;
-        if (!wait(&b->kt_ready[kb], i / kKt)) break;
-        if (STATE && i >= 1 && !wait(&b->u_free, i - 1)) break;
-        tc_fence_after();
+        wait(&b->vfull[s], u);
+        // U = W V, a quarter of the tokens at a time, the smallest parts first
+#pragma unroll 1
+        for (int qt = 0; qt < quarters; ++qt) {
+          wait(&b->kt_ready[kt], kt_round);
+          tc_fence_after();
+          if (elect()) {
+            const uint32_t dvq = dvs + qt * (4096 >> 4), ta = tmem + kt_cols(kt), td = tmem + u_cols<STATE>(i);
 #pragma unroll
-        for (int part = 2; part >= 0; --part)
-#pragma unroll
-          for (int ks = 0; ks < C / 16; ++ks)
-            mma_bf16_ts(tmem + kU, tmem + kKT[kb][part] + 8 * ks, mn_desc(sv + ks * 2048, C * 128), id_mn,
-                        part < 2 || ks > 0);
-        mma_commit(&b->u_done);
-        mma_commit(&b->vempty[s]);
-        if (STATE) mma_commit(&b->kt_free[kb]);
+            for (int part = 3; part >= 0; --part) {
+              mma_ts(td, ta + 16 * part, dvq, id_mn, part < 3 || qt > 0);
+              mma_ts(td, ta + 16 * part + 8, dvq + (2048 >> 4), id_mn, 1);
+            }
+            mma_commit(&b->kt_free[kt]);
+          }
+          __syncwarp();
+          if (++kt == 3) kt = 0, ++kt_round;
+        }
+        if (elect()) {
+          mma_commit(&b->u_done);
+          if (STATE) mma_commit(&b->vempty[s]);      // else the output warps release V
+        }
+        __syncwarp();
+        if constexpr (!STATE) {
+          // O (+)= P V
+          if (in) wait(&b->o_scaled, n_in);
+          else if (i >= 1) wait(&b->o_free, i - 1);
+          n_in += in;
+          tc_fence_after();
+          if (elect()) {
+#pragma unroll 1
+            for (int ks = 0; ks < 2 * quarters; ++ks)
+              mma_ts(tmem + kO, tmem + kP + 8 * ks, dvs + ks * (2048 >> 4), id_mn, in || ks > 0);
+            mma_commit(&b->o_done);
+          }
+          __syncwarp();
+        }
       }
-    }
-  } else if (warp == 2) {
-    // ---------------------------------------------------------------- decays
-    // lane l: tokens 4l .. 4l + 3; eight lanes make one of the four 32s
-    Walk w(a, begin);
-    float total_piece = 0.f;
-    for (int i = 0; i < nblk; ++i, w.next()) {
-      const int s = i & 1;
-      if (i >= 2 && !wait_warp(&b->gempty[s], (i >> 1) - 1)) break;
-      const int t0 = w.token(), nt = w.count();
-      float g[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 4 * lane + e;
-        const float x = j < nt ? a.decay[(int64_t)(t0 + j) * a.decay_t + w.p.h] : 0.f;
-        g[e] = x < kFloor ? kFloor : x;
-      }
-      float pre[4], suf[4];              // inclusive sums up to, exclusive sums after each token, in the 32
-      pre[0] = g[0]; pre[1] = pre[0] + g[1]; pre[2] = pre[1] + g[2]; pre[3] = pre[2] + g[3];
-      suf[3] = 0.f; suf[2] = g[3]; suf[1] = suf[2] + g[2]; suf[0] = suf[1] + g[1];
-      float up = pre[3], down = suf[0] + g[0];
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        const float x = __shfl_up_sync(0xffffffffu, up, o, 8), y = __shfl_down_sync(0xffffffffu, down, o, 8);
-        if ((lane & 7) >= o) up += x;
-        if ((lane & 7) + o < 8) down += y;
-      }
-      float after = __shfl_down_sync(0xffffffffu, down, 1, 8);
-      if ((lane & 7) == 7) after = 0.f;
-      float bef = __shfl_up_sync(0xffffffffu, up, 1, 8);
-      if ((lane & 7) == 0) bef = 0.f;
-      const float t[4] = {__shfl_sync(0xffffffffu, up, 7), __shfl_sync(0xffffffffu, up, 15),
-                          __shfl_sync(0xffffffffu, up, 23), __shfl_sync(0xffffffffu, up, 31)};
-      float later = 0.f;                 // the 32s after this one
-#pragma unroll
-      for (int q = 3; q > 0; --q)
-        if (lane / 8 < q) later += t[q];
-      Block& k = b->blk[s];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 4 * lane + e;
-        k.gl[j] = (bef + pre[e]) * kLog2e;
-        k.e[j] = expf(suf[e] + after);
-        k.w[j] = j < nt ? expf(suf[e] + after + later) : 0.f;
-      }
-      const float total = (t[3] + t[2]) + (t[1] + t[0]);
-      if (lane < 4) k.t2[lane] = (lane == 0 ? t[0] : lane == 1 ? t[1] : lane == 2 ? t[2] : t[3]) * kLog2e;
-      if (lane == 0) {
-        k.slow = total > -0.5f;
-        k.f = k.slow ? expm1f(total) : expf(total);
-        total_piece += total;
-      }
+      // products in flight still read shared memory and TMEM
+      if (elect()) mma_commit(&b->drain);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&b->gfull[s]);
+      bar_drain(&b->drain, 0);
+    } else if (warp == 2) {
+      // -------------------------------------------------------------- decays and descriptions
+      // lane l: tokens 4l .. 4l + 3; eight lanes make one of the four 32s
+      const Range rg = b->range;
+      Walk w(a, STATE ? Pos{rg.end.n, rg.end.h, rg.end.c - rg.tail} : rg.begin);
+      if (STATE && lane == 0) {
+        ws_meta[blockIdx.x * 2] = make_int4(rg.cut_end, 0, w.p.c == 0, w.p.n);
+        ws_meta[blockIdx.x * 2 + 1].x = w.p.h;
+      }
+      float total_piece = 0.f;
+      for (int i = 0; i < nblk; ++i) {
+        const int r = i % kRing, t0 = w.token(), nt = w.count();
+        float g[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * lane + e;
+          const float x = j < nt ? a.decay[(int64_t)(t0 + j) * a.decay_t + w.p.h] : 0.f;
+          g[e] = x < kFloor ? kFloor : x;
+        }
+        if (i >= kRing) wait(&b->gempty[r], i / kRing - 1);
+        if (aborted()) break;
+        float pre[4], suf[4];              // inclusive sums up to, exclusive sums after each token, in the 32
+        pre[0] = g[0]; pre[1] = pre[0] + g[1]; pre[2] = pre[1] + g[2]; pre[3] = pre[2] + g[3];
+        suf[3] = 0.f; suf[2] = g[3]; suf[1] = suf[2] + g[2]; suf[0] = suf[1] + g[1];
+        float up = pre[3], down = suf[0] + g[0];
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          const float x = __shfl_up_sync(0xffffffffu, up, o, 8), y = __shfl_down_sync(0xffffffffu, down, o, 8);
+          if ((lane & 7) >= o) up += x;
+          if ((lane & 7) + o < 8) down += y;
+        }
+        float after = __shfl_down_sync(0xffffffffu, down, 1, 8), bef = __shfl_up_sync(0xffffffffu, up, 1, 8);
+        if ((lane & 7) == 7) after = 0.f;
+        if ((lane & 7) == 0) bef = 0.f;
+        const float t[4] = {__shfl_sync(0xffffffffu, up, 7), __shfl_sync(0xffffffffu, up, 15),
+                            __shfl_sync(0xffffffffu, up, 23), __shfl_sync(0xffffffffu, up, 31)};
+        float later = 0.f;                 // the 32s after this one
+#pragma unroll
+        for (int q = 3; q > 0; --q)
+          if (lane / 8 < q) later += t[q];
+        Block& k = b->blk[r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * lane + e;
+          k.gl[j] = (bef + pre[e]) * kLog2e;
+          k.e[j] = ex2((suf[e] + after) * kLog2e);
+          float w = j < nt ? expf(suf[e] + after + later) : 0.f;
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            const __nv_bfloat16 h = f2bf(w);
+            reinterpret_cast<__nv_bfloat16*>(k.w[p])[j] = h;
+            w -= bf2f(h);
+          }
+        }
+        const float total = (t[3] + t[2]) + (t[1] + t[0]);
+        if (lane < 4) k.t2[lane] = (lane == 0 ? t[0] : lane == 1 ? t[1] : lane == 2 ? t[2] : t[3]) * kLog2e;
+        if (lane == 0) {
+          const bool slow = total > -0.5f;
+          k.f = slow ? expm1f(total) : expf(total);
+          k.one = slow ? 1.f : 0.f;
+          total_piece += total;
+          k.tok = t0;
+          k.nt = nt;
+          k.h = w.p.h;
+          k.hq = w.p.h / a.q_div;
+          k.hk = w.p.h / a.k_div;
+          k.hv = w.p.h / a.v_div;
+          k.first = i == 0 || w.p.c == 0;
+          k.src = nullptr;
+          k.dst = nullptr;
+          if constexpr (STATE) {
+            if (i + 1 == nblk) k.dst = ws_state + (size_t)blockIdx.x * DV * DK;
+          } else {
+            const int64_t slot = seq_slot(a, w.p.n);
+            float* row = slot < 0 ? nullptr : a.state + ((size_t)slot * a.H + w.p.h) * DV * DK;
+            k.in = w.p.c > 0;
+            if (w.p.c == 0 && row && seq_init(a, w.p.n)) {
+              // the pool's state; of a sequence that is cut the chain kernel's copy of it, because the
+              // range that ends the sequence may write the pool's row first
+              k.in = 1;
+              k.src = rg.cut_end && w.p.n == rg.end.n && w.p.h == rg.end.h
+                          ? ws_state + (size_t)(gridDim.x + blockIdx.x) * DV * DK : row;
+            } else if (i == 0 && w.p.c > 0) {
+              k.src = ws_state + (size_t)(blockIdx.x - 1) * DV * DK;
+            }
+            if (w.last()) k.dst = row;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->gfull[r]);
+        w.next();
+      }
+      if (STATE && lane == 0) ws_meta[blockIdx.x * 2].y = __float_as_int(total_piece);   // the piece's own decay
+    } else if (!STATE) {
+      // -------------------------------------------------------------- empty sequences
+      // they keep their state, or zeros when they are fresh
+      for (int n = blockIdx.x; n < a.N; n += gridDim.x) {
+        if (seq_len(a, n) > 0 || seq_init(a, n)) continue;
+        const int64_t slot = seq_slot(a, n);
+        if (slot < 0) continue;
+        float4* dst = reinterpret_cast<float4*>(a.state + (size_t)slot * a.H * DV * DK);
+        for (int64_t x = lane; x < (int64_t)a.H * DV * DK / 4; x += 32) dst[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
     }
-    if (STATE && lane == 0 && nblk > 0) {
-      // the piece's own decay, and whether it opens its sequence
-      ws_meta[blockIdx.x * 2].y = __float_as_int(total_piece);
-      ws_meta[blockIdx.x * 2].z = begin.c == 0;
-      ws_meta[blockIdx.x * 2].w = begin.n;
-      ws_meta[blockIdx.x * 2 + 1].x = begin.h;
-    }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (warp < 8) {
     // ---------------------------------------------------------------- scores -> P, O -> out
     if constexpr (!STATE) {
       const int q = warp & 3, row = 32 * q + lane;
       const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
-      Walk w(a, begin);
       int n_in = 0;
-      for (int i = 0; i < nblk; ++i, w.next()) {
-        const int s = i & 1, u = i >> 1;
-        const bool in = incoming(w, i);
-        const int nt = w.count();
-        if (!wait_warp(&b->gfull[s], u)) break;
-        const Block& k = b->blk[s];
-        const float gl = k.gl[row];
-        float fb[4];                     // row factor of each earlier 32, and of the incoming state (index q)
+      int nt = 0, in = 0, h = 0, tok = 0;
+      float gl = 0.f, rs = 0.f;            // log2 of the decay from the row's 32's and the block's begin to the row
+      auto fetch = [&](int i) {
+        wait(&b->gfull[i % kRing], i / kRing);
+        const Block& k = b->blk[i % kRing];
+        const float4 t = *reinterpret_cast<const float4*>(k.t2);
+        nt = k.nt;
+        in = k.in;
+        h = k.h;
+        tok = k.tok;
+        gl = k.gl[row];
+        rs = gl + (q > 2 ? t.z : 0.f) + (q > 1 ? t.y : 0.f) + (q > 0 ? t.x : 0.f);
+      };
+      if (nblk > 0) fetch(0);
+#pragma unroll 1
+      for (int i = 0; i < nblk; ++i) {
+        const int s = i & 1, u = i >> 1, r = i % kRing;
+        if (aborted()) break;
+        const Block& k = b->blk[r];
+        wait(&b->sc_done, i);
+        tc_fence_after();
+        float x = rs;                      // log2 of the decay from the end of 32 c to the row
+        // rolled loops: the roles' code has to stay in the instruction cache together
+#pragma unroll 1
+        for (int c = 0; c < q; ++c) {
+          uint32_t pk[16];
+          float v[32];
+          tmem_ld32(trow + kSC + 32 * c, v);
+          x -= k.t2[c];
+          const float f = ex2(x) * a.scale;
+          const uint64_t ff = f2(f, f);
+          const float4* e4 = reinterpret_cast<const float4*>(&k.e[32 * c]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 e = e4[j];
+            float p0, p1, p2, p3;
+            unf2(mul2(f2(v[4 * j], v[4 * j + 1]), mul2(ff, f2(e.x, e.y))), p0, p1);
+            unf2(mul2(f2(v[4 * j + 2], v[4 * j + 3]), mul2(ff, f2(e.z, e.w))), p2, p3);
+            pk[2 * j] = pack_bf16(p0, p1);
+            pk[2 * j + 1] = pack_bf16(p2, p3);
+          }
+          tmem_st16(trow + kP + 16 * c, pk);
+        }
         {
-          float x = gl;
+          uint32_t pk[16];
+          float v[32];
+          tmem_ld32(trow + kSC + 32 * q, v);
+          const float4* g4 = reinterpret_cast<const float4*>(&k.gl[32 * q]);
 #pragma unroll
-          for (int c = 3; c >= 0; --c) {
-            fb[c] = 0.f;
-            if (c < q) {
-              fb[c] = exp2f(x) * a.scale;
-              x += k.t2[c];
-            }
+          for (int j = 0; j < 8; ++j) {
+            const float4 g = g4[j];
+            float p0 = v[4 * j] * a.scale * ex2(gl - g.x), p1 = v[4 * j + 1] * a.scale * ex2(gl - g.y);
+            float p2 = v[4 * j + 2] * a.scale * ex2(gl - g.z), p3 = v[4 * j + 3] * a.scale * ex2(gl - g.w);
+            p0 = 4 * j <= lane ? p0 : 0.f;
+            p1 = 4 * j + 1 <= lane ? p1 : 0.f;
+            p2 = 4 * j + 2 <= lane ? p2 : 0.f;
+            p3 = 4 * j + 3 <= lane ? p3 : 0.f;
+            pk[2 * j] = pack_bf16(p0, p1);
+            pk[2 * j + 1] = pack_bf16(p2, p3);
           }
-          if (!wait_warp(&b->sc_done, i)) break;
-          tc_fence_after();
-          const float rs = exp2f(x) * a.scale;      // exp(G_i): the incoming state's factor
+          tmem_st16(trow + kP + 16 * q, pk);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-            if (c <= q) {
-              float v[32];
-              tmem_ld32(trow + kSC + 32 * c, v);
-              if (c < q) {
-                const float4* e4 = reinterpret_cast<const float4*>(&k.e[32 * c]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float4 e = e4[j];
-                  pk[2 * j] = pack_bf16(v[4 * j] * fb[c] * e.x, v[4 * j + 1] * fb[c] * e.y);
-                  pk[2 * j + 1] = pack_bf16(v[4 * j + 2] * fb[c] * e.z, v[4 * j + 3] * fb[c] * e.w);
-                }
-              } else {
-                const float4* g4 = reinterpret_cast<const float4*>(&k.gl[32 * c]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float4 g = g4[j];
-                  const float p0 = 4 * j <= lane ? v[4 * j] * a.scale * exp2f(gl - g.x) : 0.f;
-                  const float p1 = 4 * j + 1 <= lane ? v[4 * j + 1] * a.scale * exp2f(gl - g.y) : 0.f;
-                  const float p2 = 4 * j + 2 <= lane ? v[4 * j + 2] * a.scale * exp2f(gl - g.z) : 0.f;
-                  const float p3 = 4 * j + 3 <= lane ? v[4 * j + 3] * a.scale * exp2f(gl - g.w) : 0.f;
-                  pk[2 * j] = pack_bf16(p0, p1);
-                  pk[2 * j + 1] = pack_bf16(p2, p3);
-                }
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) pk[j] = 0u;
-            }
-            tmem_st16(trow + kSC + 16 * c, pk);
+          for (int j = 0; j < 16; ++j) pk[j] = 0u;
+#pragma unroll 1
+          for (int c = q + 1; c < 4; ++c) tmem_st16(trow + kP + 16 * c, pk);
+        }
+        tmem_wait_st();
+        if (nt < C) {
+          // rows of V past the sequence's end: 0 x whatever they hold must stay 0
+          wait(&b->vfull[s], u);
+          if (row >= nt && row < (nt + 31) / 32 * 32) {
+#pragma unroll 1
+            for (int c = 0; c < DV / 8; ++c)
+              *reinterpret_cast<uint4*>(smem + M::kV + s * M::kVTile + (c / 8) * C * 128 + row * 128 + 16 * (c % 8)) =
+                  make_uint4(0, 0, 0, 0);
           }
-          tmem_wait_st();
-          if (nt < C) {
-            // rows of V past the sequence's end: 0 x whatever they hold must stay 0
-            if (!wait_warp(&b->vfull[s], u)) break;
-            if (row >= nt) {
-#pragma unroll
-              for (int p = 0; p < DV / 64; ++p)
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                  *reinterpret_cast<uint4*>(smem + M::kV + s * M::kVTile + p * C * 128 + row * 128 + 16 * c) =
-                      make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&b->gempty[s]);
-            mbar_arrive(&b->p_ready);
-          }
-          if (in) {
-            if (!wait_warp(&b->qs_done, n_in)) break;
-            ++n_in;
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < DV / 32; ++c) {
-              float v[32];
-              tmem_ld32(trow + kO + 32 * c, v);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                uint32_t r[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(v[16 * h + j] * rs);
-                tmem_st16(trow + kO + 32 * c + 16 * h, r);
-              }
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b->o_scaled);
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&b->p_ready);
+          mbar_arrive(&b->gempty[r]);
+          if (i > 0) {                     // the copies out of the block before's tile of V
+            tma_store_wait<true>();
+            mbar_arrive(&b->vempty[s ^ 1]);
           }
         }
-        if (!wait_warp(&b->o_done, i)) break;
-        tc_fence_after();
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (int64_t)(w.token() + row) * a.os_t + (int64_t)w.p.h * a.os_h;
+        if (in) {
+          wait(&b->qs_done, n_in);
+          ++n_in;
+          tc_fence_after();
+          const float f = ex2(rs) * a.scale;
+          const uint64_t ff = f2(f, f);
+#pragma unroll 1
+          for (int c = 0; c < DV / 32; ++c) {
+            float v[32];
+            tmem_ld32(trow + kO + 32 * c, v);
 #pragma unroll
-        for (int c = 0; c < DV / 32; ++c) {
-          float v[32];
-          tmem_ld32(trow + kO + 32 * c, v);
-          if (c == DV / 32 - 1) {
+            for (int h = 0; h < 2; ++h) {
+              uint32_t o[16];
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                float o0, o1;
+                unf2(mul2(f2(v[16 * h + j], v[16 * h + j + 1]), ff), o0, o1);
+                o[j] = __float_as_uint(o0);
+                o[j + 1] = __float_as_uint(o1);
+              }
+              tmem_st16(trow + kO + 32 * c + 16 * h, o);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b->o_scaled);
+        }
+        // the next block's facts, before this one's output is waited for
+        const int o_nt = nt, o_tok = tok + row;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (int64_t)o_tok * a.os_t + (int64_t)h * a.os_h;
+        const int o_h = h;
+        if (i + 1 < nblk) fetch(i + 1);
+        wait(&b->o_done, i);
+        tc_fence_after();
+        // 32 full rows leave through the tile of V, which the products have finished with, as copies of
+        // 64 columns (a thread's own row is 256 bytes in global memory: 32 lines a store); the rows of a
+        // partial 32 one by one
+        const bool full = 32 * q + 32 <= o_nt;
+        uint8_t* stage = smem + M::kV + s * M::kVTile + row * 128;
+        const uint32_t st32 = smem_u32(stage);
+#pragma unroll 1
+        for (int c = 0; c < DV / 64; ++c) {
+          float v[2][32];
+          tmem_ld32x2(trow + kO + 64 * c, v[0], v[1]);
+          if (c == DV / 64 - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&b->o_free);
           }
-          if (row < nt) {
+          uint32_t o[32];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<uint4*>(out + 32 * c + 8 * j) =
-                  make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
-                             pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
+          for (int j = 0; j < 32; ++j) o[j] = pack_bf16(v[j / 16][2 * (j % 16)], v[j / 16][2 * (j % 16) + 1]);
+          if (full) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              sts128(st32 + c * C * 128 + ((j ^ (lane & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          } else if (row < o_nt) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(out + 64 * c + 8 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (full && lane == 0) {
+#pragma unroll
+          for (int c = 0; c < DV / 64; ++c) tma_store_3d(&tm_o, stage + c * C * 128, 64 * c, o_h, o_tok);
+        }
       }
+      if (lane == 0) tma_store_wait<false>();
     }
-  } else if (warp >= 8) {
+  } else {
     // ---------------------------------------------------------------- transposed keys, state
     // warps 8..11 and 12..15 share the lanes (state columns k); the first four take the first half of
     // the tokens of W and of the state's dv columns, the others the second half
@@ -611,142 +833,142 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
     constexpr int HV = DV / 2;
     const bool live = k0 < DK;
+    const int kc = live ? k0 : k0 - DK;          // dk = 64: the upper lanes are zeros
     float S[HV];
+    int kt = 0, kt_round = 0;                    // place in the ring of quarter blocks
+    int kj = 0, kq = 0;                          // block and quarter of the keys to come
+    // the decayed keys up to quarter tq of block tj
+    auto keys = [&](int tj, int tq) {
+#pragma unroll 1
+      while (kj < tj || (kj == tj && kq < tq)) {
+        const int s = kj & 1;
+        const Block& k = b->blk[kj % kRing];
+        if (kq == 0) {
+          wait(&b->gfull[kj % kRing], kj / kRing);
+          wait(&b->kfull[s], kj >> 1);
+        }
+        const int nt = k.nt;
+        // 16 tokens a thread, two to a word: the products k w of bf16 numbers in four parts that add up
+        // to all their bits. k w1 is its rounding plus an exact rest (16 bits), k w2 the same with k w3.
+        const uint8_t* col = smem + M::kK + s * M::kKTile + (kc / 64) * C * 128 + (kc & 7) * 2 + (32 * kq + 16 * half) * 128;
+        const int ch = (kc % 64) / 8;
+        uint32_t x[8], hi[8], lo[8], hi2[8], lo2[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t x0 = *reinterpret_cast<const uint16_t*>(col + 256 * e + ((ch ^ (2 * e & 7)) << 4));
+          const uint32_t x1 = *reinterpret_cast<const uint16_t*>(col + 256 * e + 128 + ((ch ^ ((2 * e + 1) & 7)) << 4));
+          x[e] = __byte_perm(x0, x1, 0x5410);
+        }
+        const int j0 = 32 * kq + 16 * half;
+        if (j0 + 16 > nt || !live) {             // tokens past the end count as zeros, whatever they hold
+          const int from = live ? nt : 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] &= (j0 + 2 * e < from ? 0xFFFFu : 0u) | (j0 + 2 * e + 1 < from ? 0xFFFF0000u : 0u);
+        }
+        const uint32_t t0 = trow + kt_cols(kt) + 8 * half;
+        {
+          const uint4 wa = *reinterpret_cast<const uint4*>(&k.w[0][j0 / 2]), wb = *reinterpret_cast<const uint4*>(&k.w[0][j0 / 2 + 4]);
+          const uint32_t w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            hi[e] = bf2_mul(x[e], w[e]);
+            lo[e] = bf2_fma(x[e], w[e], bf2_neg(hi[e]));
+          }
+        }
+        {
+          const uint4 wa = *reinterpret_cast<const uint4*>(&k.w[1][j0 / 2]), wb = *reinterpret_cast<const uint4*>(&k.w[1][j0 / 2 + 4]);
+          const uint4 va = *reinterpret_cast<const uint4*>(&k.w[2][j0 / 2]), vb = *reinterpret_cast<const uint4*>(&k.w[2][j0 / 2 + 4]);
+          const uint32_t w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+          const uint32_t v[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            hi2[e] = bf2_mul(x[e], w[e]);
+            lo2[e] = bf2_fma(x[e], v[e], bf2_fma(x[e], w[e], bf2_neg(hi2[e])));
+          }
+        }
+        if (kt_round) wait(&b->kt_free[kt], kt_round - 1);
+        tc_fence_after();
+        tmem_st8(t0, hi);
+        tmem_st8(t0 + 16, lo);
+        tmem_st8(t0 + 32, hi2);
+        tmem_st8(t0 + 48, lo2);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (++kq * 32 >= nt) {
+          if (lane == 0) mbar_arrive(&b->kempty[s]);
+          kq = 0;
+          ++kj;
+        }
+        if (lane == 0) mbar_arrive(&b->kt_ready[kt]);
+        if (++kt == 3) kt = 0, ++kt_round;
+      }
+    };
 #pragma unroll
     for (int j = 0; j < HV; ++j) S[j] = 0.f;
-    Walk w(a, begin);
-    for (int i = 0; i < nblk; ++i, w.next()) {
-      const int s = i & 1, u = i >> 1;
-      const int nt = w.count();
-      if constexpr (!STATE) {
-        const bool in = incoming(w, i);
-        if (w.p.c == 0 || i == 0) {
-          // a new piece: its incoming state is the range's (cut), the pool's, or zero. Of a sequence that
-          // is cut the chain kernel copied the pool's: the range that ends it may write that row first
-          const float* src = nullptr;
-          if (w.p.c > 0) src = ws_state + (size_t)(blockIdx.x - 1) * DV * DK;
-          else if (in && rg.cut_end && w.p.n == rg.end.n && w.p.h == rg.end.h)
-            src = ws_state + (size_t)(gridDim.x + blockIdx.x) * DV * DK;
-          else if (in) src = a.state + ((size_t)seq_slot(a, w.p.n) * a.H + w.p.h) * DV * DK;
+#pragma unroll 1
+    for (int i = -1; i < nblk; ++i) {
+      if (aborted()) break;
+      if (i >= 0) {
+        // the rest of the block's keys, and the next block's first quarter
+        keys(i + 1 < nblk ? i + 1 : i, i + 1 < nblk ? 1 : 4);
+        // S after the block: the products' update, and the state's row at the end of a piece
+        const Block& k = b->blk[i % kRing];
+        const uint64_t ff = f2(k.f, k.f), one = f2(k.one, k.one);
+        float* dst = k.dst;
+        wait(&b->u_done, i);
+        tc_fence_after();
 #pragma unroll
-          for (int j = 0; j < HV; ++j) S[j] = src && live ? src[(size_t)(half * HV + j) * DK + k0] : 0.f;
-        }
-        if (in) {
-          // bf16 copy for Q S (the products that read the one before are complete: u_done)
-          if (live) {
+        for (int c = 0; c < HV / 32; ++c) {
+          float v[32];
+          tmem_ld32(trow + u_cols<STATE>(i) + half * HV + 32 * c, v);
 #pragma unroll
-            for (int c = 0; c < HV / 8; ++c) {
-              const int v0 = half * HV + 8 * c;
-              uint8_t* dst = smem + M::kS + (v0 / 64) * DK * 128 + k0 * 128 + ((((v0 % 64) / 8) ^ (k0 & 7)) << 4);
-              *reinterpret_cast<uint4*>(dst) =
-                  make_uint4(pack_bf16(S[8 * c], S[8 * c + 1]), pack_bf16(S[8 * c + 2], S[8 * c + 3]),
-                             pack_bf16(S[8 * c + 4], S[8 * c + 5]), pack_bf16(S[8 * c + 6], S[8 * c + 7]));
-            }
+          for (int j = 0; j < 32; j += 2) {
+            const uint64_t x = f2(S[32 * c + j], S[32 * c + j + 1]);
+            unf2(fma2(x, one, fma2(x, ff, f2(v[j], v[j + 1]))), S[32 * c + j], S[32 * c + j + 1]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b->s_ready);
         }
-      }
-      const int kb = i % kKt;
-      if (!wait_warp(&b->kfull[s], u) || !wait_warp(&b->gfull[s], u)) break;
-      if constexpr (STATE) {
-        if (i >= kKt && !wait_warp(&b->kt_free[kb], i / kKt - 1)) break;
-      } else {
-        if (!wait_warp(&b->p_ready, i)) break;       // the scores' columns are free
-      }
-      tc_fence_after();
-      const Block& k = b->blk[s];
-      const float bf = k.f;
-      const bool slow = k.slow;
-      {
-        const uint8_t* col = smem + M::kK + s * M::kKTile + (k0 / 64) * C * 128 + (k0 & 7) * 2;
-        const int ch = (k0 % 64) / 8;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {            // 32 tokens: 16 columns of each part
-          const int j0 = 64 * half + 32 * c;
-          uint32_t part[3][16];
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 wj = *reinterpret_cast<const float4*>(&k.w[j0 + j]);
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int tok = j0 + j + e;
-              const uint16_t raw = live && tok < nt ? *reinterpret_cast<const uint16_t*>(col + tok * 128 + ((ch ^ (tok & 7)) << 4)) : 0;
-              x[e] = __uint_as_float((uint32_t)raw << 16) * (e == 0 ? wj.x : e == 1 ? wj.y : e == 2 ? wj.z : wj.w);
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x0 = x[2 * e], x1 = x[2 * e + 1];
-              const int o = j / 2 + e;
-              part[0][o] = pack_bf16(x0, x1);
-              x0 -= lo_f(part[0][o]);
-              x1 -= hi_f(part[0][o]);
-              part[1][o] = pack_bf16(x0, x1);
-              part[2][o] = pack_bf16(x0 - lo_f(part[1][o]), x1 - hi_f(part[1][o]));
-            }
-          }
-#pragma unroll
-          for (int p = 0; p < 3; ++p) tmem_st16(trow + kKT[kb][p] + 32 * half + 16 * c, part[p]);
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&b->kt_ready[kb]);
-        mbar_arrive(&b->kempty[s]);
-        mbar_arrive(&b->gempty[s]);
-      }
-      if (!wait_warp(&b->u_done, i)) break;
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < HV / 32; ++c) {
-        float v[32];
-        tmem_ld32(trow + kU + half * HV + 32 * c, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          float& x = S[32 * c + j];
-          x = slow ? x + fmaf(x, bf, v[j]) : fmaf(x, bf, v[j]);
-        }
-      }
-      tc_fence_before();
-      if constexpr (STATE) {
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&b->u_free);
-        if (i + 1 == nblk && live) {
-          float* dst = ws_state + (size_t)blockIdx.x * DV * DK;
-#pragma unroll
-          for (int j = 0; j < HV; ++j) dst[(size_t)(half * HV + j) * DK + k0] = S[j];
+        if (lane == 0) {
+          mbar_arrive(&b->u_free);
+          mbar_arrive(&b->gempty[i % kRing]);
         }
-      } else if (w.last() && live) {
-        const int64_t slot = seq_slot(a, w.p.n);
-        if (slot >= 0) {
-          float* dst = a.state + ((size_t)slot * a.H + w.p.h) * DV * DK;
+        if (dst && live) {
 #pragma unroll
-          for (int j = 0; j < HV; ++j) dst[(size_t)(half * HV + j) * DK + k0] = S[j];
+          for (int j = 0; j < HV; ++j) dst[(half * HV + j) * DK + k0] = S[j];
         }
       }
-    }
-  } else if (!STATE) {
-    // warp 3: empty sequences keep their state, or zeros when they are fresh
-    for (int n = blockIdx.x; n < a.N; n += gridDim.x) {
-      if (seq_len(a, n) > 0 || seq_init(a, n)) continue;
-      const int64_t slot = seq_slot(a, n);
-      if (slot < 0) continue;
-      float4* dst = reinterpret_cast<float4*>(a.state + (size_t)slot * a.H * DV * DK);
-      for (int64_t x = lane; x < (int64_t)a.H * DV * DK / 4; x += 32) dst[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (STATE || i + 1 >= nblk) continue;
+      wait(&b->gfull[(i + 1) % kRing], (i + 1) / kRing);
+      const Block& k = b->blk[(i + 1) % kRing];
+      if (k.first) {
+        const float* src = k.src;
+#pragma unroll
+        for (int j = 0; j < HV; ++j) S[j] = src && live ? src[(half * HV + j) * DK + k0] : 0.f;
+      }
+      if (k.in) {
+        // bf16 copy for Q S (the products that read the one before are complete: u_done)
+        if (live) {
+#pragma unroll
+          for (int c = 0; c < HV / 8; ++c) {
+            const int v0 = half * HV + 8 * c;
+            sts128(smem_u32(smem) + M::kS + (v0 / 64) * DK * 128 + k0 * 128 + ((((v0 % 64) / 8) ^ (k0 & 7)) << 4),
+                   pack_bf16(S[8 * c], S[8 * c + 1]), pack_bf16(S[8 * c + 2], S[8 * c + 3]),
+                   pack_bf16(S[8 * c + 4], S[8 * c + 5]), pack_bf16(S[8 * c + 6], S[8 * c + 7]));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->s_ready);
+      }
     }
   }
   __syncwarp();
-  if (warp == 1 && lane == 0) {
-    // products in flight still read shared memory and TMEM
-    mma_commit(&b->kt_free[1]);
-    mbar_wait(&b->kt_free[1], STATE ? (nblk / 2) & 1 : 0, nullptr, 50ull * 1000 * 1000);
-  }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && aborted()) set_error(a.err, kErrTimeout);
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -801,14 +1023,14 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [T, heads, d] rows in boxes of 128 tokens x one head x 64 columns
-bool encode_rows(CUtensorMap* m, const void* p, int d, int heads, int T, int64_t st_h, int64_t st_t) {
+// [T, heads, d] rows in boxes of some tokens x one head x 64 columns
+bool encode_rows(CUtensorMap* m, const void* p, int d, int heads, int T, int64_t st_h, int64_t st_t, int rows = C) {
   auto fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)T};
   // the stride of a dimension of one element is never used; it only has to be valid
   cuuint64_t strides[2] = {heads > 1 ? (cuuint64_t)st_h * 2 : (cuuint64_t)d * 2, T > 1 ? (cuuint64_t)st_t * 2 : (cuuint64_t)d * 2};
-  cuuint32_t box[3] = {64, 1, C};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)rows};
   cuuint32_t es[3] = {1, 1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -823,10 +1045,11 @@ bool needs_cut(const LinAttnArgs& a, int sms) {
 
 template <int DK, int DV>
 const char* launch_dims(const LinAttnArgs& a, float* ws, int sms, cudaStream_t st) {
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   if (!encode_rows(&tq, a.q, DK, a.H / a.q_div, a.T, a.qs_h, a.qs_t) ||
       !encode_rows(&tk, a.k, DK, a.H / a.k_div, a.T, a.ks_h, a.ks_t) ||
-      !encode_rows(&tv, a.v, DV, a.H / a.v_div, a.T, a.vs_h, a.vs_t))
+      !encode_rows(&tv, a.v, DV, a.H / a.v_div, a.T, a.vs_h, a.vs_t) ||
+      !encode_rows(&to, a.out, DV, a.H, a.T, a.os_h, a.os_t, 32))
     return "linear_attention: cuTensorMapEncodeTiled failed";
   constexpr int kSmem = Smem<DK, DV>::kBars + (int)sizeof(Bars) + 1024;
   static unsigned long long done_main = 0, done_state = 0;
@@ -837,10 +1060,10 @@ const char* launch_dims(const LinAttnArgs& a, float* ws, int sms, cudaStream_t s
   if (needs_cut(a, sms)) {
     if (!ws) return "linear_attention: workspace";
     meta = reinterpret_cast<int4*>(ws + (size_t)2 * sms * DK * DV);
-    linear_blocks_kernel<DK, DV, true><<<sms, kThreads, kSmem, st>>>(tq, tk, tv, a, ws, meta);
+    linear_blocks_kernel<DK, DV, true><<<sms, kThreads, kSmem, st>>>(tq, tk, tv, to, a, ws, meta);
     linear_chain_kernel<<<dim3(sms, (DK * DV + 1023) / 1024), 256, 0, st>>>(a, ws, meta);
   }
-  linear_blocks_kernel<DK, DV, false><<<sms, kThreads, kSmem, st>>>(tq, tk, tv, a, ws, meta);
+  linear_blocks_kernel<DK, DV, false><<<sms, kThreads, kSmem, st>>>(tq, tk, tv, to, a, ws, meta);
   return nullptr;
 }
 
