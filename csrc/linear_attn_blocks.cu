@@ -69,30 +69,30 @@ struct Range {
 };
 
 // The position of list index p (warp-wide), its item's length and the index within the item.
-AIR_DEVICE Pos locate(const LinAttnArgs& a, int64_t p, int64_t total, int& len) {
+AIR_DEVICE Pos locate(const LinAttnArgs& a, int p, int total, int& len) {
   const int lane = threadIdx.x & 31;
   Pos r{a.N, 0, 0};
   len = 0;
   if (p >= total) return r;
-  int64_t base = 0;
+  int base = 0;
   for (int n0 = 0; n0 < a.N; n0 += 32) {
     const int nb = n0 + lane < a.N ? seq_blocks(a, n0 + lane) : 0;
-    int64_t inc = (int64_t)nb * a.H;
+    int inc = nb * a.H;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
-    const int64_t all = __shfl_sync(0xffffffffu, inc, 31);
+    const int all = __shfl_sync(0xffffffffu, inc, 31);
     if (p < base + all) {
       const unsigned past = __ballot_sync(0xffffffffu, base + inc > p);
       const int l = __ffs(past) - 1;
-      const int64_t before = l ? __shfl_sync(0xffffffffu, inc, l ? l - 1 : 0) : 0;
+      const int before = l ? __shfl_sync(0xffffffffu, inc, l ? l - 1 : 0) : 0;
       len = __shfl_sync(0xffffffffu, nb, l);
-      const int64_t rel = p - base - before;
+      const int rel = p - base - before;
       r.n = n0 + l;
-      r.h = (int)(rel / len);
-      r.c = (int)(rel % len);
+      r.h = rel / len;
+      r.c = rel % len;
       return r;
     }
     base += all;
@@ -102,7 +102,7 @@ AIR_DEVICE Pos locate(const LinAttnArgs& a, int64_t p, int64_t total, int& len) 
 
 // The first position at or after list index p where a range may start: p itself inside an item that
 // is cut, else the nearer end of the item (warp-wide). Index and position.
-AIR_DEVICE Pos snap(const LinAttnArgs& a, int64_t p, int64_t total, int longest, int64_t& at) {
+AIR_DEVICE Pos snap(const LinAttnArgs& a, int p, int total, int longest, int& at) {
   int len;
   at = p < total ? p : total;
   Pos r = locate(a, p, total, len);
@@ -113,7 +113,7 @@ AIR_DEVICE Pos snap(const LinAttnArgs& a, int64_t p, int64_t total, int longest,
 
 __device__ __noinline__ Range make_range(const LinAttnArgs& a, int r, int R) {
   const int lane = threadIdx.x & 31;
-  int64_t total = 0;
+  int total = 0;
   int most = 0;
   for (int n = lane; n < a.N; n += 32) {
     const int nb = seq_blocks(a, n);
@@ -124,14 +124,14 @@ __device__ __noinline__ Range make_range(const LinAttnArgs& a, int r, int R) {
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   most = __reduce_max_sync(0xffffffffu, most);
   total *= a.H;
-  int64_t per = (total + R - 1) / R;
-  const int longest = (int)(2 * (per > kMinCut ? per : kMinCut));
+  int per = (total + R - 1) / R;
+  const int longest = 2 * max(per, kMinCut);
   if (most > longest && per < kMinCut) per = kMinCut;
   Range g;
-  int64_t i0, i1;
-  g.begin = snap(a, r * per, total, longest, i0);
-  g.end = snap(a, (r + 1) * per, total, longest, i1);
-  g.blocks = (int)(i1 - i0);
+  int i0, i1;
+  g.begin = snap(a, min(r * (int64_t)per, (int64_t)total), total, longest, i0);
+  g.end = snap(a, min((r + 1) * (int64_t)per, (int64_t)total), total, longest, i1);
+  g.blocks = i1 - i0;
   g.cut_begin = g.blocks > 0 && g.begin.c > 0;
   g.cut_end = g.blocks > 0 && g.end.n < a.N && g.end.c > 0;
   g.tail = g.cut_end ? min(g.blocks, g.end.c) : 0;
@@ -203,25 +203,6 @@ AIR_DEVICE void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-// The same for two times 32 columns, waiting once.
-AIR_DEVICE void tmem_ld32x2(uint32_t taddr, float (&v)[32], float (&w)[32]) {
-  uint32_t r[32], q[32];
-#define AIR_LD32(R, A)                                                                                               \
-  asm volatile(                                                                                                      \
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"               \
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                                     \
-      : "=r"(R[0]), "=r"(R[1]), "=r"(R[2]), "=r"(R[3]), "=r"(R[4]), "=r"(R[5]), "=r"(R[6]), "=r"(R[7]), "=r"(R[8]),  \
-        "=r"(R[9]), "=r"(R[10]), "=r"(R[11]), "=r"(R[12]), "=r"(R[13]), "=r"(R[14]), "=r"(R[15]), "=r"(R[16]),       \
-        "=r"(R[17]), "=r"(R[18]), "=r"(R[19]), "=r"(R[20]), "=r"(R[21]), "=r"(R[22]), "=r"(R[23]), "=r"(R[24]),      \
-        "=r"(R[25]), "=r"(R[26]), "=r"(R[27]), "=r"(R[28]), "=r"(R[29]), "=r"(R[30]), "=r"(R[31])                    \
-      : "r"(A))
-  AIR_LD32(r, taddr);
-  AIR_LD32(q, taddr + 32);
-#undef AIR_LD32
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]), w[i] = __uint_as_float(q[i]);
 }
 AIR_DEVICE void tma_load_3d(uint32_t dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
   asm volatile(
@@ -341,25 +322,25 @@ struct alignas(16) Block {
 struct Bars {
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], gfull[kRing], gempty[kRing];
   uint64_t qfull, qempty;
-  uint64_t sc_done, qs_done, o_done, u_done, p_ready, o_scaled, o_free, s_ready, kt_ready[3], kt_free[3], u_free, drain;
+  uint64_t sc_done, qs_done, o_done, p_ready, o_scaled, o_free, s_ready, drain;
+  uint64_t u_done[2], u_free[2], kt_ready[2], kt_free[2];   // pairs: the waiting side may be two phases behind
   uint32_t tmem;
   int abort;
   Range range;
   Block blk[kRing];
 };
 
-constexpr int kThreads = 512;      // 16 warps: 4 of service (copies, products, decays, empty sequences), 4 of output, 8 of state
+// 20 warps: 4 of service (copies, products, decays, empty sequences), 4 of output, 4 of keys, 8 of state
+constexpr int kThreads = 640;
 AIR_DEVICE bool elect() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
-// TMEM columns. The scores and the update U take turns in one region: U is read before the next
-// block's scores are formed, and these are read (into P) before the next update. The decayed keys go
-// through a ring of three quarter blocks (32 tokens: four parts of 16 columns).
-constexpr uint32_t kP = 0, kO = 128, kSC = 256, kU = 256;
-AIR_DEVICE uint32_t kt_cols(int n) { return n == 0 ? 64 : n == 1 ? 384 : 448; }
-// The state-only kernel has neither P nor O and takes two regions for U in turn.
+// TMEM columns. P takes the lower half of the scores' columns as they are read. The decayed keys go
+// through a ring of two quarter blocks (32 tokens: four parts of 16 columns).
+constexpr uint32_t kSC = 0, kP = 0, kKT = 128, kO = 256, kU = 384;
+// The state-only kernel has neither scores nor O and takes two regions for U in turn.
 template <bool STATE> AIR_DEVICE uint32_t u_cols(int i) { return STATE && (i & 1) ? kO : kU; }
 
 // STATE: the state-only pass over each range's cut-off last piece.
@@ -382,29 +363,27 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b->kfull[i], 1);
-      mbar_init(&b->kempty[i], STATE ? 8 : 9);
+      mbar_init(&b->kempty[i], STATE ? 4 : 5);
       mbar_init(&b->vfull[i], 1);
       mbar_init(&b->vempty[i], STATE ? 1 : 4);
-    }
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(&b->kt_ready[i], 8);
+      mbar_init(&b->kt_ready[i], 4);
       mbar_init(&b->kt_free[i], 1);
+      mbar_init(&b->u_done[i], 1);
+      mbar_init(&b->u_free[i], 8);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&b->gfull[i], 1);
-      mbar_init(&b->gempty[i], STATE ? 10 : 14);
+      mbar_init(&b->gempty[i], STATE ? 14 : 18);
     }
     mbar_init(&b->qfull, 1);
     mbar_init(&b->qempty, 1);
     mbar_init(&b->sc_done, 1);
     mbar_init(&b->qs_done, 1);
     mbar_init(&b->o_done, 1);
-    mbar_init(&b->u_done, 1);
     mbar_init(&b->p_ready, 4);
     mbar_init(&b->o_scaled, 4);
     mbar_init(&b->o_free, 4);
     mbar_init(&b->s_ready, 8);
-    mbar_init(&b->u_free, 8);
     mbar_init(&b->drain, 1);
     b->abort = 0;
     fence_mbar_init();
@@ -469,87 +448,95 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       int kt = 0, kt_round = 0;            // place in the ring of quarter blocks
       const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
       const uint32_t dq = k_desc(sm + M::kQ), ds = mn_desc(sm + M::kS, DK * 128);
-#pragma unroll 1
-      for (int i = 0; i < nblk; ++i) {
-        const int s = i & 1, u = i >> 1, r = i % kRing;
-        const uint32_t dks = k_desc(sm + M::kK + s * M::kKTile), dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
-        wait(&b->gfull[r], i / kRing);
-        const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
-        const int quarters = __shfl_sync(0xffffffffu, (b->blk[r].nt + 31) / 32, 0);
-        if (aborted()) break;
-        if (lane == 0) mbar_arrive(&b->gempty[r]);
-        if constexpr (!STATE) {
-          // scores = Q K^T
-          wait(&b->kfull[s], u);
-          wait(&b->qfull, i);
-          if (i >= 1) wait(&b->u_free, i - 1);
-          tc_fence_after();
-          if (elect()) {
+      auto scores = [&](int i) {           // Q K^T of block i
+        const uint32_t dks = k_desc(sm + M::kK + (i & 1) * M::kKTile);
+        wait(&b->kfull[i & 1], i >> 1);
+        wait(&b->qfull, i);
+        tc_fence_after();
+        if (elect()) {
 #pragma unroll
-            for (int ks = 0; ks < DK / 16; ++ks) {
-              const int off = (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3);
-              mma_ss(tmem + kSC, dq + off, dks + off, id_qk, ks > 0);
-            }
-            mma_commit(&b->sc_done);
-            mma_commit(&b->kempty[s]);
+          for (int ks = 0; ks < DK / 16; ++ks) {
+            const int off = (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3);
+            mma_ss(tmem + kSC, dq + off, dks + off, id_qk, ks > 0);
           }
-          __syncwarp();
-          if (in) {
-            // O = Q S
-            wait(&b->s_ready, n_in);
-            if (i >= 1) wait(&b->o_free, i - 1);
+          mma_commit(&b->sc_done);
+          mma_commit(&b->kempty[i & 1]);
+        }
+        __syncwarp();
+      };
+#pragma unroll 1
+      for (int i = STATE ? 0 : -1; i < nblk; ++i) {
+        // a block: W V of two quarters | Q S | W V of the other two | P V | the next block's Q K^T, so that
+        // P, the scaling of O and the state's update go on beside products
+        if (i >= 0) {
+          const int s = i & 1, r = i % kRing;
+          const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
+          wait(&b->gfull[r], i / kRing);
+          const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
+          const int nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0);
+          const int quarters = (nt + 31) / 32;
+          if (aborted()) break;
+          if (lane == 0) mbar_arrive(&b->gempty[r]);
+          wait(&b->vfull[s], i >> 1);
+          if (!STATE && nt < C) wait(&b->p_ready, i);       // V's rows past the end are zeroed by then
+          if (const int f = i - (STATE ? 2 : 1); f >= 0) wait(&b->u_free[f & 1], f >> 1);
+          // U = W V, a quarter of the tokens at a time, the smallest parts first
+#pragma unroll 1
+          for (int qt = 0; qt < 4; ++qt) {
+            if (qt < quarters) {
+              wait(&b->kt_ready[kt], kt_round);
+              tc_fence_after();
+              if (elect()) {
+                const uint32_t dvq = dvs + qt * (4096 >> 4), ta = tmem + kKT + 64 * kt, td = tmem + u_cols<STATE>(i);
+#pragma unroll
+                for (int part = 3; part >= 0; --part) {
+                  mma_ts(td, ta + 16 * part, dvq, id_mn, part < 3 || qt > 0);
+                  mma_ts(td, ta + 16 * part + 8, dvq + (2048 >> 4), id_mn, 1);
+                }
+                mma_commit(&b->kt_free[kt]);
+                if (qt + 1 == quarters) {
+                  mma_commit(&b->u_done[i & 1]);
+                  if (STATE) mma_commit(&b->vempty[s]);     // else the output warps release V
+                }
+              }
+              __syncwarp();
+              if (++kt == 2) kt = 0, ++kt_round;
+            }
+            if (!STATE && qt == 1) {
+              if (in) {
+                // O = Q S
+                wait(&b->s_ready, n_in);
+                if (i >= 1) wait(&b->o_free, i - 1);
+                tc_fence_after();
+                if (elect()) {
+#pragma unroll
+                  for (int ks = 0; ks < DK / 16; ++ks)
+                    mma_ss(tmem + kO, dq + (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3), ds + ks * (2048 >> 4), id_mn, ks > 0);
+                  mma_commit(&b->qs_done);
+                }
+                __syncwarp();
+              }
+              if (elect()) mma_commit(&b->qempty);
+              __syncwarp();
+            }
+          }
+          if constexpr (!STATE) {
+            // O (+)= P V
+            wait(&b->p_ready, i);
+            if (in) wait(&b->o_scaled, n_in);
+            else if (i >= 1) wait(&b->o_free, i - 1);
+            n_in += in;
             tc_fence_after();
             if (elect()) {
-#pragma unroll
-              for (int ks = 0; ks < DK / 16; ++ks)
-                mma_ss(tmem + kO, dq + (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3), ds + ks * (2048 >> 4), id_mn, ks > 0);
-              mma_commit(&b->qs_done);
+#pragma unroll 1
+              for (int ks = 0; ks < 2 * quarters; ++ks)
+                mma_ts(tmem + kO, tmem + kP + 8 * ks, dvs + ks * (2048 >> 4), id_mn, in || ks > 0);
+              mma_commit(&b->o_done);
             }
             __syncwarp();
           }
-          if (elect()) mma_commit(&b->qempty);
-          __syncwarp();
-          wait(&b->p_ready, i);            // the scores are read
-        } else {
-          if (i >= 2) wait(&b->u_free, i - 2);
         }
-        wait(&b->vfull[s], u);
-        // U = W V, a quarter of the tokens at a time, the smallest parts first
-#pragma unroll 1
-        for (int qt = 0; qt < quarters; ++qt) {
-          wait(&b->kt_ready[kt], kt_round);
-          tc_fence_after();
-          if (elect()) {
-            const uint32_t dvq = dvs + qt * (4096 >> 4), ta = tmem + kt_cols(kt), td = tmem + u_cols<STATE>(i);
-#pragma unroll
-            for (int part = 3; part >= 0; --part) {
-              mma_ts(td, ta + 16 * part, dvq, id_mn, part < 3 || qt > 0);
-              mma_ts(td, ta + 16 * part + 8, dvq + (2048 >> 4), id_mn, 1);
-            }
-            mma_commit(&b->kt_free[kt]);
-          }
-          __syncwarp();
-          if (++kt == 3) kt = 0, ++kt_round;
-        }
-        if (elect()) {
-          mma_commit(&b->u_done);
-          if (STATE) mma_commit(&b->vempty[s]);      // else the output warps release V
-        }
-        __syncwarp();
-        if constexpr (!STATE) {
-          // O (+)= P V
-          if (in) wait(&b->o_scaled, n_in);
-          else if (i >= 1) wait(&b->o_free, i - 1);
-          n_in += in;
-          tc_fence_after();
-          if (elect()) {
-#pragma unroll 1
-            for (int ks = 0; ks < 2 * quarters; ++ks)
-              mma_ts(tmem + kO, tmem + kP + 8 * ks, dvs + ks * (2048 >> 4), id_mn, in || ks > 0);
-            mma_commit(&b->o_done);
-          }
-          __syncwarp();
-        }
+        if (!STATE && i + 1 < nblk) scores(i + 1);
       }
       // products in flight still read shared memory and TMEM
       if (elect()) mma_commit(&b->drain);
@@ -795,25 +782,26 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         uint8_t* stage = smem + M::kV + s * M::kVTile + row * 128;
         const uint32_t st32 = smem_u32(stage);
 #pragma unroll 1
-        for (int c = 0; c < DV / 64; ++c) {
-          float v[2][32];
-          tmem_ld32x2(trow + kO + 64 * c, v[0], v[1]);
-          if (c == DV / 64 - 1) {
+        for (int c = 0; c < DV / 32; ++c) {
+          float v[32];
+          tmem_ld32(trow + kO + 32 * c, v);
+          if (c == DV / 32 - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&b->o_free);
           }
-          uint32_t o[32];
+          uint32_t o[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = pack_bf16(v[j / 16][2 * (j % 16)], v[j / 16][2 * (j % 16) + 1]);
+          for (int j = 0; j < 16; ++j) o[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
           if (full) {
+            const uint32_t at = st32 + (c >> 1) * C * 128;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              sts128(st32 + c * C * 128 + ((j ^ (lane & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int j = 0; j < 4; ++j)
+              sts128(at + (((4 * (c & 1) + j) ^ (lane & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           } else if (row < o_nt) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(out + 64 * c + 8 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint4*>(out + 32 * c + 8 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
         }
         fence_proxy_async_smem();
@@ -825,119 +813,120 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
       if (lane == 0) tma_store_wait<false>();
     }
-  } else {
-    // ---------------------------------------------------------------- transposed keys, state
-    // warps 8..11 and 12..15 share the lanes (state columns k); the first four take the first half of
-    // the tokens of W and of the state's dv columns, the others the second half
-    const int q = warp & 3, half = (warp - 8) >> 2, k0 = 32 * q + lane;
-    const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
-    constexpr int HV = DV / 2;
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------- transposed, decayed keys
+    // a thread has one column k of the keys, 16 tokens at a time and two to a word: the products k w of
+    // bf16 numbers in four parts that add up to all their bits. k w1 is its rounding plus an exact rest
+    // (16 bits), k w2 the same with k w3.
+    const int q = warp & 3, k0 = 32 * q + lane;
     const bool live = k0 < DK;
     const int kc = live ? k0 : k0 - DK;          // dk = 64: the upper lanes are zeros
-    float S[HV];
+    const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + kKT;
+    const uint8_t* col0 = smem + M::kK + (kc / 64) * C * 128 + (kc & 7) * 2;
+    const int ch = (kc % 64) / 8;
     int kt = 0, kt_round = 0;                    // place in the ring of quarter blocks
-    int kj = 0, kq = 0;                          // block and quarter of the keys to come
-    // the decayed keys up to quarter tq of block tj
-    auto keys = [&](int tj, int tq) {
 #pragma unroll 1
-      while (kj < tj || (kj == tj && kq < tq)) {
-        const int s = kj & 1;
-        const Block& k = b->blk[kj % kRing];
-        if (kq == 0) {
-          wait(&b->gfull[kj % kRing], kj / kRing);
-          wait(&b->kfull[s], kj >> 1);
-        }
-        const int nt = k.nt;
-        // 16 tokens a thread, two to a word: the products k w of bf16 numbers in four parts that add up
-        // to all their bits. k w1 is its rounding plus an exact rest (16 bits), k w2 the same with k w3.
-        const uint8_t* col = smem + M::kK + s * M::kKTile + (kc / 64) * C * 128 + (kc & 7) * 2 + (32 * kq + 16 * half) * 128;
-        const int ch = (kc % 64) / 8;
-        uint32_t x[8], hi[8], lo[8], hi2[8], lo2[8];
+    for (int i = 0; i < nblk; ++i) {
+      const int s = i & 1, r = i % kRing;
+      wait(&b->gfull[r], i / kRing);
+      wait(&b->kfull[s], i >> 1);
+      if (aborted()) break;
+      const Block& k = b->blk[r];
+      const int nt = k.nt, units = (nt + 31) / 32 * 2;
+      const int from = live ? nt : 0;            // tokens from here on count as zeros, whatever they hold
+#pragma unroll 1
+      for (int c = 0; c < units; ++c) {
+        const uint8_t* col = col0 + s * M::kKTile + c * 2048;
+        uint32_t x[8], p0[8], p1[8], p2[8], p3[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t x0 = *reinterpret_cast<const uint16_t*>(col + 256 * e + ((ch ^ (2 * e & 7)) << 4));
           const uint32_t x1 = *reinterpret_cast<const uint16_t*>(col + 256 * e + 128 + ((ch ^ ((2 * e + 1) & 7)) << 4));
           x[e] = __byte_perm(x0, x1, 0x5410);
         }
-        const int j0 = 32 * kq + 16 * half;
-        if (j0 + 16 > nt || !live) {             // tokens past the end count as zeros, whatever they hold
-          const int from = live ? nt : 0;
+        const int j0 = 16 * c;
+        if (j0 + 16 > from) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             x[e] &= (j0 + 2 * e < from ? 0xFFFFu : 0u) | (j0 + 2 * e + 1 < from ? 0xFFFF0000u : 0u);
         }
-        const uint32_t t0 = trow + kt_cols(kt) + 8 * half;
-        {
-          const uint4 wa = *reinterpret_cast<const uint4*>(&k.w[0][j0 / 2]), wb = *reinterpret_cast<const uint4*>(&k.w[0][j0 / 2 + 4]);
-          const uint32_t w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            hi[e] = bf2_mul(x[e], w[e]);
-            lo[e] = bf2_fma(x[e], w[e], bf2_neg(hi[e]));
+        for (int e = 0; e < 8; e += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(&k.w[0][j0 / 2 + e]), v = *reinterpret_cast<const uint4*>(&k.w[1][j0 / 2 + e]),
+                      t = *reinterpret_cast<const uint4*>(&k.w[2][j0 / 2 + e]);
+          const uint32_t w1[4] = {u.x, u.y, u.z, u.w}, w2[4] = {v.x, v.y, v.z, v.w}, w3[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            p0[e + f] = bf2_mul(x[e + f], w1[f]);
+            p1[e + f] = bf2_fma(x[e + f], w1[f], bf2_neg(p0[e + f]));
+            p2[e + f] = bf2_mul(x[e + f], w2[f]);
+            p3[e + f] = bf2_fma(x[e + f], w3[f], bf2_fma(x[e + f], w2[f], bf2_neg(p2[e + f])));
           }
         }
-        {
-          const uint4 wa = *reinterpret_cast<const uint4*>(&k.w[1][j0 / 2]), wb = *reinterpret_cast<const uint4*>(&k.w[1][j0 / 2 + 4]);
-          const uint4 va = *reinterpret_cast<const uint4*>(&k.w[2][j0 / 2]), vb = *reinterpret_cast<const uint4*>(&k.w[2][j0 / 2 + 4]);
-          const uint32_t w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
-          const uint32_t v[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            hi2[e] = bf2_mul(x[e], w[e]);
-            lo2[e] = bf2_fma(x[e], v[e], bf2_fma(x[e], w[e], bf2_neg(hi2[e])));
-          }
+        if (!(c & 1) && kt_round) {
+          wait(&b->kt_free[kt], kt_round - 1);
+          tc_fence_after();
         }
-        if (kt_round) wait(&b->kt_free[kt], kt_round - 1);
-        tc_fence_after();
-        tmem_st8(t0, hi);
-        tmem_st8(t0 + 16, lo);
-        tmem_st8(t0 + 32, hi2);
-        tmem_st8(t0 + 48, lo2);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (++kq * 32 >= nt) {
-          if (lane == 0) mbar_arrive(&b->kempty[s]);
-          kq = 0;
-          ++kj;
+        const uint32_t at = trow + 64 * kt + 8 * (c & 1);
+        tmem_st8(at, p0);
+        tmem_st8(at + 16, p1);
+        tmem_st8(at + 32, p2);
+        tmem_st8(at + 48, p3);
+        if (c & 1) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b->kt_ready[kt]);
+          if (++kt == 2) kt = 0, ++kt_round;
         }
-        if (lane == 0) mbar_arrive(&b->kt_ready[kt]);
-        if (++kt == 3) kt = 0, ++kt_round;
       }
-    };
+      if (lane == 0) {
+        mbar_arrive(&b->kempty[s]);
+        mbar_arrive(&b->gempty[r]);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- state
+    // a thread has row k of the state (transposed) and half of its dv columns, in registers
+    const int q = warp & 3, half = (warp - 12) >> 2, k0 = 32 * q + lane;
+    const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
+    constexpr int HV = DV / 2;
+    const bool live = k0 < DK;
+    const uint32_t srow = smem_u32(smem) + M::kS + k0 * 128 + (half * HV / 64) * DK * 128;
+    float S[HV];
 #pragma unroll
     for (int j = 0; j < HV; ++j) S[j] = 0.f;
 #pragma unroll 1
     for (int i = -1; i < nblk; ++i) {
       if (aborted()) break;
       if (i >= 0) {
-        // the rest of the block's keys, and the next block's first quarter
-        keys(i + 1 < nblk ? i + 1 : i, i + 1 < nblk ? 1 : 4);
         // S after the block: the products' update, and the state's row at the end of a piece
+        wait(&b->gfull[i % kRing], i / kRing);
         const Block& k = b->blk[i % kRing];
         const uint64_t ff = f2(k.f, k.f), one = f2(k.one, k.one);
         float* dst = k.dst;
-        wait(&b->u_done, i);
+        wait(&b->u_done[i & 1], i >> 1);
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < HV / 32; ++c) {
-          float v[32];
-          tmem_ld32(trow + u_cols<STATE>(i) + half * HV + 32 * c, v);
+        for (int c = 0; c < HV / 16; ++c) {
+          float v[16];
+          tmem_ld16(trow + u_cols<STATE>(i) + half * HV + 16 * c, v);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const uint64_t x = f2(S[32 * c + j], S[32 * c + j + 1]);
-            unf2(fma2(x, one, fma2(x, ff, f2(v[j], v[j + 1]))), S[32 * c + j], S[32 * c + j + 1]);
+          for (int j = 0; j < 16; j += 2) {
+            const uint64_t x = f2(S[16 * c + j], S[16 * c + j + 1]);
+            unf2(fma2(x, one, fma2(x, ff, f2(v[j], v[j + 1]))), S[16 * c + j], S[16 * c + j + 1]);
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&b->u_free);
+          mbar_arrive(&b->u_free[i & 1]);
           mbar_arrive(&b->gempty[i % kRing]);
         }
         if (dst && live) {
+          float* d = dst + half * HV * DK + k0;
 #pragma unroll
-          for (int j = 0; j < HV; ++j) dst[(half * HV + j) * DK + k0] = S[j];
+          for (int j = 0; j < HV; ++j) d[j * DK] = S[j];
         }
       }
       if (STATE || i + 1 >= nblk) continue;
@@ -945,19 +934,17 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const Block& k = b->blk[(i + 1) % kRing];
       if (k.first) {
         const float* src = k.src;
+        const float* d = src + half * HV * DK + k0;
 #pragma unroll
-        for (int j = 0; j < HV; ++j) S[j] = src && live ? src[(half * HV + j) * DK + k0] : 0.f;
+        for (int j = 0; j < HV; ++j) S[j] = src && live ? d[j * DK] : 0.f;
       }
       if (k.in) {
         // bf16 copy for Q S (the products that read the one before are complete: u_done)
         if (live) {
 #pragma unroll
-          for (int c = 0; c < HV / 8; ++c) {
-            const int v0 = half * HV + 8 * c;
-            sts128(smem_u32(smem) + M::kS + (v0 / 64) * DK * 128 + k0 * 128 + ((((v0 % 64) / 8) ^ (k0 & 7)) << 4),
-                   pack_bf16(S[8 * c], S[8 * c + 1]), pack_bf16(S[8 * c + 2], S[8 * c + 3]),
-                   pack_bf16(S[8 * c + 4], S[8 * c + 5]), pack_bf16(S[8 * c + 6], S[8 * c + 7]));
-          }
+          for (int c = 0; c < HV / 8; ++c)
+            sts128(srow + ((((half * HV % 64) / 8 + c) ^ (k0 & 7)) << 4), pack_bf16(S[8 * c], S[8 * c + 1]),
+                   pack_bf16(S[8 * c + 2], S[8 * c + 3]), pack_bf16(S[8 * c + 4], S[8 * c + 5]), pack_bf16(S[8 * c + 6], S[8 * c + 7]));
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -1074,7 +1061,7 @@ bool linear_blocks_supported(const LinAttnArgs& a, bool f32) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (heads == 1 || (sh % 8 == 0 && sh > 0)) &&
            (T == 1 || (st % 8 == 0 && st > 0)) && sh < (1ll << 38) && st < (1ll << 38);
   };
-  return !f32 && (a.dk == 64 || a.dk == 128) && (a.dv == 64 || a.dv == 128) && a.T > 0 &&
+  return !f32 && ((int64_t)a.T / C + a.N) * a.H < (1ll << 30) && (a.dk == 64 || a.dk == 128) && (a.dv == 64 || a.dv == 128) && a.T > 0 &&
          ok(a.q, a.qs_h, a.qs_t, a.H / a.q_div, a.T) && ok(a.k, a.ks_h, a.ks_t, a.H / a.k_div, a.T) &&
          ok(a.v, a.vs_h, a.vs_t, a.H / a.v_div, a.T) && ok(a.out, a.os_h, a.os_t, a.H, a.T) &&
          reinterpret_cast<uintptr_t>(a.state) % 16 == 0;
