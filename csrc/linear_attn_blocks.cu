@@ -284,10 +284,19 @@ AIR_DEVICE uint32_t bf2_neg(uint32_t a) {
   asm("neg.bf16x2 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
-AIR_DEVICE void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+// 16 lanes x 32 columns from matrix fragments: for every 4 columns 4 j + t % 4, thread t writes lane t / 4
+// (r[2 j]) and 8 + t / 4 (r[2 j + 1]).
+AIR_DEVICE void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Four transposed 8 x 8 tiles of 16-bit numbers: thread t gets rows 2 (t % 4), + 1 of column t / 4 of each.
+AIR_DEVICE void ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 AIR_DEVICE void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -338,7 +347,7 @@ AIR_DEVICE bool elect() {
   return p != 0;
 }
 // TMEM columns. P takes the lower half of the scores' columns as they are read. The decayed keys go
-// through a ring of two quarter blocks (32 tokens: four parts of 16 columns).
+// through a ring of two quarter blocks (two times 16 tokens: four parts of 8 columns).
 constexpr uint32_t kSC = 0, kP = 0, kKT = 128, kO = 256, kU = 384;
 // The state-only kernel has neither scores nor O and takes two regions for U in turn.
 template <bool STATE> AIR_DEVICE uint32_t u_cols(int i) { return STATE && (i & 1) ? kO : kU; }
@@ -360,10 +369,16 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const Range g = make_range(a, blockIdx.x, gridDim.x);
     if (lane == 0) b->range = g;
   }
+  if (warp == 3 && lane == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    if (!STATE) prefetch_tmap(&tm_q);
+    if (!STATE) prefetch_tmap(&tm_o);
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b->kfull[i], 1);
-      mbar_init(&b->kempty[i], STATE ? 4 : 5);
+      mbar_init(&b->kempty[i], STATE ? 4 : 8);
       mbar_init(&b->vfull[i], 1);
       mbar_init(&b->vempty[i], STATE ? 1 : 4);
       mbar_init(&b->kt_ready[i], 4);
@@ -376,7 +391,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&b->gempty[i], STATE ? 14 : 18);
     }
     mbar_init(&b->qfull, 1);
-    mbar_init(&b->qempty, 1);
+    mbar_init(&b->qempty, 4);
     mbar_init(&b->sc_done, 1);
     mbar_init(&b->qs_done, 1);
     mbar_init(&b->o_done, 1);
@@ -398,7 +413,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   auto aborted = [&] { return *(volatile int*)&b->abort != 0; };
 
   if (warp < 4) {
-    if (warp == 0) {
+    if (warp == 1) {
       // -------------------------------------------------------------- TMA producer
       if (lane == 0) {
         const uint32_t sm = smem_u32(smem);
@@ -439,8 +454,9 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         if (q_issued) bar_drain(&b->qfull, q_issued - 1);
       }
-    } else if (warp == 1) {
+    } else if (warp == 0) {
       // -------------------------------------------------------------- MMA issuer
+      // (on the scheduler of the output warp with the least to do)
       // the whole warp walks and waits, so that operands stay in uniform registers; one lane issues
       constexpr uint32_t id_qk = idesc_bf16_f32(128, C);
       constexpr uint32_t id_mn = idesc_bf16_f32(128, DV) | kBMn;
@@ -448,6 +464,14 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       int kt = 0, kt_round = 0;            // place in the ring of quarter blocks
       const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
       const uint32_t dq = k_desc(sm + M::kQ), ds = mn_desc(sm + M::kS, DK * 128);
+      int f_in = 0, f_nt = 0;
+      auto facts = [&](int i) {
+        const int r = i % kRing;
+        wait(&b->gfull[r], i / kRing);
+        f_in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
+        f_nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0);
+        if (lane == 0) mbar_arrive(&b->gempty[r]);
+      };
       auto scores = [&](int i) {           // Q K^T of block i
         const uint32_t dks = k_desc(sm + M::kK + (i & 1) * M::kKTile);
         wait(&b->kfull[i & 1], i >> 1);
@@ -460,23 +484,19 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             mma_ss(tmem + kSC, dq + off, dks + off, id_qk, ks > 0);
           }
           mma_commit(&b->sc_done);
-          mma_commit(&b->kempty[i & 1]);
         }
         __syncwarp();
+        facts(i);
       };
 #pragma unroll 1
-      for (int i = STATE ? 0 : -1; i < nblk; ++i) {
+      for (int i = -1; i < nblk; ++i) {
         // a block: W V of two quarters | Q S | W V of the other two | P V | the next block's Q K^T, so that
         // P, the scaling of O and the state's update go on beside products
         if (i >= 0) {
-          const int s = i & 1, r = i % kRing;
+          const int s = i & 1;
           const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
-          wait(&b->gfull[r], i / kRing);
-          const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
-          const int nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0);
-          const int quarters = (nt + 31) / 32;
+          const int in = f_in, nt = f_nt, quarters = (nt + 31) / 32;
           if (aborted()) break;
-          if (lane == 0) mbar_arrive(&b->gempty[r]);
           wait(&b->vfull[s], i >> 1);
           if (!STATE && nt < C) wait(&b->p_ready, i);       // V's rows past the end are zeroed by then
           if (const int f = i - (STATE ? 2 : 1); f >= 0) wait(&b->u_free[f & 1], f >> 1);
@@ -490,8 +510,8 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 const uint32_t dvq = dvs + qt * (4096 >> 4), ta = tmem + kKT + 64 * kt, td = tmem + u_cols<STATE>(i);
 #pragma unroll
                 for (int part = 3; part >= 0; --part) {
-                  mma_ts(td, ta + 16 * part, dvq, id_mn, part < 3 || qt > 0);
-                  mma_ts(td, ta + 16 * part + 8, dvq + (2048 >> 4), id_mn, 1);
+                  mma_ts(td, ta + 8 * part, dvq, id_mn, part < 3 || qt > 0);
+                  mma_ts(td, ta + 8 * part + 32, dvq + (2048 >> 4), id_mn, 1);
                 }
                 mma_commit(&b->kt_free[kt]);
                 if (qt + 1 == quarters) {
@@ -516,8 +536,6 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 }
                 __syncwarp();
               }
-              if (elect()) mma_commit(&b->qempty);
-              __syncwarp();
             }
           }
           if constexpr (!STATE) {
@@ -537,6 +555,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           }
         }
         if (!STATE && i + 1 < nblk) scores(i + 1);
+        if (STATE && i + 1 < nblk) facts(i + 1);
       }
       // products in flight still read shared memory and TMEM
       if (elect()) mma_commit(&b->drain);
@@ -672,6 +691,10 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (aborted()) break;
         const Block& k = b->blk[r];
         wait(&b->sc_done, i);
+        if (lane == 0) {
+          mbar_arrive(&b->kempty[s]);      // Q K^T is done with K, and with Q unless Q S is to come
+          if (!in) mbar_arrive(&b->qempty);
+        }
         tc_fence_after();
         float x = rs;                      // log2 of the decay from the end of 32 c to the row
         // rolled loops: the roles' code has to stay in the instruction cache together
@@ -742,6 +765,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         if (in) {
           wait(&b->qs_done, n_in);
+          if (lane == 0) mbar_arrive(&b->qempty);
           ++n_in;
           tc_fence_after();
           const float f = ex2(rs) * a.scale;
@@ -815,15 +839,15 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     }
   } else if (warp < 12) {
     // ---------------------------------------------------------------- transposed, decayed keys
-    // a thread has one column k of the keys, 16 tokens at a time and two to a word: the products k w of
-    // bf16 numbers in four parts that add up to all their bits. k w1 is its rounding plus an exact rest
-    // (16 bits), k w2 the same with k w3.
-    const int q = warp & 3, k0 = 32 * q + lane;
-    const bool live = k0 < DK;
-    const int kc = live ? k0 : k0 - DK;          // dk = 64: the upper lanes are zeros
+    // A warp has 32 columns k of the keys, 16 tokens at a time and two to a word: transposed loads give
+    // a thread columns t / 4, + 8, + 16, + 24 and tokens 2 (t % 4), + 1, + 8, + 9. The products k w of
+    // bf16 numbers come in four parts that add up to all their bits: k w1 is its rounding plus an exact
+    // rest (16 bits), k w2 the same with k w3.
+    const int q = warp & 3;
+    const bool live = 32 * q < DK;               // dk = 64: the upper lanes are zeros
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + kKT;
-    const uint8_t* col0 = smem + M::kK + (kc / 64) * C * 128 + (kc & 7) * 2;
-    const int ch = (kc % 64) / 8;
+    const uint32_t col0 = smem_u32(smem) + M::kK + (live ? q / 2 : 0) * C * 128 + (lane & 7) * 128 +
+                          (((4 * (q & 1) + (lane >> 3)) ^ (lane & 7)) << 4);
     int kt = 0, kt_round = 0;                    // place in the ring of quarter blocks
 #pragma unroll 1
     for (int i = 0; i < nblk; ++i) {
@@ -834,44 +858,44 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const Block& k = b->blk[r];
       const int nt = k.nt, units = (nt + 31) / 32 * 2;
       const int from = live ? nt : 0;            // tokens from here on count as zeros, whatever they hold
+      const uint32_t col = col0 + s * M::kKTile;
+      uint32_t x[2][4];
+      ldsm_t(col, x[0]);
+      ldsm_t(col + 1024, x[1]);
 #pragma unroll 1
       for (int c = 0; c < units; ++c) {
-        const uint8_t* col = col0 + s * M::kKTile + c * 2048;
-        uint32_t x[8], p0[8], p1[8], p2[8], p3[8];
+        if (16 * c + 16 > from) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t x0 = *reinterpret_cast<const uint16_t*>(col + 256 * e + ((ch ^ (2 * e & 7)) << 4));
-          const uint32_t x1 = *reinterpret_cast<const uint16_t*>(col + 256 * e + 128 + ((ch ^ ((2 * e + 1) & 7)) << 4));
-          x[e] = __byte_perm(x0, x1, 0x5410);
-        }
-        const int j0 = 16 * c;
-        if (j0 + 16 > from) {
+          for (int h = 0; h < 2; ++h) {
+            const int j = 16 * c + 8 * h + 2 * (lane & 3);
+            const uint32_t keep = (j < from ? 0xFFFFu : 0u) | (j + 1 < from ? 0xFFFF0000u : 0u);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] &= (j0 + 2 * e < from ? 0xFFFFu : 0u) | (j0 + 2 * e + 1 < from ? 0xFFFF0000u : 0u);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(&k.w[0][j0 / 2 + e]), v = *reinterpret_cast<const uint4*>(&k.w[1][j0 / 2 + e]),
-                      t = *reinterpret_cast<const uint4*>(&k.w[2][j0 / 2 + e]);
-          const uint32_t w1[4] = {u.x, u.y, u.z, u.w}, w2[4] = {v.x, v.y, v.z, v.w}, w3[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-          for (int f = 0; f < 4; ++f) {
-            p0[e + f] = bf2_mul(x[e + f], w1[f]);
-            p1[e + f] = bf2_fma(x[e + f], w1[f], bf2_neg(p0[e + f]));
-            p2[e + f] = bf2_mul(x[e + f], w2[f]);
-            p3[e + f] = bf2_fma(x[e + f], w3[f], bf2_fma(x[e + f], w2[f], bf2_neg(p2[e + f])));
+            for (int e = 0; e < 4; ++e) x[h][e] &= keep;
           }
         }
-        if (!(c & 1) && kt_round) {
-          wait(&b->kt_free[kt], kt_round - 1);
-          tc_fence_after();
+        uint32_t p[2][16];                       // lanes 0..15 and 16..31: [part][8 tokens][8 columns]
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = 8 * c + 4 * h + (lane & 3);
+          const uint32_t w1 = k.w[0][j], w2 = k.w[1][j], w3 = k.w[2][j];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t* o = &p[e / 2][2 * h + e % 2];
+            o[0] = bf2_mul(x[h][e], w1);
+            o[4] = bf2_fma(x[h][e], w1, bf2_neg(o[0]));
+            o[8] = bf2_mul(x[h][e], w2);
+            o[12] = bf2_fma(x[h][e], w3, bf2_fma(x[h][e], w2, bf2_neg(o[8])));
+          }
         }
-        const uint32_t at = trow + 64 * kt + 8 * (c & 1);
-        tmem_st8(at, p0);
-        tmem_st8(at + 16, p1);
-        tmem_st8(at + 32, p2);
-        tmem_st8(at + 48, p3);
+        if (c + 1 < units) {
+          ldsm_t(col + (c + 1) * 2048, x[0]);
+          ldsm_t(col + (c + 1) * 2048 + 1024, x[1]);
+        }
+        if (!(c & 1) && kt_round) wait(&b->kt_free[kt], kt_round - 1);
+        tc_fence_after();
+        const uint32_t at = trow + 64 * kt + 32 * (c & 1);
+        tmem_st_frag(at, p[0]);
+        tmem_st_frag(at + (16u << 16), p[1]);
         if (c & 1) {
           tmem_wait_st();
           tc_fence_before();
