@@ -61,94 +61,133 @@ AIR_DEVICE bool seq_init(const LinAttnArgs& a, int n) {
   return a.has_state ? a.has_state[n] != 0 : a.has_state_all != 0;
 }
 
+constexpr int kSort = 32;          // so many sequences are put in order of their length
 struct Range {
   Pos begin, end;                  // end: one past the last block, as the position of the next one
   int blocks;                      // blocks of the range
-  int cut_begin, cut_end;          // the range starts / ends inside an item
-  int tail;                        // blocks of the last piece when cut_end
+  int whole;                       // whole items, dealt out in turns, instead of a stretch of the list
+  int cut_end, tail;               // the stretch ends inside an item; blocks of that last piece
 };
+// The sequence of item t, and the item that CTA r of R gets in turn k: forth and back over the CTAs.
+AIR_DEVICE int item_seq(const LinAttnArgs& a, const int* order, int t) { return a.N <= kSort ? order[t / a.H] : t / a.H; }
+AIR_DEVICE int item_of(int k, int r, int R) { return k * R + (k & 1 ? R - 1 - r : r); }
 
-// The position of list index p (warp-wide), its item's length and the index within the item.
-AIR_DEVICE Pos locate(const LinAttnArgs& a, int p, int total, int& len) {
+// The first position at or after list index p where a stretch may start: p itself inside an item that is
+// cut, else the nearer end of the item (warp-wide). Returns its index. nb, inc: blocks of sequence `lane`
+// and their running sum.
+AIR_DEVICE int snap(const LinAttnArgs& a, int p, int total, int longest, int nb, int inc, Pos& pos) {
   const int lane = threadIdx.x & 31;
-  Pos r{a.N, 0, 0};
-  len = 0;
-  if (p >= total) return r;
-  int base = 0;
-  for (int n0 = 0; n0 < a.N; n0 += 32) {
-    const int nb = n0 + lane < a.N ? seq_blocks(a, n0 + lane) : 0;
-    int inc = nb * a.H;
-#pragma unroll
+  pos = Pos{a.N, 0, 0};
+  if (p >= total) return total;
+  int base = 0, len = 0;
+  for (int n0 = 0;;) {
+    const int all = __shfl_sync(0xffffffffu, inc, 31) * a.H;
+    if (p < base + all) {
+      const int l = __ffs(__ballot_sync(0xffffffffu, base + inc * a.H > p)) - 1;
+      len = __shfl_sync(0xffffffffu, nb, l);
+      const int rel = p - base - (__shfl_sync(0xffffffffu, inc, l) - len) * a.H;
+      pos = Pos{n0 + l, rel / len, rel % len};
+      break;
+    }
+    base += all;
+    n0 += 32;
+    nb = n0 + lane < a.N ? seq_blocks(a, n0 + lane) : 0;
+    inc = nb;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
-    const int all = __shfl_sync(0xffffffffu, inc, 31);
-    if (p < base + all) {
-      const unsigned past = __ballot_sync(0xffffffffu, base + inc > p);
-      const int l = __ffs(past) - 1;
-      const int before = l ? __shfl_sync(0xffffffffu, inc, l ? l - 1 : 0) : 0;
-      len = __shfl_sync(0xffffffffu, nb, l);
-      const int rel = p - base - before;
-      r.n = n0 + l;
-      r.h = rel / len;
-      r.c = rel % len;
-      return r;
-    }
-    base += all;
   }
-  return r;
+  if (pos.c == 0 || len > longest) return p;
+  const int c = pos.c;
+  pos.c = 0;
+  if (2 * c < len) return p - c;
+  if (++pos.h == a.H) {
+    pos.h = 0;
+    do { ++pos.n; } while (pos.n < a.N && seq_len(a, pos.n) == 0);
+  }
+  return p + len - c;
 }
 
-// The first position at or after list index p where a range may start: p itself inside an item that
-// is cut, else the nearer end of the item (warp-wide). Index and position.
-AIR_DEVICE Pos snap(const LinAttnArgs& a, int p, int total, int longest, int& at) {
-  int len;
-  at = p < total ? p : total;
-  Pos r = locate(a, p, total, len);
-  if (r.c == 0 || r.n >= a.N || len > longest) return r;
-  at += 2 * r.c < len ? -r.c : len - r.c;
-  return locate(a, at, total, len);
-}
-
-__device__ __noinline__ Range make_range(const LinAttnArgs& a, int r, int R) {
+// What CTA r of R works on (warp-wide; order: shared memory for kSort entries).
+__device__ __noinline__ Range make_range(const LinAttnArgs& a, int r, int R, int* order) {
   const int lane = threadIdx.x & 31;
-  int total = 0;
-  int most = 0;
-  for (int n = lane; n < a.N; n += 32) {
-    const int nb = seq_blocks(a, n);
-    total += nb;
-    most = max(most, nb);
+  const int nb = lane < a.N ? seq_blocks(a, lane) : 0;
+  int total = nb, most = nb;
+  for (int n = lane + 32; n < a.N; n += 32) {
+    const int x = seq_blocks(a, n);
+    total += x;
+    most = max(most, x);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total = __reduce_add_sync(0xffffffffu, total) * a.H;
   most = __reduce_max_sync(0xffffffffu, most);
-  total *= a.H;
+  Range g{};
   int per = (total + R - 1) / R;
   const int longest = 2 * max(per, kMinCut);
-  if (most > longest && per < kMinCut) per = kMinCut;
-  Range g;
-  int i0, i1;
-  g.begin = snap(a, min(r * (int64_t)per, (int64_t)total), total, longest, i0);
-  g.end = snap(a, min((r + 1) * (int64_t)per, (int64_t)total), total, longest, i1);
+  if (most <= longest) {
+    // no item is worth a cut: the longest first, so that the turns even out
+    g.whole = 1;
+    if (a.N <= kSort) {
+      int rank = 0;
+      for (int m = 0; m < a.N; ++m) {
+        const int x = __shfl_sync(0xffffffffu, nb, m);
+        rank += x > nb || (x == nb && m < lane);
+      }
+      if (lane < a.N) order[rank] = lane;
+      __syncwarp();
+    }
+    int blocks = 0;
+    for (int k = lane; k * (int64_t)R < (int64_t)a.N * a.H; k += 32) {
+      const int t = item_of(k, r, R);
+      if (t < a.N * a.H) blocks += seq_blocks(a, item_seq(a, order, t));
+    }
+    g.blocks = __reduce_add_sync(0xffffffffu, blocks);
+    return g;
+  }
+  per = max(per, kMinCut);
+  int inc = nb;
+#pragma unroll 1
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  const int64_t p0 = (int64_t)r * per, p1 = p0 + per;
+  const int i0 = snap(a, (int)min(p0, (int64_t)total), total, longest, nb, inc, g.begin);
+  const int i1 = snap(a, (int)min(p1, (int64_t)total), total, longest, nb, inc, g.end);
   g.blocks = i1 - i0;
-  g.cut_begin = g.blocks > 0 && g.begin.c > 0;
   g.cut_end = g.blocks > 0 && g.end.n < a.N && g.end.c > 0;
   g.tail = g.cut_end ? min(g.blocks, g.end.c) : 0;
   return g;
 }
 
-// Walks blocks of the list in order.
+// Walks the blocks of a range in order.
 struct Walk {
   const LinAttnArgs& a;
+  const int* order;
   Pos p;
-  int nb, t0, len;
-  AIR_DEVICE Walk(const LinAttnArgs& args, const Pos& begin) : a(args), p(begin) { load(); }
+  int nb, t0, len, turn, whole;
+  AIR_DEVICE Walk(const LinAttnArgs& args, const int* ord, const Pos& begin, int dealt)
+      : a(args), order(ord), p(begin), nb(0), turn(-1), whole(dealt) {
+    if (whole) deal();
+    else load();
+  }
   AIR_DEVICE void load() {
-    if (p.n < a.N) {
-      t0 = seq_begin(a, p.n);
-      len = seq_len(a, p.n);
-      nb = (len + C - 1) / C;
+    nb = 0;
+    if (p.n >= a.N) return;
+    t0 = seq_begin(a, p.n);
+    len = seq_len(a, p.n);
+    nb = (len + C - 1) / C;
+  }
+  AIR_DEVICE void deal() {
+    for (p.c = 0;;) {
+      const int t = item_of(++turn, blockIdx.x, gridDim.x);
+      if (turn * (int64_t)gridDim.x >= (int64_t)a.N * a.H) return;
+      if (t >= a.N * a.H) continue;
+      p.n = item_seq(a, order, t);
+      p.h = t % a.H;
+      load();
+      if (nb > 0) return;
     }
   }
   AIR_DEVICE int token() const { return t0 + p.c * C; }
@@ -156,6 +195,7 @@ struct Walk {
   AIR_DEVICE bool last() const { return p.c + 1 == nb; }
   AIR_DEVICE void next() {
     if (++p.c < nb) return;
+    if (whole) return deal();
     p.c = 0;
     if (++p.h < a.H) return;
     p.h = 0;
@@ -329,13 +369,14 @@ struct alignas(16) Block {
   float* dst;                      // where S goes after the block (null: nowhere)
 };
 struct Bars {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], gfull[kRing], gempty[kRing];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], dfull[kRing], gfull[kRing], gempty[kRing];
   uint64_t qfull, qempty;
   uint64_t sc_done, qs_done, o_done, p_ready, o_scaled, o_free, s_ready, drain;
   uint64_t u_done[2], u_free[2], kt_ready[2], kt_free[2];   // pairs: the waiting side may be two phases behind
   uint32_t tmem;
   int abort;
   Range range;
+  int order[kSort];
   Block blk[kRing];
 };
 
@@ -366,7 +407,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == 2) {
-    const Range g = make_range(a, blockIdx.x, gridDim.x);
+    const Range g = make_range(a, blockIdx.x, gridDim.x, b->order);
     if (lane == 0) b->range = g;
   }
   if (warp == 3 && lane == 0) {
@@ -378,7 +419,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b->kfull[i], 1);
-      mbar_init(&b->kempty[i], STATE ? 4 : 8);
+      mbar_init(&b->kempty[i], 8);
       mbar_init(&b->vfull[i], 1);
       mbar_init(&b->vempty[i], STATE ? 1 : 4);
       mbar_init(&b->kt_ready[i], 4);
@@ -387,8 +428,9 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&b->u_free[i], 8);
     }
     for (int i = 0; i < kRing; ++i) {
+      mbar_init(&b->dfull[i], 1);
       mbar_init(&b->gfull[i], 1);
-      mbar_init(&b->gempty[i], STATE ? 14 : 18);
+      mbar_init(&b->gempty[i], 18);
     }
     mbar_init(&b->qfull, 1);
     mbar_init(&b->qempty, 4);
@@ -402,6 +444,14 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     mbar_init(&b->drain, 1);
     b->abort = 0;
     fence_mbar_init();
+  }
+  if constexpr (STATE) {
+    // most ranges of most calls have nothing to do here
+    __syncthreads();
+    if (b->range.tail == 0) {
+      if (threadIdx.x == 0) ws_meta[blockIdx.x * 2].x = 0;
+      return;
+    }
   }
   if (warp == 1) tmem_alloc(&b->tmem, 512);
   tc_fence_before();
@@ -421,7 +471,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll 1
         for (int i = 0; i < nblk; ++i) {
           const int s = i & 1, u = i >> 1, r = i % kRing;
-          wait(&b->gfull[r], i / kRing);
+          wait(&b->dfull[r], i / kRing);
           if (i >= 2) {
             wait(&b->kempty[s], u - 1);
             wait(&b->vempty[s], u - 1);
@@ -565,7 +615,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       // -------------------------------------------------------------- decays and descriptions
       // lane l: tokens 4l .. 4l + 3; eight lanes make one of the four 32s
       const Range rg = b->range;
-      Walk w(a, STATE ? Pos{rg.end.n, rg.end.h, rg.end.c - rg.tail} : rg.begin);
+      Walk w(a, b->order, STATE ? Pos{rg.end.n, rg.end.h, rg.end.c - rg.tail} : rg.begin, rg.whole);
       if (STATE && lane == 0) {
         ws_meta[blockIdx.x * 2] = make_int4(rg.cut_end, 0, w.p.c == 0, w.p.n);
         ws_meta[blockIdx.x * 2 + 1].x = w.p.h;
@@ -582,46 +632,8 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         if (i >= kRing) wait(&b->gempty[r], i / kRing - 1);
         if (aborted()) break;
-        float pre[4], suf[4];              // inclusive sums up to, exclusive sums after each token, in the 32
-        pre[0] = g[0]; pre[1] = pre[0] + g[1]; pre[2] = pre[1] + g[2]; pre[3] = pre[2] + g[3];
-        suf[3] = 0.f; suf[2] = g[3]; suf[1] = suf[2] + g[2]; suf[0] = suf[1] + g[1];
-        float up = pre[3], down = suf[0] + g[0];
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-          const float x = __shfl_up_sync(0xffffffffu, up, o, 8), y = __shfl_down_sync(0xffffffffu, down, o, 8);
-          if ((lane & 7) >= o) up += x;
-          if ((lane & 7) + o < 8) down += y;
-        }
-        float after = __shfl_down_sync(0xffffffffu, down, 1, 8), bef = __shfl_up_sync(0xffffffffu, up, 1, 8);
-        if ((lane & 7) == 7) after = 0.f;
-        if ((lane & 7) == 0) bef = 0.f;
-        const float t[4] = {__shfl_sync(0xffffffffu, up, 7), __shfl_sync(0xffffffffu, up, 15),
-                            __shfl_sync(0xffffffffu, up, 23), __shfl_sync(0xffffffffu, up, 31)};
-        float later = 0.f;                 // the 32s after this one
-#pragma unroll
-        for (int q = 3; q > 0; --q)
-          if (lane / 8 < q) later += t[q];
         Block& k = b->blk[r];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = 4 * lane + e;
-          k.gl[j] = (bef + pre[e]) * kLog2e;
-          k.e[j] = ex2((suf[e] + after) * kLog2e);
-          float w = j < nt ? expf(suf[e] + after + later) : 0.f;
-#pragma unroll
-          for (int p = 0; p < 3; ++p) {
-            const __nv_bfloat16 h = f2bf(w);
-            reinterpret_cast<__nv_bfloat16*>(k.w[p])[j] = h;
-            w -= bf2f(h);
-          }
-        }
-        const float total = (t[3] + t[2]) + (t[1] + t[0]);
-        if (lane < 4) k.t2[lane] = (lane == 0 ? t[0] : lane == 1 ? t[1] : lane == 2 ? t[2] : t[3]) * kLog2e;
-        if (lane == 0) {
-          const bool slow = total > -0.5f;
-          k.f = slow ? expm1f(total) : expf(total);
-          k.one = slow ? 1.f : 0.f;
-          total_piece += total;
+        if (lane == 0) {                   // what the copies need does not wait for the decays
           k.tok = t0;
           k.nt = nt;
           k.h = w.p.h;
@@ -648,6 +660,47 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             }
             if (w.last()) k.dst = row;
           }
+          mbar_arrive(&b->dfull[r]);
+        }
+        float pre[4], suf[4];              // inclusive sums up to, exclusive sums after each token, in the 32
+        pre[0] = g[0]; pre[1] = pre[0] + g[1]; pre[2] = pre[1] + g[2]; pre[3] = pre[2] + g[3];
+        suf[3] = 0.f; suf[2] = g[3]; suf[1] = suf[2] + g[2]; suf[0] = suf[1] + g[1];
+        float up = pre[3], down = suf[0] + g[0];
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          const float x = __shfl_up_sync(0xffffffffu, up, o, 8), y = __shfl_down_sync(0xffffffffu, down, o, 8);
+          if ((lane & 7) >= o) up += x;
+          if ((lane & 7) + o < 8) down += y;
+        }
+        float after = __shfl_down_sync(0xffffffffu, down, 1, 8), bef = __shfl_up_sync(0xffffffffu, up, 1, 8);
+        if ((lane & 7) == 7) after = 0.f;
+        if ((lane & 7) == 0) bef = 0.f;
+        const float t[4] = {__shfl_sync(0xffffffffu, up, 7), __shfl_sync(0xffffffffu, up, 15),
+                            __shfl_sync(0xffffffffu, up, 23), __shfl_sync(0xffffffffu, up, 31)};
+        float later = 0.f;                 // the 32s after this one
+#pragma unroll
+        for (int q = 3; q > 0; --q)
+          if (lane / 8 < q) later += t[q];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * lane + e;
+          k.gl[j] = (bef + pre[e]) * kLog2e;
+          k.e[j] = ex2((suf[e] + after) * kLog2e);
+          float w = j < nt ? expf(suf[e] + after + later) : 0.f;
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            const __nv_bfloat16 h = f2bf(w);
+            reinterpret_cast<__nv_bfloat16*>(k.w[p])[j] = h;
+            w -= bf2f(h);
+          }
+        }
+        const float total = (t[3] + t[2]) + (t[1] + t[0]);
+        if (lane < 4) k.t2[lane] = (lane == 0 ? t[0] : lane == 1 ? t[1] : lane == 2 ? t[2] : t[3]) * kLog2e;
+        if (lane == 0) {
+          const bool slow = total > -0.5f;
+          k.f = slow ? expm1f(total) : expf(total);
+          k.one = slow ? 1.f : 0.f;
+          total_piece += total;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&b->gfull[r]);
@@ -665,7 +718,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         for (int64_t x = lane; x < (int64_t)a.H * DV * DK / 4; x += 32) dst[x] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < 8 && !STATE) {
     // ---------------------------------------------------------------- scores -> P, O -> out
     if constexpr (!STATE) {
       const int q = warp & 3, row = 32 * q + lane;
@@ -848,7 +901,10 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + kKT;
     const uint32_t col0 = smem_u32(smem) + M::kK + (live ? q / 2 : 0) * C * 128 + (lane & 7) * 128 +
                           (((4 * (q & 1) + (lane >> 3)) ^ (lane & 7)) << 4);
-    int kt = 0, kt_round = 0;                    // place in the ring of quarter blocks
+    // In the state-only kernel (full blocks) the output warps share the work: the second quarters of two.
+    constexpr int kStep = STATE ? 2 : 1;
+    const int mine = STATE && warp < 8;
+    int kt = mine, kt_round = 0;                 // place in the ring of quarter blocks
 #pragma unroll 1
     for (int i = 0; i < nblk; ++i) {
       const int s = i & 1, r = i % kRing;
@@ -860,10 +916,11 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const int from = live ? nt : 0;            // tokens from here on count as zeros, whatever they hold
       const uint32_t col = col0 + s * M::kKTile;
       uint32_t x[2][4];
-      ldsm_t(col, x[0]);
-      ldsm_t(col + 1024, x[1]);
+      ldsm_t(col + mine * 4096, x[0]);
+      ldsm_t(col + mine * 4096 + 1024, x[1]);
 #pragma unroll 1
-      for (int c = 0; c < units; ++c) {
+      for (int c = 2 * mine; c < units;) {
+        const int next = c & 1 ? c + 2 * kStep - 1 : c + 1;
         if (16 * c + 16 > from) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -887,9 +944,9 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             o[12] = bf2_fma(x[h][e], w3, bf2_fma(x[h][e], w2, bf2_neg(o[8])));
           }
         }
-        if (c + 1 < units) {
-          ldsm_t(col + (c + 1) * 2048, x[0]);
-          ldsm_t(col + (c + 1) * 2048 + 1024, x[1]);
+        if (next < units) {
+          ldsm_t(col + next * 2048, x[0]);
+          ldsm_t(col + next * 2048 + 1024, x[1]);
         }
         if (!(c & 1) && kt_round) wait(&b->kt_free[kt], kt_round - 1);
         tc_fence_after();
@@ -901,8 +958,10 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&b->kt_ready[kt]);
-          if (++kt == 2) kt = 0, ++kt_round;
+          if (STATE || kt) ++kt_round;
+          if (!STATE) kt ^= 1;
         }
+        c = next;
       }
       if (lane == 0) {
         mbar_arrive(&b->kempty[s]);

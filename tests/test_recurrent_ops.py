@@ -110,6 +110,33 @@ def test_prompts_match_the_recurrence(case, dtype, per_token):
 
 
 @gpu
+@pytest.mark.parametrize("N", [32, 33, 70])
+def test_many_sequences_in_one_call(N):
+    """More sequences than a warp has lanes, empty ones among them, with and without one that is long
+    enough to be split."""
+    H, d = 3, 64
+    r = torch.Generator().manual_seed(N)
+    lens = torch.randint(0, 90, (N,), generator=r).tolist()
+    lens[5] = lens[-1] = 0
+    if N == 70:
+        lens[40] = 2900
+    T = sum(lens)
+    q, k, v, g = _inputs(N, T, H, H, H, H, d, d, torch.bfloat16)
+    pool = torch.randn(N, H, d, d, generator=r)
+    has = torch.randint(0, 2, (N,), generator=r)
+    ref, st, mag, sm = _oracle(q, k, v, g, lens, pool * has[:, None, None, None], 0.125)
+    dpool = pool.to(DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device=DEV)
+    out = ops.linear_attention(q.to(DEV), k.to(DEV), v.to(DEV), g.to(DEV), state=dpool, cu_seqlens=cu,
+                               has_state=has.to(torch.int32).to(DEV), err=err)
+    assert int(err) == 0
+    co, cs = _c(max(lens), d, True)
+    _near(out, ref, mag, co, True)
+    _near(dpool, st, sm, cs, False)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_prompt_without_state_and_defaults(dtype):
     q, k, v, g = _inputs(5, 200, 2, 2, 2, 2, 64, 64, dtype)
