@@ -371,8 +371,8 @@ struct alignas(16) Block {
 struct Bars {
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], dfull[kRing], gfull[kRing], gempty[kRing];
   uint64_t qfull, qempty;
-  uint64_t sc_done, qs_done, o_done, p_ready, o_scaled, o_free, s_ready, drain;
-  uint64_t u_done[2], u_free[2], kt_ready[2], kt_free[2];   // pairs: the waiting side may be two phases behind
+  uint64_t sc_done, qs_done, o_done, o_scaled, o_free, o_staged, s_ready, drain[2];
+  uint64_t p_ready[2], u_done[2], u_free[2], kt_ready[2], kt_free[2];   // pairs: the waiting side may be two phases behind
   uint32_t tmem;
   int abort;
   Range range;
@@ -380,7 +380,8 @@ struct Bars {
   Block blk[kRing];
 };
 
-// 20 warps: 4 of service (copies, products, decays, empty sequences), 4 of output, 4 of keys, 8 of state
+// 20 warps: 4 of service (products of the output, copies, decays, products of the state), 4 of output, 4 of
+// keys, 8 of state.
 constexpr int kThreads = 640;
 AIR_DEVICE bool elect() {
   uint32_t p;
@@ -421,27 +422,28 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&b->kfull[i], 1);
       mbar_init(&b->kempty[i], 8);
       mbar_init(&b->vfull[i], 1);
-      mbar_init(&b->vempty[i], STATE ? 1 : 4);
+      mbar_init(&b->vempty[i], 1);
       mbar_init(&b->kt_ready[i], 4);
       mbar_init(&b->kt_free[i], 1);
+      mbar_init(&b->drain[i], 1);
+      mbar_init(&b->p_ready[i], 4);
       mbar_init(&b->u_done[i], 1);
       mbar_init(&b->u_free[i], 8);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&b->dfull[i], 1);
       mbar_init(&b->gfull[i], 1);
-      mbar_init(&b->gempty[i], 18);
+      mbar_init(&b->gempty[i], STATE ? 18 : 19);
     }
     mbar_init(&b->qfull, 1);
     mbar_init(&b->qempty, 4);
     mbar_init(&b->sc_done, 1);
     mbar_init(&b->qs_done, 1);
     mbar_init(&b->o_done, 1);
-    mbar_init(&b->p_ready, 4);
     mbar_init(&b->o_scaled, 4);
     mbar_init(&b->o_free, 4);
     mbar_init(&b->s_ready, 8);
-    mbar_init(&b->drain, 1);
+    mbar_init(&b->o_staged, 4);
     b->abort = 0;
     fence_mbar_init();
   }
@@ -460,34 +462,50 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const uint32_t tmem = __shfl_sync(0xffffffffu, b->tmem, 0);
   const int nblk = __shfl_sync(0xffffffffu, STATE ? b->range.tail : b->range.blocks, 0);
   auto wait = [&](uint64_t* bar, int parity) { bar_wait(bar, parity, &b->abort); };
+  constexpr uint32_t id_mn = idesc_bf16_f32(128, DV) | kBMn;
   auto aborted = [&] { return *(volatile int*)&b->abort != 0; };
 
   if (warp < 4) {
     if (warp == 1) {
-      // -------------------------------------------------------------- TMA producer
+      // -------------------------------------------------------------- copies
       if (lane == 0) {
         const uint32_t sm = smem_u32(smem);
-        int issued = 0, q_issued = 0;
+        int k_issued = 0, v_issued = 0, q_issued = 0;
+        int h0 = 0, tok0 = 0, rows0 = 0, h1 = 0, tok1 = 0, rows1 = 0;    // the two blocks before
+        // the output of a block out of V's tile, of which it took the place
+        auto out = [&](int i, int h, int tok, int rows) {
+          wait(&b->o_staged, i);
+          if (aborted()) return;
+#pragma unroll 1
+          for (int x = 0; x < rows; x += 32)
+#pragma unroll
+            for (int c = 0; c < DV / 64; ++c)
+              tma_store_3d(&tm_o, smem + M::kV + (i & 1) * M::kVTile + c * C * 128 + x * 128, 64 * c, h, tok + x);
+          tma_store_wait<true>();
+        };
 #pragma unroll 1
         for (int i = 0; i < nblk; ++i) {
           const int s = i & 1, u = i >> 1, r = i % kRing;
           wait(&b->dfull[r], i / kRing);
-          if (i >= 2) {
-            wait(&b->kempty[s], u - 1);
-            wait(&b->vempty[s], u - 1);
-          }
-          if (aborted()) break;
-          const int z = b->blk[r].tok, hq = b->blk[r].hq, hk = b->blk[r].hk, hv = b->blk[r].hv;
+          const int z = b->blk[r].tok, h = b->blk[r].h, nt = b->blk[r].nt, hq = b->blk[r].hq, hk = b->blk[r].hk, hv = b->blk[r].hv;
           mbar_arrive(&b->gempty[r]);
+          if (i >= 2) wait(&b->kempty[s], u - 1);
+          if (aborted()) break;
           mbar_expect_tx(&b->kfull[s], M::kKTile);
-          mbar_expect_tx(&b->vfull[s], M::kVTile);
 #pragma unroll
           for (int p = 0; p < DK / 64; ++p)
             tma_load_3d(sm + M::kK + s * M::kKTile + p * C * 128, &tm_k, &b->kfull[s], 64 * p, hk, z);
+          ++k_issued;
+          if (i >= 2) {
+            if constexpr (STATE) wait(&b->vempty[s], u - 1);
+            else out(i - 2, h0, tok0, rows0);
+          }
+          if (aborted()) break;
+          mbar_expect_tx(&b->vfull[s], M::kVTile);
 #pragma unroll
           for (int p = 0; p < DV / 64; ++p)
             tma_load_3d(sm + M::kV + s * M::kVTile + p * C * 128, &tm_v, &b->vfull[s], 64 * p, hv, z);
-          issued = i + 1;
+          ++v_issued;
           if constexpr (!STATE) {
             if (i >= 1) wait(&b->qempty, i - 1);
             if (aborted()) break;
@@ -496,121 +514,139 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             for (int p = 0; p < DK / 64; ++p) tma_load_3d(sm + M::kQ + p * C * 128, &tm_q, &b->qfull, 64 * p, hq, z);
             ++q_issued;
           }
+          h0 = h1, tok0 = tok1, rows0 = rows1;
+          h1 = h, tok1 = z, rows1 = nt & ~31;
         }
         // never leave the CTA with copies in flight into its shared memory
-        for (int i = max(0, issued - 2); i < issued; ++i) {
-          bar_drain(&b->kfull[i & 1], i >> 1);
-          bar_drain(&b->vfull[i & 1], i >> 1);
-        }
+        for (int i = max(0, k_issued - 2); i < k_issued; ++i) bar_drain(&b->kfull[i & 1], i >> 1);
+        for (int i = max(0, v_issued - 2); i < v_issued; ++i) bar_drain(&b->vfull[i & 1], i >> 1);
         if (q_issued) bar_drain(&b->qfull, q_issued - 1);
+        if (!STATE && !aborted()) {
+          if (nblk > 1) out(nblk - 2, h0, tok0, rows0);
+          if (nblk > 0) out(nblk - 1, h1, tok1, rows1);
+        }
+        tma_store_wait<false>();
+      }
+      __syncwarp();
+      if constexpr (!STATE) {
+        // empty sequences keep their state, or zeros when they are fresh
+        for (int n = blockIdx.x; n < a.N; n += gridDim.x) {
+          if (seq_len(a, n) > 0 || seq_init(a, n)) continue;
+          const int64_t slot = seq_slot(a, n);
+          if (slot < 0) continue;
+          float4* dst = reinterpret_cast<float4*>(a.state + (size_t)slot * a.H * DV * DK);
+          for (int64_t x = lane; x < (int64_t)a.H * DV * DK / 4; x += 32) dst[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
       }
     } else if (warp == 0) {
-      // -------------------------------------------------------------- MMA issuer
-      // (on the scheduler of the output warp with the least to do)
-      // the whole warp walks and waits, so that operands stay in uniform registers; one lane issues
-      constexpr uint32_t id_qk = idesc_bf16_f32(128, C);
-      constexpr uint32_t id_mn = idesc_bf16_f32(128, DV) | kBMn;
-      int n_in = 0;                        // blocks with an incoming state so far
-      int kt = 0, kt_round = 0;            // place in the ring of quarter blocks
-      const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
-      const uint32_t dq = k_desc(sm + M::kQ), ds = mn_desc(sm + M::kS, DK * 128);
-      int f_in = 0, f_nt = 0;
-      auto facts = [&](int i) {
-        const int r = i % kRing;
-        wait(&b->gfull[r], i / kRing);
-        f_in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
-        f_nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0);
-        if (lane == 0) mbar_arrive(&b->gempty[r]);
-      };
-      auto scores = [&](int i) {           // Q K^T of block i
-        const uint32_t dks = k_desc(sm + M::kK + (i & 1) * M::kKTile);
-        wait(&b->kfull[i & 1], i >> 1);
-        wait(&b->qfull, i);
-        tc_fence_after();
-        if (elect()) {
-#pragma unroll
-          for (int ks = 0; ks < DK / 16; ++ks) {
-            const int off = (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3);
-            mma_ss(tmem + kSC, dq + off, dks + off, id_qk, ks > 0);
-          }
-          mma_commit(&b->sc_done);
-        }
-        __syncwarp();
-        facts(i);
-      };
+      // -------------------------------------------------------------- products of the output
+      // The whole warp walks and waits, so that operands stay in uniform registers; one lane issues. Q K^T
+      // of the next block goes out behind P V, so that its P is there when its Q S can start.
+      if constexpr (!STATE) {
+        constexpr uint32_t id_qk = idesc_bf16_f32(128, C);
+        int n_in = 0;                      // blocks with an incoming state so far
+        const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+        const uint32_t dq = k_desc(sm + M::kQ), ds = mn_desc(sm + M::kS, DK * 128);
 #pragma unroll 1
-      for (int i = -1; i < nblk; ++i) {
-        // a block: W V of two quarters | Q S | W V of the other two | P V | the next block's Q K^T, so that
-        // P, the scaling of O and the state's update go on beside products
-        if (i >= 0) {
-          const int s = i & 1;
-          const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
-          const int in = f_in, nt = f_nt, quarters = (nt + 31) / 32;
-          if (aborted()) break;
-          wait(&b->vfull[s], i >> 1);
-          if (!STATE && nt < C) wait(&b->p_ready, i);       // V's rows past the end are zeroed by then
-          if (const int f = i - (STATE ? 2 : 1); f >= 0) wait(&b->u_free[f & 1], f >> 1);
-          // U = W V, a quarter of the tokens at a time, the smallest parts first
-#pragma unroll 1
-          for (int qt = 0; qt < 4; ++qt) {
-            if (qt < quarters) {
-              wait(&b->kt_ready[kt], kt_round);
+        for (int i = -1; i < nblk; ++i) {
+          if (i >= 0) {
+            const int s = i & 1, r = i % kRing;
+            const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
+            wait(&b->dfull[r], i / kRing);
+            const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
+            const int steps = __shfl_sync(0xffffffffu, (b->blk[r].nt + 31) / 32 * 2, 0);
+            if (aborted()) break;
+            if (lane == 0) mbar_arrive(&b->gempty[r]);
+            if (in) {
+              // O = Q S
+              wait(&b->s_ready, n_in);
+              if (i >= 1) wait(&b->o_free, i - 1);
               tc_fence_after();
               if (elect()) {
-                const uint32_t dvq = dvs + qt * (4096 >> 4), ta = tmem + kKT + 64 * kt, td = tmem + u_cols<STATE>(i);
 #pragma unroll
-                for (int part = 3; part >= 0; --part) {
-                  mma_ts(td, ta + 8 * part, dvq, id_mn, part < 3 || qt > 0);
-                  mma_ts(td, ta + 8 * part + 32, dvq + (2048 >> 4), id_mn, 1);
-                }
-                mma_commit(&b->kt_free[kt]);
-                if (qt + 1 == quarters) {
-                  mma_commit(&b->u_done[i & 1]);
-                  if (STATE) mma_commit(&b->vempty[s]);     // else the output warps release V
-                }
+                for (int ks = 0; ks < DK / 16; ++ks)
+                  mma_ss(tmem + kO, dq + (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3), ds + ks * (2048 >> 4), id_mn, ks > 0);
+                mma_commit(&b->qs_done);
               }
               __syncwarp();
-              if (++kt == 2) kt = 0, ++kt_round;
             }
-            if (!STATE && qt == 1) {
-              if (in) {
-                // O = Q S
-                wait(&b->s_ready, n_in);
-                if (i >= 1) wait(&b->o_free, i - 1);
-                tc_fence_after();
-                if (elect()) {
-#pragma unroll
-                  for (int ks = 0; ks < DK / 16; ++ks)
-                    mma_ss(tmem + kO, dq + (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3), ds + ks * (2048 >> 4), id_mn, ks > 0);
-                  mma_commit(&b->qs_done);
-                }
-                __syncwarp();
-              }
-            }
-          }
-          if constexpr (!STATE) {
             // O (+)= P V
-            wait(&b->p_ready, i);
+            wait(&b->vfull[s], i >> 1);
+            wait(&b->p_ready[s], i >> 1);
             if (in) wait(&b->o_scaled, n_in);
             else if (i >= 1) wait(&b->o_free, i - 1);
             n_in += in;
             tc_fence_after();
             if (elect()) {
 #pragma unroll 1
-              for (int ks = 0; ks < 2 * quarters; ++ks)
+              for (int ks = 0; ks < steps; ++ks)
                 mma_ts(tmem + kO, tmem + kP + 8 * ks, dvs + ks * (2048 >> 4), id_mn, in || ks > 0);
               mma_commit(&b->o_done);
             }
             __syncwarp();
           }
+          if (i + 1 < nblk) {
+            // scores = Q K^T
+            const uint32_t dks = k_desc(sm + M::kK + ((i + 1) & 1) * M::kKTile);
+            wait(&b->kfull[(i + 1) & 1], (i + 1) >> 1);
+            wait(&b->qfull, i + 1);
+            tc_fence_after();
+            if (elect()) {
+#pragma unroll
+              for (int ks = 0; ks < DK / 16; ++ks) {
+                const int off = (ks / 4) * (C * 128 >> 4) + 2 * (ks & 3);
+                mma_ss(tmem + kSC, dq + off, dks + off, id_qk, ks > 0);
+              }
+              mma_commit(&b->sc_done);
+            }
+            __syncwarp();
+          }
         }
-        if (!STATE && i + 1 < nblk) scores(i + 1);
-        if (STATE && i + 1 < nblk) facts(i + 1);
+        // products in flight still read shared memory and TMEM
+        if (elect()) mma_commit(&b->drain[0]);
+        __syncwarp();
+        bar_drain(&b->drain[0], 0);
       }
-      // products in flight still read shared memory and TMEM
-      if (elect()) mma_commit(&b->drain);
+    } else if (warp == 3) {
+      // -------------------------------------------------------------- products of the state
+      int kt = 0, kt_round = 0;            // place in the ring of quarter blocks
+      const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+#pragma unroll 1
+      for (int i = 0; i < nblk; ++i) {
+        const int s = i & 1, r = i % kRing;
+        const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
+        wait(&b->dfull[r], i / kRing);
+        const int nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0), quarters = (nt + 31) / 32;
+        if (aborted()) break;
+        if (lane == 0) mbar_arrive(&b->gempty[r]);
+        wait(&b->vfull[s], i >> 1);
+        if (!STATE && nt < C) wait(&b->p_ready[s], i >> 1);       // V's rows past the end are zeroed by then
+        if (const int f = i - (STATE ? 2 : 1); f >= 0) wait(&b->u_free[f & 1], f >> 1);
+        // U = W V, a quarter of the tokens at a time, the smallest parts first
+#pragma unroll 1
+        for (int qt = 0; qt < quarters; ++qt) {
+          wait(&b->kt_ready[kt], kt_round);
+          tc_fence_after();
+          if (elect()) {
+            const uint32_t dvq = dvs + qt * (4096 >> 4), ta = tmem + kKT + 64 * kt, td = tmem + u_cols<STATE>(i);
+#pragma unroll
+            for (int part = 3; part >= 0; --part) {
+              mma_ts(td, ta + 8 * part, dvq, id_mn, part < 3 || qt > 0);
+              mma_ts(td, ta + 8 * part + 32, dvq + (2048 >> 4), id_mn, 1);
+            }
+            mma_commit(&b->kt_free[kt]);
+            if (qt + 1 == quarters) {
+              mma_commit(&b->u_done[s]);
+              if (STATE) mma_commit(&b->vempty[s]);     // else V's tile goes on to hold the output
+            }
+          }
+          __syncwarp();
+          if (++kt == 2) kt = 0, ++kt_round;
+        }
+      }
+      if (elect()) mma_commit(&b->drain[1]);
       __syncwarp();
-      bar_drain(&b->drain, 0);
+      bar_drain(&b->drain[1], 0);
     } else if (warp == 2) {
       // -------------------------------------------------------------- decays and descriptions
       // lane l: tokens 4l .. 4l + 3; eight lanes make one of the four 32s
@@ -632,6 +668,13 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         if (i >= kRing) wait(&b->gempty[r], i / kRing - 1);
         if (aborted()) break;
+        if (!STATE && w.p.c == 0 && seq_init(a, w.p.n)) {
+          // the state that a resumed sequence starts from, on its way into L2
+          const int64_t slot = seq_slot(a, w.p.n);
+          const char* row = reinterpret_cast<const char*>(a.state + ((size_t)max(slot, (int64_t)0) * a.H + w.p.h) * DV * DK);
+          if (slot >= 0)
+            for (int x = lane * 128; x < DV * DK * 4; x += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + x));
+        }
         Block& k = b->blk[r];
         if (lane == 0) {                   // what the copies need does not wait for the decays
           k.tok = t0;
@@ -707,16 +750,6 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         w.next();
       }
       if (STATE && lane == 0) ws_meta[blockIdx.x * 2].y = __float_as_int(total_piece);   // the piece's own decay
-    } else if (!STATE) {
-      // -------------------------------------------------------------- empty sequences
-      // they keep their state, or zeros when they are fresh
-      for (int n = blockIdx.x; n < a.N; n += gridDim.x) {
-        if (seq_len(a, n) > 0 || seq_init(a, n)) continue;
-        const int64_t slot = seq_slot(a, n);
-        if (slot < 0) continue;
-        float4* dst = reinterpret_cast<float4*>(a.state + (size_t)slot * a.H * DV * DK);
-        for (int64_t x = lane; x < (int64_t)a.H * DV * DK / 4; x += 32) dst[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
     }
   } else if (warp < 8 && !STATE) {
     // ---------------------------------------------------------------- scores -> P, O -> out
@@ -809,12 +842,8 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&b->p_ready);
+          mbar_arrive(&b->p_ready[s]);
           mbar_arrive(&b->gempty[r]);
-          if (i > 0) {                     // the copies out of the block before's tile of V
-            tma_store_wait<true>();
-            mbar_arrive(&b->vempty[s ^ 1]);
-          }
         }
         if (in) {
           wait(&b->qs_done, n_in);
@@ -846,11 +875,11 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           if (lane == 0) mbar_arrive(&b->o_scaled);
         }
         // the next block's facts, before this one's output is waited for
-        const int o_nt = nt, o_tok = tok + row;
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (int64_t)o_tok * a.os_t + (int64_t)h * a.os_h;
-        const int o_h = h;
+        const int o_nt = nt;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (int64_t)(tok + row) * a.os_t + (int64_t)h * a.os_h;
         if (i + 1 < nblk) fetch(i + 1);
         wait(&b->o_done, i);
+        wait(&b->u_done[s], u);            // the state's products are done with V, too
         tc_fence_after();
         // 32 full rows leave through the tile of V, which the products have finished with, as copies of
         // 64 columns (a thread's own row is 256 bytes in global memory: 32 lines a store); the rows of a
@@ -883,12 +912,8 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (full && lane == 0) {
-#pragma unroll
-          for (int c = 0; c < DV / 64; ++c) tma_store_3d(&tm_o, stage + c * C * 128, 64 * c, o_h, o_tok);
-        }
+        if (lane == 0) mbar_arrive(&b->o_staged);
       }
-      if (lane == 0) tma_store_wait<false>();
     }
   } else if (warp < 12) {
     // ---------------------------------------------------------------- transposed, decayed keys
@@ -977,6 +1002,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const bool live = k0 < DK;
     const uint32_t srow = smem_u32(smem) + M::kS + k0 * 128 + (half * HV / 64) * DK * 128;
     float S[HV];
+    int n_in = 0;                                // blocks with an incoming state so far
 #pragma unroll
     for (int j = 0; j < HV; ++j) S[j] = 0.f;
 #pragma unroll 1
@@ -1022,7 +1048,9 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         for (int j = 0; j < HV; ++j) S[j] = src && live ? d[j * DK] : 0.f;
       }
       if (k.in) {
-        // bf16 copy for Q S (the products that read the one before are complete: u_done)
+        // bf16 copy for Q S, once the products that read the one before are complete
+        if (n_in > 0) wait(&b->qs_done, n_in - 1);
+        ++n_in;
         if (live) {
 #pragma unroll
           for (int c = 0; c < HV / 8; ++c)
