@@ -372,7 +372,8 @@ struct Bars {
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], dfull[kRing], gfull[kRing], gempty[kRing];
   uint64_t qfull, qempty;
   uint64_t sc_done, qs_done, o_done, o_scaled, o_free, o_staged, s_ready, drain[2];
-  uint64_t p_ready[2], u_done[2], u_free[2], kt_ready[2], kt_free[2];   // pairs: the waiting side may be two phases behind
+  uint64_t p_ready[2], u_done[2], u_free[2];   // pairs: the waiting side may be two phases behind
+  uint64_t kt_ready[4], kt_free[4];
   uint32_t tmem;
   int abort;
   Range range;
@@ -389,7 +390,7 @@ AIR_DEVICE bool elect() {
   return p != 0;
 }
 // TMEM columns. P takes the lower half of the scores' columns as they are read. The decayed keys go
-// through a ring of two quarter blocks (two times 16 tokens: four parts of 8 columns).
+// through a ring of four times 16 tokens (four parts of 8 columns).
 constexpr uint32_t kSC = 0, kP = 0, kKT = 128, kO = 256, kU = 384;
 // The state-only kernel has neither scores nor O and takes two regions for U in turn.
 template <bool STATE> AIR_DEVICE uint32_t u_cols(int i) { return STATE && (i & 1) ? kO : kU; }
@@ -423,12 +424,14 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&b->kempty[i], 8);
       mbar_init(&b->vfull[i], 1);
       mbar_init(&b->vempty[i], 1);
-      mbar_init(&b->kt_ready[i], 4);
-      mbar_init(&b->kt_free[i], 1);
       mbar_init(&b->drain[i], 1);
       mbar_init(&b->p_ready[i], 4);
       mbar_init(&b->u_done[i], 1);
       mbar_init(&b->u_free[i], 8);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&b->kt_ready[i], 4);
+      mbar_init(&b->kt_free[i], 1);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&b->dfull[i], 1);
@@ -554,7 +557,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
             wait(&b->dfull[r], i / kRing);
             const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
-            const int steps = __shfl_sync(0xffffffffu, (b->blk[r].nt + 31) / 32 * 2, 0);
+            const int steps = __shfl_sync(0xffffffffu, (b->blk[r].nt + 15) / 16, 0);
             if (aborted()) break;
             if (lane == 0) mbar_arrive(&b->gempty[r]);
             if (in) {
@@ -609,39 +612,36 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
     } else if (warp == 3) {
       // -------------------------------------------------------------- products of the state
-      int kt = 0, kt_round = 0;            // place in the ring of quarter blocks
+      int n = 0;                           // 16s of tokens so far
       const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
 #pragma unroll 1
       for (int i = 0; i < nblk; ++i) {
         const int s = i & 1, r = i % kRing;
         const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
         wait(&b->dfull[r], i / kRing);
-        const int nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0), quarters = (nt + 31) / 32;
+        const int nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0), units = (nt + 15) / 16;
         if (aborted()) break;
         if (lane == 0) mbar_arrive(&b->gempty[r]);
         wait(&b->vfull[s], i >> 1);
         if (!STATE && nt < C) wait(&b->p_ready[s], i >> 1);       // V's rows past the end are zeroed by then
         if (const int f = i - (STATE ? 2 : 1); f >= 0) wait(&b->u_free[f & 1], f >> 1);
-        // U = W V, a quarter of the tokens at a time, the smallest parts first
+        // U = W V, 16 tokens at a time, the smallest parts first
 #pragma unroll 1
-        for (int qt = 0; qt < quarters; ++qt) {
-          wait(&b->kt_ready[kt], kt_round);
+        for (int c = 0; c < units; ++c, ++n) {
+          wait(&b->kt_ready[n & 3], n >> 2);
           tc_fence_after();
           if (elect()) {
-            const uint32_t dvq = dvs + qt * (4096 >> 4), ta = tmem + kKT + 64 * kt, td = tmem + u_cols<STATE>(i);
+            const uint32_t ta = tmem + kKT + 32 * (n & 3), td = tmem + u_cols<STATE>(i);
 #pragma unroll
-            for (int part = 3; part >= 0; --part) {
-              mma_ts(td, ta + 8 * part, dvq, id_mn, part < 3 || qt > 0);
-              mma_ts(td, ta + 8 * part + 32, dvq + (2048 >> 4), id_mn, 1);
-            }
-            mma_commit(&b->kt_free[kt]);
-            if (qt + 1 == quarters) {
+            for (int part = 3; part >= 0; --part)
+              mma_ts(td, ta + 8 * part, dvs + c * (2048 >> 4), id_mn, part < 3 || c > 0);
+            mma_commit(&b->kt_free[n & 3]);
+            if (c + 1 == units) {
               mma_commit(&b->u_done[s]);
               if (STATE) mma_commit(&b->vempty[s]);     // else V's tile goes on to hold the output
             }
           }
           __syncwarp();
-          if (++kt == 2) kt = 0, ++kt_round;
         }
       }
       if (elect()) mma_commit(&b->drain[1]);
@@ -831,7 +831,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (nt < C) {
           // rows of V past the sequence's end: 0 x whatever they hold must stay 0
           wait(&b->vfull[s], u);
-          if (row >= nt && row < (nt + 31) / 32 * 32) {
+          if (row >= nt && row < (nt + 15) / 16 * 16) {
 #pragma unroll 1
             for (int c = 0; c < DV / 8; ++c)
               *reinterpret_cast<uint4*>(smem + M::kV + s * M::kVTile + (c / 8) * C * 128 + row * 128 + 16 * (c % 8)) =
@@ -926,10 +926,10 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + kKT;
     const uint32_t col0 = smem_u32(smem) + M::kK + (live ? q / 2 : 0) * C * 128 + (lane & 7) * 128 +
                           (((4 * (q & 1) + (lane >> 3)) ^ (lane & 7)) << 4);
-    // In the state-only kernel (full blocks) the output warps share the work: the second quarters of two.
+    // In the state-only kernel (full blocks) the output warps share the work: every second 16 tokens.
     constexpr int kStep = STATE ? 2 : 1;
     const int mine = STATE && warp < 8;
-    int kt = mine, kt_round = 0;                 // place in the ring of quarter blocks
+    int n = 0;                                   // 16s of tokens in the blocks before
 #pragma unroll 1
     for (int i = 0; i < nblk; ++i) {
       const int s = i & 1, r = i % kRing;
@@ -937,15 +937,14 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       wait(&b->kfull[s], i >> 1);
       if (aborted()) break;
       const Block& k = b->blk[r];
-      const int nt = k.nt, units = (nt + 31) / 32 * 2;
+      const int nt = k.nt, units = (nt + 15) / 16;
       const int from = live ? nt : 0;            // tokens from here on count as zeros, whatever they hold
       const uint32_t col = col0 + s * M::kKTile;
       uint32_t x[2][4];
-      ldsm_t(col + mine * 4096, x[0]);
-      ldsm_t(col + mine * 4096 + 1024, x[1]);
+      ldsm_t(col + mine * 2048, x[0]);
+      ldsm_t(col + mine * 2048 + 1024, x[1]);
 #pragma unroll 1
-      for (int c = 2 * mine; c < units;) {
-        const int next = c & 1 ? c + 2 * kStep - 1 : c + 1;
+      for (int c = mine; c < units; c += kStep) {
         if (16 * c + 16 > from) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -969,25 +968,21 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             o[12] = bf2_fma(x[h][e], w3, bf2_fma(x[h][e], w2, bf2_neg(o[8])));
           }
         }
-        if (next < units) {
-          ldsm_t(col + next * 2048, x[0]);
-          ldsm_t(col + next * 2048 + 1024, x[1]);
+        if (c + kStep < units) {
+          ldsm_t(col + (c + kStep) * 2048, x[0]);
+          ldsm_t(col + (c + kStep) * 2048 + 1024, x[1]);
         }
-        if (!(c & 1) && kt_round) wait(&b->kt_free[kt], kt_round - 1);
+        const int kt = (n + c) & 3;
+        if (n + c >= 4) wait(&b->kt_free[kt], (n + c) / 4 - 1);
         tc_fence_after();
-        const uint32_t at = trow + 64 * kt + 32 * (c & 1);
-        tmem_st_frag(at, p[0]);
-        tmem_st_frag(at + (16u << 16), p[1]);
-        if (c & 1) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b->kt_ready[kt]);
-          if (STATE || kt) ++kt_round;
-          if (!STATE) kt ^= 1;
-        }
-        c = next;
+        tmem_st_frag(trow + 32 * kt, p[0]);
+        tmem_st_frag(trow + 32 * kt + (16u << 16), p[1]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->kt_ready[kt]);
       }
+      n += units;
       if (lane == 0) {
         mbar_arrive(&b->kempty[s]);
         mbar_arrive(&b->gempty[r]);
