@@ -14,6 +14,16 @@ import torch
 from . import count_launch, require_ext
 from .gemm import workspace
 
+_ERR: dict = {}
+
+
+def _err(t: torch.Tensor) -> torch.Tensor:
+    """The shared error word of t's device."""
+    e = _ERR.get(t.device)
+    if e is None:
+        e = _ERR[t.device] = workspace(t.device).err
+    return e
+
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *,
                      state: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None,
@@ -35,12 +45,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Returns out [T, H, dv] in q's type. bf16 prompts with head sizes 64 / 128 run on the tensor
     cores in blocks of 128 tokens; a NaN or infinity in v reaches the outputs of its whole block.
     """
-    if out is None:
-        out = torch.empty(q.shape[0], log_decay.shape[-1], v.shape[-1], dtype=q.dtype, device=q.device)
-    if err is None:
-        err = workspace(q.device).err
-    require_ext().linear_attention(q, k, v, log_decay, state, cu_seqlens, slots, has_state,
-                                   scale if scale is not None else q.shape[-1] ** -0.5, out, err)
+    out = require_ext().linear_attention(q, k, v, log_decay, state, cu_seqlens, slots, has_state, scale, out,
+                                         _err(q) if err is None else err)
     count_launch()
     return out
 
@@ -51,12 +57,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     """One new token per sequence of :func:`linear_attention`: row n of q [B, Hq, dk], k, v and
     ``log_decay`` ([H] or [B, H]) advances state row ``slots[n]`` (None: n) in place. Slot -1 is a
     padding row: no state, output zero. Rows of one call are distinct. Returns out [B, H, dv]."""
-    if out is None:
-        out = torch.empty(q.shape[0], log_decay.shape[-1], v.shape[-1], dtype=q.dtype, device=q.device)
-    if err is None:
-        err = workspace(q.device).err
-    require_ext().linear_attention_step(q, k, v, log_decay, state, slots,
-                                        scale if scale is not None else q.shape[-1] ** -0.5, out, err)
+    out = require_ext().linear_attention_step(q, k, v, log_decay, state, slots, scale, out,
+                                              _err(q) if err is None else err)
     count_launch()
     return out
 
@@ -70,16 +72,11 @@ def add_rmsnorm_fp8(x: torch.Tensor, y: torch.Tensor | None, w: torch.Tensor, ep
     x f32 [T, K] is the residual stream, y bf16 / f32 [T, K] (None: nothing is added), K a multiple
     of 8 up to 32768. r goes to ``resid_out`` (None: back into x when there is a y), n also to
     ``out_bf16`` when given. Returns (codes uint8 [T, K], scales f32 [T])."""
-    T, K = x.shape
-    if xq is None:
-        xq = torch.empty(T, K, dtype=torch.uint8, device=x.device)
-    if xs is None:
-        xs = torch.empty(T, dtype=torch.float32, device=x.device)
     if resid_out is None and y is not None:
         resid_out = x
-    require_ext().add_rmsnorm_fp8(x, y, w, eps, w_offset, resid_out, xq, xs, out_bf16)
+    codes = require_ext().add_rmsnorm_fp8(x, y, w, eps, w_offset, resid_out, xq, xs, out_bf16)
     count_launch()
-    return xq, xs
+    return codes
 
 
 def logit_rules(logits: torch.Tensor, *, out: torch.Tensor | None = None, counts: torch.Tensor | None = None,
@@ -101,7 +98,7 @@ def logit_rules(logits: torch.Tensor, *, out: torch.Tensor | None = None, counts
     if out is None:
         out = logits if logits.dtype == torch.float32 else torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
     if err is None:
-        err = workspace(logits.device).err
+        err = _err(logits)
     ptr, ids, vals = bias if bias is not None else (None, None, None)
     require_ext().logit_rules(logits, out, counts, count_row, repetition, frequency, presence, ptr, ids, vals, mask, err)
     count_launch()

@@ -3,6 +3,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cmath>
 
 #include "linear_attn.h"
 #include "logit_rules.h"
@@ -99,9 +100,23 @@ air::LinAttnArgs lin_args(const char* op, const Tensor& q, const Tensor& k, cons
   return a;
 }
 
+// The caller's output, or a new one.
+Tensor or_new(const optional<Tensor>& out, at::IntArrayRef sizes, const Tensor& as, at::ScalarType type) {
+  if (out.has_value()) return *out;
+  TORCH_CHECK(as.is_cuda(), "the operands must be CUDA tensors");
+  return at::empty(sizes, as.options().dtype(type));
+}
+Tensor rows_or_new(const char* op, const optional<Tensor>& out, const Tensor& q, const Tensor& v, const Tensor& decay) {
+  TORCH_CHECK(q.dim() == 3 && v.dim() == 3 && decay.dim() >= 1, op, ": q and v must be [tokens, heads, dim], log_decay [.., heads]");
+  return or_new(out, {q.size(0), decay.size(-1), v.size(2)}, q, q.scalar_type());
+}
+
 // Packed prompts. cu [N + 1] int32 token offsets (none: one sequence of all tokens).
-void linear_attention(Tensor q, Tensor k, Tensor v, Tensor decay, optional<Tensor> state, optional<Tensor> cu,
-                      optional<Tensor> slots, optional<Tensor> has_state, double scale, Tensor out, Tensor err) {
+Tensor linear_attention(Tensor q, Tensor k, Tensor v, Tensor decay, optional<Tensor> state, optional<Tensor> cu,
+                        optional<Tensor> slots, optional<Tensor> has_state, optional<double> scale_, optional<Tensor> out_,
+                        Tensor err) {
+  Tensor out = rows_or_new("linear_attention", out_, q, v, decay);
+  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)q.size(2));
   air::LinAttnArgs a = lin_args("linear_attention", q, k, v, decay, state, scale, out, err);
   const c10::cuda::CUDAGuard guard(q.device());
   int64_t N = 1;
@@ -118,7 +133,7 @@ void linear_attention(Tensor q, Tensor k, Tensor v, Tensor decay, optional<Tenso
   a.slots = int_row(slots, N, q, "slots");
   a.has_state = int_row(has_state, N, q, "has_state");
   TORCH_CHECK(!a.state || a.slots || N <= a.S, "linear_attention: ", str(N), " sequences, ", str(a.S), " state rows");
-  if (N == 0) return;
+  if (N == 0) return out;
   const bool f32 = q.scalar_type() == at::kFloat;
   auto st = at::cuda::getCurrentCUDAStream();
   if (air::linear_blocks_supported(a, f32)) {
@@ -133,11 +148,14 @@ void linear_attention(Tensor q, Tensor k, Tensor v, Tensor decay, optional<Tenso
     air::launch_linear_scan(a, f32, st);
   }
   post("linear_attention");
+  return out;
 }
 
 // One new token per sequence: row n of q, k and v belongs to state row slots[n] (none: n).
-void linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor state, optional<Tensor> slots,
-                           double scale, Tensor out, Tensor err) {
+Tensor linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor state, optional<Tensor> slots,
+                             optional<double> scale_, optional<Tensor> out_, Tensor err) {
+  Tensor out = rows_or_new("linear_attention_step", out_, q, v, decay);
+  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)q.size(2));
   air::LinAttnArgs a = lin_args("linear_attention_step", q, k, v, decay, state, scale, out, err);
   const c10::cuda::CUDAGuard guard(q.device());
   a.N = a.T;
@@ -146,20 +164,22 @@ void linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor st
   TORCH_CHECK((int64_t)a.N < (1ll << 31) / a.H, "linear_attention_step: too many rows");
   a.slots = int_row(slots, a.N, q, "slots");
   TORCH_CHECK(a.slots || a.N <= a.S, "linear_attention_step: ", str(a.N), " rows, ", str(a.S), " state rows");
-  if (a.N == 0) return;
+  if (a.N == 0) return out;
   const bool f32 = q.scalar_type() == at::kFloat;
   auto st = at::cuda::getCurrentCUDAStream();
   if (air::linear_step_supported(a, f32)) air::launch_linear_step(a, f32, st);
   else air::launch_linear_scan(a, f32, st);
   post("linear_attention_step");
+  return out;
 }
 
 bool aligned(const Tensor& t, int64_t bytes, bool rows = true) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0 && (!rows || t.stride(0) * t.element_size() % bytes == 0);
 }
 
-void add_rmsnorm_fp8(Tensor x, optional<Tensor> y, Tensor w, double eps, double w_offset, optional<Tensor> resid,
-                     Tensor xq, Tensor xs, optional<Tensor> out_bf16) {
+std::tuple<Tensor, Tensor> add_rmsnorm_fp8(Tensor x, optional<Tensor> y, Tensor w, double eps, double w_offset,
+                                           optional<Tensor> resid, optional<Tensor> xq_, optional<Tensor> xs_,
+                                           optional<Tensor> out_bf16) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.scalar_type() == at::kFloat && x.stride(1) == 1,
               "add_rmsnorm_fp8: x must be a CUDA float32 [tokens, dim] with contiguous rows");
   const c10::cuda::CUDAGuard guard(x.device());
@@ -199,6 +219,7 @@ void add_rmsnorm_fp8(Tensor x, optional<Tensor> y, Tensor w, double eps, double 
     a.out_bf16 = out_bf16->data_ptr();
     a.ldo = out_bf16->stride(0);
   }
+  Tensor xq = or_new(xq_, {T, K}, x, at::kByte), xs = or_new(xs_, {T}, x, at::kFloat);
   same_device(xq, x, "xq");
   same_device(xs, x, "xs");
   TORCH_CHECK(xq.element_size() == 1 && xq.is_contiguous() && xq.numel() == T * K && aligned(xq, 8, false),
@@ -214,6 +235,7 @@ void add_rmsnorm_fp8(Tensor x, optional<Tensor> y, Tensor w, double eps, double 
   const char* e = air::launch_add_rmsnorm_fp8(a, at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(e == nullptr, e ? e : "");
   post("add_rmsnorm_fp8");
+  return {xq, xs};
 }
 
 void logit_rules(Tensor logits, Tensor out, optional<Tensor> counts, optional<Tensor> count_row,
