@@ -455,13 +455,16 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     __syncthreads();
     if (b->range.tail == 0) {
       if (threadIdx.x == 0) ws_meta[blockIdx.x * 2].x = 0;
-      return;
+      return;                              // counts as the trigger of the next kernel
     }
   }
   if (warp == 1) tmem_alloc(&b->tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // the chained states come from the kernel before, which may still run; so may the copies of the pool
+  if (ws_state) pdl_wait();
+  pdl_trigger();
   const uint32_t tmem = __shfl_sync(0xffffffffu, b->tmem, 0);
   const int nblk = __shfl_sync(0xffffffffu, STATE ? b->range.tail : b->range.blocks, 0);
   auto wait = [&](uint64_t* bar, int parity) { bar_wait(bar, parity, &b->abort); };
@@ -555,7 +558,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           if (i >= 0) {
             const int s = i & 1, r = i % kRing;
             const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
-            wait(&b->dfull[r], i / kRing);
+            wait(&b->gfull[r], i / kRing);
             const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
             const int steps = __shfl_sync(0xffffffffu, (b->blk[r].nt + 15) / 16, 0);
             if (aborted()) break;
@@ -659,52 +662,50 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       float total_piece = 0.f;
       for (int i = 0; i < nblk; ++i) {
         const int r = i % kRing, t0 = w.token(), nt = w.count();
-        float g[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = 4 * lane + e;
-          const float x = j < nt ? a.decay[(int64_t)(t0 + j) * a.decay_t + w.p.h] : 0.f;
-          g[e] = x < kFloor ? kFloor : x;
-        }
         if (i >= kRing) wait(&b->gempty[r], i / kRing - 1);
         if (aborted()) break;
-        if (!STATE && w.p.c == 0 && seq_init(a, w.p.n)) {
-          // the state that a resumed sequence starts from, on its way into L2
-          const int64_t slot = seq_slot(a, w.p.n);
-          const char* row = reinterpret_cast<const char*>(a.state + ((size_t)max(slot, (int64_t)0) * a.H + w.p.h) * DV * DK);
-          if (slot >= 0)
-            for (int x = lane * 128; x < DV * DK * 4; x += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + x));
-        }
         Block& k = b->blk[r];
-        if (lane == 0) {                   // what the copies need does not wait for the decays
+        if (lane == 0) {                   // what the copies need does not wait for the rest
           k.tok = t0;
           k.nt = nt;
           k.h = w.p.h;
           k.hq = w.p.h / a.q_div;
           k.hk = w.p.h / a.k_div;
           k.hv = w.p.h / a.v_div;
+          mbar_arrive(&b->dfull[r]);
+        }
+        float g[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * lane + e;
+          g[e] = j < nt ? a.decay[(int64_t)(t0 + j) * a.decay_t + w.p.h] : 0.f;
+        }
+        const int64_t slot = STATE ? -1 : seq_slot(a, w.p.n);
+        float* row = slot < 0 ? nullptr : a.state + ((size_t)slot * a.H + w.p.h) * DV * DK;
+        const bool resumes = !STATE && w.p.c == 0 && row && seq_init(a, w.p.n);
+        if (resumes)                       // the state that a sequence starts from, on its way into L2
+          for (int x = lane * 128; x < DV * DK * 4; x += 32 * 128)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(row) + x));
+        if (lane == 0) {
           k.first = i == 0 || w.p.c == 0;
           k.src = nullptr;
           k.dst = nullptr;
           if constexpr (STATE) {
             if (i + 1 == nblk) k.dst = ws_state + (size_t)blockIdx.x * DV * DK;
           } else {
-            const int64_t slot = seq_slot(a, w.p.n);
-            float* row = slot < 0 ? nullptr : a.state + ((size_t)slot * a.H + w.p.h) * DV * DK;
-            k.in = w.p.c > 0;
-            if (w.p.c == 0 && row && seq_init(a, w.p.n)) {
-              // the pool's state; of a sequence that is cut the chain kernel's copy of it, because the
-              // range that ends the sequence may write the pool's row first
-              k.in = 1;
+            k.in = w.p.c > 0 || resumes;
+            // The incoming state: the pool's; of a sequence that is cut the chain kernel's copy of it, because
+            // the range that ends the sequence may write the pool's row first; inside a cut, the chain's.
+            if (resumes)
               k.src = rg.cut_end && w.p.n == rg.end.n && w.p.h == rg.end.h
                           ? ws_state + (size_t)(gridDim.x + blockIdx.x) * DV * DK : row;
-            } else if (i == 0 && w.p.c > 0) {
+            else if (i == 0 && w.p.c > 0)
               k.src = ws_state + (size_t)(blockIdx.x - 1) * DV * DK;
-            }
             if (w.last()) k.dst = row;
           }
-          mbar_arrive(&b->dfull[r]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = g[e] < kFloor ? kFloor : g[e];
         float pre[4], suf[4];              // inclusive sums up to, exclusive sums after each token, in the 32
         pre[0] = g[0]; pre[1] = pre[0] + g[1]; pre[2] = pre[1] + g[2]; pre[3] = pre[2] + g[3];
         suf[3] = 0.f; suf[2] = g[3]; suf[1] = suf[2] + g[2]; suf[0] = suf[1] + g[1];
@@ -1075,6 +1076,8 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 // Grid (R, elements / 1024): the CTAs of a row that opens a sequence walk the rows that continue it.
 __global__ void __launch_bounds__(256) linear_chain_kernel(const LinAttnArgs a, float* __restrict__ ws_state,
                                                           const int4* __restrict__ ws_meta) {
+  pdl_wait();
+  pdl_trigger();
   int4 m = ws_meta[blockIdx.x * 2];
   if (!m.x || !m.z) return;
   const int n = m.w, h = ws_meta[blockIdx.x * 2 + 1].x;
@@ -1154,10 +1157,27 @@ const char* launch_dims(const LinAttnArgs& a, float* ws, int sms, cudaStream_t s
     if (!ws) return "linear_attention: workspace";
     meta = reinterpret_cast<int4*>(ws + (size_t)2 * sms * DK * DV);
     linear_blocks_kernel<DK, DV, true><<<sms, kThreads, kSmem, st>>>(tq, tk, tv, to, a, ws, meta);
-    linear_chain_kernel<<<dim3(sms, (DK * DV + 1023) / 1024), 256, 0, st>>>(a, ws, meta);
   }
-  linear_blocks_kernel<DK, DV, false><<<sms, kThreads, kSmem, st>>>(tq, tk, tv, to, a, ws, meta);
-  return nullptr;
+  // The other two start while their predecessor ends (programmatic dependent launch): they set up, and wait for
+  // it to be complete before they read what it wrote.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = meta ? 1 : 0;
+  cudaError_t e = cudaSuccess;
+  if (meta) {
+    cfg.gridDim = dim3(sms, (DK * DV + 1023) / 1024);
+    cfg.blockDim = dim3(256);
+    e = cudaLaunchKernelEx(&cfg, linear_chain_kernel, a, ws, (const int4*)meta);
+  }
+  cfg.gridDim = dim3(sms);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, linear_blocks_kernel<DK, DV, false>, tq, tk, tv, to, a, ws, meta);
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
 }  // namespace
