@@ -36,6 +36,7 @@ void launch_linear_step(const LinAttnArgs& a, bool f32, cudaStream_t st);
 // Blocks of 128 tokens on the tensor cores: bf16, dk and dv in {64, 128}, rows and strides of whole
 // 16-byte units.
 bool linear_blocks_supported(const LinAttnArgs& a, bool f32);
+bool linear_blocks_worth(const LinAttnArgs& a);         // against launch_linear_scan, by size
 // Floats of scratch that launch_linear_blocks needs (0: none).
 int64_t linear_blocks_workspace(const LinAttnArgs& a, int sms);
 const char* launch_linear_blocks(const LinAttnArgs& a, float* ws, int sms, cudaStream_t st);

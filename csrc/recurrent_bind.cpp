@@ -136,7 +136,7 @@ Tensor linear_attention(Tensor q, Tensor k, Tensor v, Tensor decay, optional<Ten
   if (N == 0) return out;
   const bool f32 = q.scalar_type() == at::kFloat;
   auto st = at::cuda::getCurrentCUDAStream();
-  if (air::linear_blocks_supported(a, f32)) {
+  if (air::linear_blocks_supported(a, f32) && air::linear_blocks_worth(a)) {
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     // scratch of the split over the length, from the allocator's pool of this stream
     Tensor ws;
