@@ -13,7 +13,7 @@
 // are exact). S itself stays f32: the keys times their f32 decay factors are split into four bf16
 // parts that add up to all 24 bits, each block's update is accumulated on its own and added to S in
 // registers, because adding it to a long-lived accumulator inside the tensor core would round the
-// whole state 24 times a block.
+// whole state 32 times a block.
 //
 // A CTA has 20 warps, each with one task, that pass blocks on through mbarriers (every wait is bounded): copies;
 // decays (sums of log decays within 32 tokens, so that no difference of large sums is taken); the two groups
@@ -29,8 +29,8 @@
 // All sums have a fixed order.
 //
 // Measured (B200, 32 heads of 128): about 5600 clocks a block where tensor products need 3600 and the memory
-// 5400 with all SMs at it. One prompt of 16384 tokens: 183 us (62 + 9 + 112 for the three kernels), 2.9 TB/s of
-// the 83 us floor's bytes; 13 ragged prompts of 8111 tokens together: 93 us; 77 tokens: 8.9 us. Bound by shared
+// 5400 with all SMs at it. One prompt of 16384 tokens: 183 us (64, 9 and 123 for each of the three kernels
+// alone; their ends overlap) of an 83 us floor; 13 ragged prompts of 8111 tokens together: 93 us; 77 tokens: 8.9 us. Bound by shared
 // memory: the products' operands (2300 clocks a block), the warps' accesses (2300) and the copies (1000) share it.
 #include <cuda.h>
 #include <cudaTypedefs.h>
