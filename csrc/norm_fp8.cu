@@ -4,7 +4,7 @@
 // goes to memory: 4 + 2 bytes read and 4 + 1 written per element (bf16 addend). The sum of squares,
 // the maximum and the norm stay f32; the codes are the only rounding (the separate norm and
 // quantiser round the norm's output to bf16 between them). Memory-bound with many rows: 6007 x 4096 takes
-// 42.5 us of a 41.9 us floor (6.4 TB/s); one row 2.8 us, latency of two block reductions.
+// 42.6 us of a 41.9 us floor (6.4 TB/s); one row 2.5 us, latency of two block reductions.
 #include <cuda_fp8.h>
 #include "common.cuh"
 #include "norm_fp8.h"
@@ -103,10 +103,16 @@ __global__ void __launch_bounds__(NT) add_rmsnorm_fp8_kernel(const AddNormF8Args
 const char* launch_add_rmsnorm_fp8(const AddNormF8Args& a, cudaStream_t st) {
   if (a.T <= 0) return nullptr;
   if (a.K % 8 || a.K < 8 || a.K > kAddNormMaxK) return "add_rmsnorm_fp8: K must be a multiple of 8 up to 32768";
-  // eight elements a thread up to 8192 (at 6007 x 4096: 48 us with 512 threads x 8, 50 with 256 x 16, 61 with
-  // 128 x 32); beyond it the row needs more of the block's 1024 threads
+  // Eight elements a thread up to 8192 (at 6007 x 4096: 42.6 us with 512 threads x 8, 50 with 256 x 16, 61 with
+  // 128 x 32); beyond it the row needs more of the block's 1024 threads. Rows of at most 512 leave half or more of
+  // 128 threads idle: once the rows are more than one wave of such blocks (16 an SM), blocks of 32 or 64 threads
+  // take 13.6 against 19.6 us at 20000 x 256, 18.7 against 22.7 at 20000 x 512 and 3.8 against 4.2 at 3200 x 256;
+  // with fewer rows the larger block is done sooner (400 x 256: 2.2 against 2.4 us).
+  const bool waves = a.T > 148 * 16;
 #define AIR_ANQ(NT, V) add_rmsnorm_fp8_kernel<NT, V><<<a.T, NT, 0, st>>>(a)
-  if (a.K <= 1024) AIR_ANQ(128, 2);
+  if (waves && a.K <= 256) AIR_ANQ(32, 2);
+  else if (waves && a.K <= 512) AIR_ANQ(64, 2);
+  else if (a.K <= 1024) AIR_ANQ(128, 2);
   else if (a.K <= 2048) AIR_ANQ(256, 2);
   else if (a.K <= 4096) AIR_ANQ(512, 2);
   else if (a.K <= 8192) AIR_ANQ(1024, 2);

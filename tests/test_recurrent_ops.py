@@ -461,6 +461,13 @@ def test_add_rmsnorm_fp8(T, K, ydt):
 
 
 @gpu
+@pytest.mark.parametrize("T,K", [(2369, 8), (2368, 256), (2369, 256), (2400, 136), (2400, 264), (2369, 512), (2400, 520)])
+@pytest.mark.parametrize("ydt", [None, torch.bfloat16])
+def test_add_rmsnorm_fp8_many_narrow_rows(T, K, ydt):
+    test_add_rmsnorm_fp8(T, K, ydt)   # blocks of 32 and 64 threads: at most 8 squares a thread, inside K / 64 + 24
+
+
+@gpu
 def test_add_rmsnorm_fp8_special_rows():
     K = 256
     x = torch.randn(6, K, generator=torch.Generator().manual_seed(0))
