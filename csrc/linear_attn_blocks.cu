@@ -384,8 +384,9 @@ struct alignas(16) Block {
 struct Bars {
   uint64_t kfull[2], kempty[2], vfull[2], vempty[2], dfull[kRing], gfull[kRing], gempty[kRing];
   uint64_t qfull, qempty;
-  uint64_t sc_done, qs_done, o_done, o_scaled, o_free, o_staged, s_ready, drain[2];
-  uint64_t p_ready[2], u_done[2], u_free[2];   // pairs: the waiting side may be two phases behind
+  uint64_t sc_done, qs_done, o_done, o_scaled, o_free, s_ready, drain[2];
+  // pairs: the waiting side may be two phases behind (for o_staged: copies that wait for a late description)
+  uint64_t p_ready[2], u_done[2], u_free[2], o_staged[2];
   uint64_t kt_ready[4], kt_free[4];
   uint32_t tmem;
   int abort;
@@ -441,6 +442,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&b->p_ready[i], 4);
       mbar_init(&b->u_done[i], 1);
       mbar_init(&b->u_free[i], 8);
+      mbar_init(&b->o_staged[i], 4);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&b->kt_ready[i], 4);
@@ -459,7 +461,6 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     mbar_init(&b->o_scaled, 4);
     mbar_init(&b->o_free, 4);
     mbar_init(&b->s_ready, 8);
-    mbar_init(&b->o_staged, 4);
     b->abort = 0;
     fence_mbar_init();
   }
@@ -493,7 +494,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         int h0 = 0, tok0 = 0, rows0 = 0, h1 = 0, tok1 = 0, rows1 = 0;    // the two blocks before
         // the output of a block out of V's tile, of which it took the place
         auto out = [&](int i, int h, int tok, int rows) {
-          wait(&b->o_staged, i);
+          wait(&b->o_staged[i & 1], i >> 1);
           if (aborted()) return;
 #pragma unroll 1
           for (int x = 0; x < rows; x += 32)
@@ -926,7 +927,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&b->o_staged);
+        if (lane == 0) mbar_arrive(&b->o_staged[s]);
       }
     }
   } else if (warp < 12) {

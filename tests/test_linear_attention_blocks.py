@@ -1,0 +1,86 @@
+"""The block form of linear attention where its hand-overs, its split over the length and its state's precision are
+at work: long runs of empty sequences between a CTA's blocks, every pair of head sizes, sequences that resume from
+the pool and are cut. Definitions, inputs and bounds are those of test_recurrent_ops."""
+import pytest
+import torch
+
+from air_rs import ops
+from test_recurrent_ops import _c, _inputs, _near, _oracle
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+
+
+def _cu(lens):
+    return torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+
+
+# ---------------------------------------------------------------------------------- runs of empty sequences
+RUNS = [  # heads, lengths
+    # whole items dealt out in turns (more sequences than are sorted): a CTA steps over hundreds of empty ones
+    (64, [1000] + [0] * 500 + [1000] + [0] * 500 + [1000]),
+    # short prompts around a run of empty slots: turns without work between two blocks of a CTA
+    (64, [128] * 30 + [0] * 200 + [100] * 30),
+    # one stretch of the list for each SM: a cut sequence, empty ones behind it, a short one at the end
+    (2, [2900] + [0] * 500 + [40]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", range(len(RUNS)))
+def test_runs_of_empty_sequences_between_blocks(case):
+    """The description of a CTA's next block can be late by many blocks' time; nothing that is waited for meanwhile
+    may be missed."""
+    H, lens = RUNS[case]
+    T, N, d = sum(lens), len(lens), 64
+    r = torch.Generator().manual_seed(case)
+    q, k, v, g = _inputs(case, T, H, 1, 1, H, d, d, torch.bfloat16)
+    has = torch.randint(0, 2, (N,), generator=r)
+    full = [n for n in range(N) if lens[n]]
+    pool = torch.randn(N, H, d, d, generator=r)
+    init = (pool * has[:, None, None, None])[full]
+    # an oracle of matrix products, sequence by sequence in blocks of 100 tokens
+    out, st, mag, sm = _by_blocks(q, k, v, g, [lens[n] for n in full], init, 0.125)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    dpool = pool.to(DEV)
+    args = [x.to(DEV) for x in (q, k, v, g)]
+    got = ops.linear_attention(*args, state=dpool, cu_seqlens=_cu(lens), has_state=has.to(torch.int32).to(DEV), err=err)
+    assert int(err) == 0
+    co, cs = _c(max(lens), d, True)
+    _near(got, out, mag, co, True)
+    _near(dpool[full], st, sm, cs, False)
+    empty = [n for n in range(N) if not lens[n]]
+    assert torch.equal(dpool[empty].cpu(), (pool * has[:, None, None, None])[empty])
+
+
+def _by_blocks(q, k, v, g, lens, init, scale, block=100):
+    """_oracle's results by products over blocks of tokens (64 bits), for sequences too long to take token by token."""
+    H = g.shape[1]
+    q, k, v = (x.double().repeat_interleave(H // x.shape[1], 1).transpose(0, 1) for x in (q, k, v))     # [H, T, d]
+    g = g.double().t()
+    out = torch.zeros(v.shape, dtype=torch.float64)
+    mag = torch.zeros_like(out)
+    st, sm = init.double().clone(), init.double().abs()
+    t = 0
+    for n, L in enumerate(lens):
+        for b in range(t, t + L, block):
+            e = min(b + block, t + L)
+            G = g[:, b:e].cumsum(1)
+            w = (G[:, :, None] - G[:, None, :]).masked_fill(~torch.ones(e - b, e - b, dtype=torch.bool).tril(), -float("inf")).exp()
+            for x, s, f in ((out, st, lambda z: z), (mag, sm, torch.abs)):
+                qb, kb, vb = f(q[:, b:e]), f(k[:, b:e]), f(v[:, b:e])
+                x[:, b:e] = abs(scale) * ((qb @ kb.transpose(1, 2) * w) @ vb + (qb * G.exp()[..., None]) @ s[n].transpose(1, 2))
+                s[n] = s[n] * G[:, -1].exp()[:, None, None] + (vb * (G[:, -1:] - G).exp()[..., None]).transpose(1, 2) @ kb
+        t += L
+    if scale < 0:
+        out = -out
+    return out.transpose(0, 1), st, mag.transpose(0, 1), sm
+
+
+def test_block_oracle_is_the_recurrence():
+    """On the CPU: the oracle by blocks against the one token by token."""
+    lens = [250, 3, 101]
+    q, k, v, g = _inputs(0, sum(lens), 4, 2, 1, 4, 16, 8, torch.bfloat16, strong=True)
+    init = torch.randn(3, 4, 8, 16, generator=torch.Generator().manual_seed(1))
+    for a, b in zip(_by_blocks(q, k, v, g, lens, init, -0.3), _oracle(q, k, v, g, lens, init, -0.3)):
+        torch.testing.assert_close(a, b, rtol=1e-11, atol=1e-11)
