@@ -295,8 +295,9 @@ __device__ __noinline__ void bar_wait_slow(uint64_t* bar, uint32_t parity, int* 
     }
   }
 }
-// After an abort the roles leave at their next block; until then they work on whatever is there, all of
-// it inside the CTA's own memory.
+// After an abort a wait returns without what it waited for. Whoever then goes on to global memory (a copy, an
+// output, a state's row) looks first whether it did, and leaves; what a role does until then stays inside the
+// CTA's own memory.
 AIR_DEVICE void bar_wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
   if (!mbar_try_wait(bar, parity & 1)) bar_wait_slow(bar, parity & 1, abort_flag);
 }
@@ -484,6 +485,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   auto wait = [&](uint64_t* bar, int parity) { bar_wait(bar, parity, &b->abort); };
   constexpr uint32_t id_mn = idesc_bf16_f32(128, DV) | kBMn;
   auto aborted = [&] { return *(volatile int*)&b->abort != 0; };
+  auto warp_aborted = [&] { return __any_sync(0xffffffffu, aborted()) != 0; };   // one answer for the whole warp
 
   if (warp < 4) {
     if (warp == 1) {
@@ -575,7 +577,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             wait(&b->gfull[r], i / kRing);
             const int in = __shfl_sync(0xffffffffu, b->blk[r].in, 0);
             const int steps = __shfl_sync(0xffffffffu, (b->blk[r].nt + 15) / 16, 0);
-            if (aborted()) break;
+            if (warp_aborted()) break;
             if (lane == 0) mbar_arrive(&b->gempty[r]);
             if (in) {
               // O = Q S
@@ -637,7 +639,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         const uint32_t dvs = mn_desc(sm + M::kV + s * M::kVTile, C * 128);
         wait(&b->dfull[r], i / kRing);
         const int nt = __shfl_sync(0xffffffffu, b->blk[r].nt, 0), units = (nt + 15) / 16;
-        if (aborted()) break;
+        if (warp_aborted()) break;
         if (lane == 0) mbar_arrive(&b->gempty[r]);
         wait(&b->vfull[s], i >> 1);
         if (!STATE && nt < C) wait(&b->p_ready[s], i >> 1);       // V's rows past the end are zeroed by then
@@ -677,7 +679,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       for (int i = 0; i < nblk; ++i) {
         const int r = i % kRing, t0 = w.token(), nt = w.count();
         if (i >= kRing) wait(&b->gempty[r], i / kRing - 1);
-        if (aborted()) break;
+        if (warp_aborted()) break;
         Block& k = b->blk[r];
         if (lane == 0) {                   // what the copies need does not wait for the rest
           k.tok = t0;
@@ -789,7 +791,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll 1
       for (int i = 0; i < nblk; ++i) {
         const int s = i & 1, u = i >> 1, r = i % kRing;
-        if (aborted()) break;
+        if (warp_aborted()) break;
         const Block& k = b->blk[r];
         wait(&b->sc_done, i);
         if (lane == 0) {
@@ -895,6 +897,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (i + 1 < nblk) fetch(i + 1);
         wait(&b->o_done, i);
         wait(&b->u_done[s], u);            // the state's products are done with V, too
+        if (warp_aborted()) break;
         tc_fence_after();
         // 32 full rows leave through the tile of V, which the products have finished with, as copies of
         // 64 columns (a thread's own row is 256 bytes in global memory: 32 lines a store); the rows of a
@@ -950,7 +953,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const int s = i & 1, r = i % kRing;
       wait(&b->gfull[r], i / kRing);
       wait(&b->kfull[s], i >> 1);
-      if (aborted()) break;
+      if (warp_aborted()) break;
       const Block& k = b->blk[r];
       const int nt = k.nt, units = (nt + 15) / 16;
       const int from = live ? nt : 0;            // tokens from here on count as zeros, whatever they hold
@@ -1017,7 +1020,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     for (int j = 0; j < HV; ++j) S[j] = 0.f;
 #pragma unroll 1
     for (int i = -1; i < nblk; ++i) {
-      if (aborted()) break;
+      if (warp_aborted()) break;
       if (i >= 0) {
         // S after the block: the products' update, and the state's row at the end of a piece
         wait(&b->gfull[i % kRing], i / kRing);
@@ -1025,6 +1028,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         const uint64_t ff = f2(k.f, k.f), one = f2(k.one, k.one);
         float* dst = k.dst;
         wait(&b->u_done[i & 1], i >> 1);
+        if (warp_aborted()) break;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < HV / 16; ++c) {
@@ -1050,6 +1054,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
       if (STATE || i + 1 >= nblk) continue;
       wait(&b->gfull[(i + 1) % kRing], (i + 1) / kRing);
+      if (warp_aborted()) break;
       const Block& k = b->blk[(i + 1) % kRing];
       if (k.first) {
         const float* src = k.src;
@@ -1076,7 +1081,10 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && aborted()) set_error(a.err, kErrTimeout);
+  if (threadIdx.x == 0 && aborted()) {
+    set_error(a.err, kErrTimeout);
+    if (STATE) ws_meta[blockIdx.x * 2].y = 0x7FC00000;   // NaN: what is chained onto this piece is none
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
