@@ -127,15 +127,23 @@ AIR_DEVICE int snap(const LinAttnArgs& a, int p, int total, int longest, int nb,
 __device__ __noinline__ Range make_range(const LinAttnArgs& a, int r, int R, int* order) {
   const int lane = threadIdx.x & 31;
   const int nb = lane < a.N ? seq_blocks(a, lane) : 0;
+  // Disjoint sequences have at most T / C + N blocks, which times H stays below 2^30. Offsets that go back and
+  // forth can name any number: such a call is reported and does nothing.
+  const int limit = a.T / C + a.N;
   int total = nb, most = nb;
   for (int n = lane + 32; n < a.N; n += 32) {
     const int x = seq_blocks(a, n);
-    total += x;
+    total = min(total + x, limit + 1);
     most = max(most, x);
   }
-  total = __reduce_add_sync(0xffffffffu, total) * a.H;
+  const int64_t sum = (int64_t)__reduce_add_sync(0xffffffffu, total >> 16) * 65536 + __reduce_add_sync(0xffffffffu, total & 0xFFFF);
   most = __reduce_max_sync(0xffffffffu, most);
   Range g{};
+  if (sum > limit) {
+    if (lane == 0) set_error(a.err, kErrBounds);
+    return g;
+  }
+  total = (int)sum * a.H;
   int per = (total + R - 1) / R;
   const int longest = 2 * max(per, kMinCut);
   if (most <= longest) {

@@ -84,3 +84,20 @@ def test_block_oracle_is_the_recurrence():
     init = torch.randn(3, 4, 8, 16, generator=torch.Generator().manual_seed(1))
     for a, b in zip(_by_blocks(q, k, v, g, lens, init, -0.3), _oracle(q, k, v, g, lens, init, -0.3)):
         torch.testing.assert_close(a, b, rtol=1e-11, atol=1e-11)
+
+
+# ---------------------------------------------------------------------------------- malformed offsets
+@gpu
+@pytest.mark.parametrize("H", [2, 80])
+def test_offsets_that_name_more_tokens_than_there_are(H):
+    """0, T, 0, T, ...: every second sequence is valid by itself, together they hold T many times over (enough of them
+    would pass 32 bits of blocks). The call reports it and writes nothing."""
+    T, N, d = 1000, 64, 64
+    q, k, v, g = (x.to(DEV) for x in _inputs(1, T, H, 1, 1, 1, d, d, torch.bfloat16))
+    pool = torch.ones(N, H, d, d, device=DEV)
+    out = torch.full((T, H, d), 3.0, dtype=torch.bfloat16, device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, T] * (N // 2) + [0], dtype=torch.int32, device=DEV)
+    ops.linear_attention(q, k, v, g, state=pool, cu_seqlens=cu, out=out, has_state=torch.ones(N, dtype=torch.int32, device=DEV),
+                         err=err)
+    assert int(err) == 1 and bool((out == 3).all()) and bool((pool == 1).all())
