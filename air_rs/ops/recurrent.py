@@ -44,8 +44,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     ``has_state[n]`` (int32; None: every sequence starts from zeros). Rows of one call are distinct.
     Returns out [T, H, dv] in q's type. bf16 prompts with head sizes 64 / 128 run on the tensor
     cores in blocks of 128 tokens (P and the state's copy that the queries read are rounded to bf16,
-    the state itself stays f32); there a NaN or infinity in v reaches the outputs of its whole block,
-    also those of earlier tokens. Tokens outside every sequence are not written.
+    the state itself stays f32). No token reaches the outputs of earlier ones, also where it holds NaN
+    or infinities; there an infinity in k or v may become NaN, in v it makes its column's outputs NaN
+    from its token on. Tokens outside every sequence are not written.
     """
     out = require_ext().linear_attention(q, k, v, log_decay, state, cu_seqlens, slots, has_state, scale, out,
                                          _err(q) if err is None else err)

@@ -18,7 +18,9 @@
 // A CTA has 20 warps, each with one task, that pass blocks on through mbarriers (every wait is bounded): copies;
 // decays (sums of log decays within 32 tokens, so that no difference of large sums is taken); the two groups
 // of products, Q K^T / Q S / P V and W V, issued by one thread each; scores -> P and O -> output; keys -> W;
-// the state. W goes through a ring of 16 tokens at a time, so that its production and W V overlap, and W V
+// the state. The state's warps also look at V for NaN and infinities, while they wait for W V: P V, where 0 times
+// them would reach earlier tokens' outputs, gets them as zeros (W V does not), and the output's warps write NaN to
+// their columns from their token on. W goes through a ring of 16 tokens at a time, so that its production and W V overlap, and W V
 // of a block overlaps Q K^T, P and P V. The tasks' code is kept short (rolled loops, waits as a call): when
 // it did not fit the instruction cache the same work took four times as long.
 //
@@ -395,10 +397,12 @@ struct Bars {
   uint64_t qfull, qempty;
   uint64_t sc_done, qs_done, o_done, o_scaled, o_free, s_ready, drain[2];
   // pairs: the waiting side may be two phases behind (for o_staged: copies that wait for a late description)
-  uint64_t p_ready[2], u_done[2], u_free[2], o_staged[2];
+  uint64_t p_ready[2], u_done[2], u_free[2], o_staged[2], v_clean[2];
   uint64_t kt_ready[4], kt_free[4];
   uint32_t tmem;
   int abort;
+  alignas(8) uint8_t odd[2][8];    // V's tile had NaN or infinities in its first, second, .. 16 rows
+  uint8_t first[2][8][128];        // then: the first row of each column that had (C: none)
   Range range;
   int order[kSort];
   Block blk[kRing];
@@ -417,6 +421,47 @@ AIR_DEVICE bool elect() {
 constexpr uint32_t kSC = 0, kP = 0, kKT = 128, kO = 256, kU = 384;
 // The state-only kernel has neither scores nor O and takes two regions for U in turn.
 template <bool STATE> AIR_DEVICE uint32_t u_cols(int i) { return STATE && (i & 1) ? kO : kU; }
+
+// NaN and infinities in rows [x0, x1) of V's tile (warp-wide, at most 16 rows): 0 x NaN and 0 x infinity are NaN, so a
+// sum of 0 x v is 0 or tells. 4 rows x 128 bytes of a panel an access.
+template <int DV>
+AIR_DEVICE bool odd_rows(const uint8_t* tile, int x0, int x1) {
+  const int lane = threadIdx.x & 31;
+  uint32_t sum[2] = {0u, 0u};
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const int x = x0 + 4 * y + lane / 8;
+#pragma unroll
+    for (int p = 0; p < DV / 64; ++p) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (x < x1) v = *reinterpret_cast<const uint4*>(tile + p * C * 128 + x * 128 + 16 * (lane & 7));
+      sum[0] = bf2_fma(v.y, 0u, bf2_fma(v.x, 0u, sum[0]));
+      sum[1] = bf2_fma(v.w, 0u, bf2_fma(v.z, 0u, sum[1]));
+    }
+  }
+  return __any_sync(0xffffffffu, (sum[0] | sum[1]) != 0u);
+}
+// Turns them into zeros; the first row of each column that had one goes to first (C: none).
+template <int DV>
+__device__ __noinline__ void clear_odd_rows(uint8_t* tile, int x0, int x1, uint8_t* first) {
+  const int lane = threadIdx.x & 31;
+  if (lane < DV / 8) {                       // eight columns a lane
+    first += 8 * lane;
+    for (int e = 0; e < 8; ++e) first[e] = C;
+#pragma unroll 1
+    for (int x = x0; x < x1; ++x) {
+      uint16_t* v = reinterpret_cast<uint16_t*>(tile + (lane >> 3) * C * 128 + x * 128 + (((lane ^ x) & 7) << 4));
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        if ((v[e] & 0x7F80u) != 0x7F80u) continue;
+        v[e] = 0;
+        if (first[e] == C) first[e] = (uint8_t)x;
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
 
 // STATE: the state-only pass over each range's cut-off last piece.
 template <int DK, int DV, bool STATE>
@@ -452,6 +497,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&b->u_done[i], 1);
       mbar_init(&b->u_free[i], 8);
       mbar_init(&b->o_staged[i], 4);
+      mbar_init(&b->v_clean[i], 8);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&b->kt_ready[i], 4);
@@ -602,6 +648,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             }
             // O (+)= P V
             wait(&b->vfull[s], i >> 1);
+            wait(&b->v_clean[s], i >> 1);
             wait(&b->p_ready[s], i >> 1);
             if (in) wait(&b->o_scaled, n_in);
             else if (i >= 1) wait(&b->o_free, i - 1);
@@ -905,6 +952,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (i + 1 < nblk) fetch(i + 1);
         wait(&b->o_done, i);
         wait(&b->u_done[s], u);            // the state's products are done with V, too
+        wait(&b->v_clean[s], u);
         if (warp_aborted()) break;
         tc_fence_after();
         // 32 full rows leave through the tile of V, which the products have finished with, as copies of
@@ -934,6 +982,15 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               *reinterpret_cast<uint4*>(out + 32 * c + 8 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+        }
+        if (*reinterpret_cast<const uint64_t*>(b->odd[s]) != 0u) {
+#pragma unroll 1
+          for (int x = 0; x < 8 * DV; ++x) {
+            const int part = x / DV, c = x % DV;
+            if (!b->odd[s][part] || row < b->first[s][part][c] || row >= o_nt) continue;
+            if (full) *reinterpret_cast<uint16_t*>(stage + (c >> 6) * C * 128 + ((((c & 63) >> 3) ^ (lane & 7)) << 4) + 2 * (c & 7)) = 0x7FFF;
+            else reinterpret_cast<uint16_t*>(out)[c] = 0x7FFF;
           }
         }
         fence_proxy_async_smem();
@@ -1035,8 +1092,23 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         const Block& k = b->blk[i % kRing];
         const uint64_t ff = f2(k.f, k.f), one = f2(k.one, k.one);
         float* dst = k.dst;
+        uint8_t* vt = smem + M::kV + (i & 1) * M::kVTile;
+        const int x0 = 16 * (warp - 12), x1 = min(x0 + 16, k.nt);
+        bool odd = false;
+        if constexpr (!STATE) {
+          wait(&b->vfull[i & 1], i >> 1);
+          odd = odd_rows<DV>(vt, x0, x1);
+          if (lane == 0) {
+            b->odd[i & 1][warp - 12] = odd;
+            if (!odd) mbar_arrive(&b->v_clean[i & 1]);
+          }
+        }
         wait(&b->u_done[i & 1], i >> 1);
         if (warp_aborted()) break;
+        if (!STATE && odd) {                     // W V has taken them as they are
+          clear_odd_rows<DV>(vt, x0, x1, b->first[i & 1][warp - 12]);
+          if (lane == 0) mbar_arrive(&b->v_clean[i & 1]);
+        }
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < HV / 16; ++c) {

@@ -101,3 +101,68 @@ def test_offsets_that_name_more_tokens_than_there_are(H):
     ops.linear_attention(q, k, v, g, state=pool, cu_seqlens=cu, out=out, has_state=torch.ones(N, dtype=torch.int32, device=DEV),
                          err=err)
     assert int(err) == 1 and bool((out == 3).all()) and bool((pool == 1).all())
+
+
+# ---------------------------------------------------------------------------------- NaN and infinities
+def _bad_v(T, Hv, dv, seed):
+    """Values with NaN and infinities in single entries, a whole token, and a sequence's first and last tokens, and
+    the first such token of each head and column (T: none)."""
+    r = torch.Generator().manual_seed(seed)
+    bad = torch.zeros(T, Hv, dv)
+    put = torch.tensor([float("nan"), float("inf"), -float("inf")])
+    for t, h, c in ((T - 1, 0, 3), (T // 2, 0, 5), (T // 2 + 1, 0, 5), (T // 3, Hv - 1, dv - 1), (0, Hv - 1, 9)):
+        bad[t, h, c] = put[int(torch.randint(0, 3, (1,), generator=r))]
+    bad[(2 * T) // 3, Hv - 1] = float("nan")
+    odd = bad != 0
+    first = torch.where(odd.any(0), odd.int().argmax(0), torch.full((Hv, dv), T))
+    return bad, first
+
+
+@gpu
+@pytest.mark.parametrize("dk,dv", [(128, 128), (128, 64), (64, 128), (64, 64)])
+@pytest.mark.parametrize("T", [13, 100, 128, 300, 2600])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nan_and_infinities_in_v_do_not_reach_earlier_tokens(T, dk, dv, dtype):
+    """o_t depends on tokens up to t: before a NaN or an infinity of its column it is what the finite values give,
+    from it on it is not finite; other columns stay as they are. The state's columns likewise."""
+    if dtype == torch.float32 and T > 300:
+        pytest.skip("the token-by-token form has no split")
+    H = 2
+    q, k, v, g = _inputs(T + dk, T, H, H, H, H, dk, dv, dtype)
+    bad, first = _bad_v(T, H, dv, T)
+    out, st, mag, sm = _by_blocks(q, k, v, g, [T], torch.zeros(1, H, dv, dk), 1.0)
+    vb = torch.where(bad != 0, bad, v.float()).to(dtype)
+    pool = torch.zeros(1, H, dv, dk, device=DEV)
+    got = ops.linear_attention(q.to(DEV), k.to(DEV), vb.to(DEV), g.to(DEV), state=pool, scale=1.0).cpu()
+    early = torch.arange(T)[:, None, None] < first[None]
+    assert bool(torch.isfinite(got[early]).all()) and not bool(torch.isfinite(got[~early]).any())
+    # the sums up to a token hold the finite values alone, those after it are not looked at
+    zero = torch.zeros(())
+    fine = _by_blocks(q, k, torch.where(bad != 0, zero, v.float()).to(dtype), g, [T], torch.zeros(1, H, dv, dk), 1.0)
+    co, cs = _c(T, dk, dtype == torch.bfloat16)
+    _near(torch.where(early, got.double(), 0.0), torch.where(early, fine[0], 0.0), mag, co, dtype == torch.bfloat16)
+    whole = (first == T)[None, :, :, None].expand_as(st)
+    assert not bool(torch.isfinite(pool.cpu()[~whole]).any())
+    _near(torch.where(whole, pool.cpu().double(), 0.0), torch.where(whole, st, 0.0), sm, cs, False)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_in_one_sequence_stays_there(d):
+    """Packed sequences that share a CTA's tiles: one with NaN in v between two without."""
+    lens, H = [200, 77, 300, 128], 3
+    T = sum(lens)
+    q, k, v, g = _inputs(d, T, H, H, H, H, d, d, torch.bfloat16)
+    out, st, mag, sm = _by_blocks(q, k, v, g, lens, torch.zeros(4, H, d, d), 1.0)
+    vb = v.clone()
+    vb[210] = float("nan")
+    vb[277 + 299, 1, 7] = float("inf")
+    pool = torch.zeros(4, H, d, d, device=DEV)
+    got = ops.linear_attention(q.to(DEV), k.to(DEV), vb.to(DEV), g.to(DEV), state=pool, cu_seqlens=_cu(lens), scale=1.0).cpu()
+    keep = torch.ones(T, H, d, dtype=torch.bool)
+    keep[210:277] = False
+    keep[576, 1, 7] = False
+    assert bool(torch.isnan(got[~keep]).all())
+    co, cs = _c(max(lens), d, True)
+    _near(torch.where(keep, got.double(), 0.0), torch.where(keep, out, 0.0), mag, co, True)
+    _near(pool[[0, 3]], st[[0, 3]], sm[[0, 3]], cs, False)
