@@ -53,11 +53,12 @@ AIR_DEVICE SeqView seq_view(const LinAttnArgs& a, int n) {
   SeqView s;
   s.t0 = a.cu ? a.cu[n] : n;
   s.t1 = a.cu ? a.cu[n + 1] : a.whole ? a.T : n + 1;
-  if (s.t0 < 0 || s.t1 < s.t0 || s.t1 > a.T) {
+  s.slot = a.state ? (a.slots ? (int64_t)a.slots[n] : (int64_t)n) : -1;
+  if (s.t0 < 0 || s.t1 < s.t0 || s.t1 > a.T) {   // skipped: no tokens, and its state stays
     set_error(a.err, kErrBounds);
     s.t0 = s.t1 = 0;
+    s.slot = -1;
   }
-  s.slot = a.state ? (a.slots ? (int64_t)a.slots[n] : (int64_t)n) : -1;
   if (s.slot >= a.S) {
     set_error(a.err, kErrBounds);
     s.slot = -1;

@@ -56,12 +56,13 @@ constexpr float kFloor = -104.f;   // exp(-104) is 0 in f32: one token's decay n
 struct Pos { int n, h, c; };       // sequence, head, block
 
 AIR_DEVICE int seq_begin(const LinAttnArgs& a, int n) { return a.cu ? a.cu[n] : 0; }
+// Tokens of sequence n, -1 where its offsets are out of range: it is skipped like an empty one, and keeps its state.
 AIR_DEVICE int seq_len(const LinAttnArgs& a, int n) {
   if (!a.cu) return a.T;
   const int t0 = a.cu[n], t1 = a.cu[n + 1];
   if (t0 < 0 || t1 < t0 || t1 > a.T) {
     set_error(a.err, kErrBounds);
-    return 0;
+    return -1;
   }
   return t1 - t0;
 }
@@ -120,7 +121,7 @@ AIR_DEVICE int snap(const LinAttnArgs& a, int p, int total, int longest, int nb,
   if (2 * c < len) return p - c;
   if (++pos.h == a.H) {
     pos.h = 0;
-    do { ++pos.n; } while (pos.n < a.N && seq_len(a, pos.n) == 0);
+    do { ++pos.n; } while (pos.n < a.N && seq_len(a, pos.n) <= 0);
   }
   return p + len - c;
 }
@@ -222,7 +223,7 @@ struct Walk {
     p.c = 0;
     if (++p.h < a.H) return;
     p.h = 0;
-    do { ++p.n; } while (p.n < a.N && seq_len(a, p.n) == 0);
+    do { ++p.n; } while (p.n < a.N && seq_len(a, p.n) <= 0);
     load();
   }
 };
@@ -607,7 +608,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       if constexpr (!STATE) {
         // empty sequences keep their state, or zeros when they are fresh
         for (int n = blockIdx.x; n < a.N; n += gridDim.x) {
-          if (seq_len(a, n) > 0 || seq_init(a, n)) continue;
+          if (seq_len(a, n) != 0 || seq_init(a, n)) continue;
           const int64_t slot = seq_slot(a, n);
           if (slot < 0) continue;
           float4* dst = reinterpret_cast<float4*>(a.state + (size_t)slot * a.H * DV * DK);

@@ -103,6 +103,26 @@ def test_offsets_that_name_more_tokens_than_there_are(H):
     assert int(err) == 1 and bool((out == 3).all()) and bool((pool == 1).all())
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_sequence_with_bad_offsets_keeps_its_state(dtype):
+    """Offsets past the tokens, and offsets that go back: those sequences are skipped, fresh or not; the others run."""
+    T, H, d = 40, 2, 64
+    q, k, v, g = _inputs(1, T, H, H, H, H, d, d, dtype)
+    out, st, mag, sm = _oracle(q[:20], k[:20], v[:20], g[:20], [20], torch.zeros(1, H, d, d), 0.125)
+    for fresh in (True, False):
+        pool = torch.full((4, H, d, d), 2.0, device=DEV)
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        has = torch.tensor([0] + [int(not fresh)] * 3, dtype=torch.int32, device=DEV)
+        cu = torch.tensor([0, 20, 50, 40, 40], dtype=torch.int32, device=DEV)
+        got = ops.linear_attention(*(x.to(DEV) for x in (q, k, v, g)), state=pool, cu_seqlens=cu, has_state=has, err=err)
+        assert int(err) == 1
+        co, cs = _c(20, d, dtype == torch.bfloat16)
+        _near(got[:20], out, mag, co, dtype == torch.bfloat16)
+        _near(pool[:1], st, sm, cs, False)
+        assert bool((pool[1:3] == 2).all()) and bool((pool[3] == (0 if fresh else 2)).all())
+
+
 # ---------------------------------------------------------------------------------- NaN and infinities
 def _bad_v(T, Hv, dv, seed):
     """Values with NaN and infinities in single entries, a whole token, and a sequence's first and last tokens, and
