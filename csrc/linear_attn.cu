@@ -59,11 +59,10 @@ AIR_DEVICE SeqView seq_view(const LinAttnArgs& a, int n) {
     s.t0 = s.t1 = 0;
     s.slot = -1;
   }
-  if (s.slot >= a.S) {
+  if (s.slot < -1 || s.slot >= a.S) {
     set_error(a.err, kErrBounds);
     s.slot = -1;
   }
-  if (s.slot < 0) s.slot = -1;
   s.init = s.slot >= 0 && (a.has_state ? a.has_state[n] != 0 : a.has_state_all != 0);
   return s;
 }

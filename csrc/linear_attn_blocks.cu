@@ -70,7 +70,7 @@ AIR_DEVICE int seq_blocks(const LinAttnArgs& a, int n) { return (seq_len(a, n) +
 AIR_DEVICE int64_t seq_slot(const LinAttnArgs& a, int n) {
   if (!a.state) return -1;
   const int64_t s = a.slots ? (int64_t)a.slots[n] : (int64_t)n;
-  if (s >= a.S) set_error(a.err, kErrBounds);
+  if (s < -1 || s >= a.S) set_error(a.err, kErrBounds);
   return s < 0 || s >= a.S ? -1 : s;
 }
 AIR_DEVICE bool seq_init(const LinAttnArgs& a, int n) {

@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const LogitRulesA
   int64_t crow = -1;
   if (a.counts) {
     crow = a.count_row ? a.count_row[row] : row;
-    if (crow >= a.S) {
+    if (crow < -1 || crow >= a.S) {
       set_error(a.err, kErrBounds);
       crow = -1;
     }

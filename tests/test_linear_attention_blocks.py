@@ -123,6 +123,27 @@ def test_a_sequence_with_bad_offsets_keeps_its_state(dtype):
         assert bool((pool[1:3] == 2).all()) and bool((pool[3] == (0 if fresh else 2)).all())
 
 
+@gpu
+@pytest.mark.parametrize("row", [-2, -2 ** 31, 3, 2 ** 31 - 1])
+def test_rows_out_of_range_are_reported_and_count_as_none(row):
+    d = 64
+    q, k, v, g = (x.to(DEV) for x in _inputs(1, 40, 2, 2, 2, 2, d, d, torch.bfloat16))
+    pool = torch.ones(3, 2, d, d, device=DEV)
+    at = torch.tensor([row], dtype=torch.int32, device=DEV)
+    word = lambda: torch.zeros(1, dtype=torch.int32, device=DEV)
+    for T in (40, 3):                       # block form, token by token
+        err = word()
+        got = ops.linear_attention(q[:T], k[:T], v[:T], g[:T], state=pool, slots=at, err=err)
+        assert int(err) == 1 and torch.equal(got, ops.linear_attention(q[:T], k[:T], v[:T], g[:T]))
+    err = word()
+    assert not ops.linear_attention_step(q[:1], k[:1], v[:1], g[:1], pool, slots=at, err=err).any() and int(err) == 1
+    assert bool((pool == 1).all())
+    err = word()
+    counts = torch.ones(3, 8, dtype=torch.uint8, device=DEV)
+    x = ops.logit_rules(torch.ones(1, 8, device=DEV), counts=counts, presence=torch.ones(1, device=DEV), count_row=at, err=err)
+    assert int(err) == 1 and bool((x == 1).all())
+
+
 # ---------------------------------------------------------------------------------- NaN and infinities
 def _bad_v(T, Hv, dv, seed):
     """Values with NaN and infinities in single entries, a whole token, and a sequence's first and last tokens, and
