@@ -313,6 +313,8 @@ def _sampler_part(device, B: int, chunks: int) -> torch.Tensor:
 
 
 def count_tokens(counts, tokens, n: int | None = None, per_row: int = 0, count_row=None):
+    """Adds token i to row ``count_row[i]`` of counts uint8 [S, V], up to 255 (``count_row`` None: row i). With ``per_row`` > 0
+    the row index is i // per_row instead of i. Tokens and rows out of range count nothing."""
     n = n if n is not None else tokens.numel()
     require_ext().count_tokens(counts, tokens, n, per_row, count_row)
     count_launch()

@@ -253,7 +253,7 @@ void sampler_greedy_merge(Tensor part_all, int64_t W, int64_t B, int64_t nch, Te
 
 void count_tokens(Tensor counts, Tensor tokens, int64_t n, int64_t per_row,
                   optional<Tensor> count_row) {
-  air::launch_count_tokens(ptr<uint8_t>(counts), (int)counts.size(1), ptr<int>(tokens), (int)n,
+  air::launch_count_tokens(ptr<uint8_t>(counts), counts.size(0), (int)counts.size(1), ptr<int>(tokens), (int)n,
                            (int)per_row, ptr<int>(count_row), stream());
   post_launch("count_tokens");
 }

@@ -308,14 +308,14 @@ sampler_kernel(const float* __restrict__ logits, int V, int64_t ld, SamplerArgs 
 }
 
 // counts[row, tok] += 1 (saturating at 255) for each new token; used after sampling.
-__global__ void count_tokens_kernel(uint8_t* counts, int V, const int* tokens, int n, int per_row,
+__global__ void count_tokens_kernel(uint8_t* counts, int64_t rows, int V, const int* tokens, int n, int per_row,
                                     const int* count_row) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n) return;
   int row = per_row > 0 ? i / per_row : i;
   if (count_row) row = count_row[row];
   const int t = tokens[i];
-  if (t < 0 || t >= V || row < 0) return;
+  if (t < 0 || t >= V || row < 0 || row >= rows) return;
   uint8_t* c = counts + (size_t)row * V + t;
   // byte atomics are not available: use a 32-bit CAS on the containing word
   unsigned int* w = reinterpret_cast<unsigned int*>(reinterpret_cast<uintptr_t>(c) & ~(uintptr_t)3);
@@ -357,10 +357,10 @@ void launch_sampler_greedy_merge(const float4* part_all, int W, int B, int nch, 
   if (step) bump_step_kernel<<<1, 1, 0, st>>>(step);
 }
 
-void launch_count_tokens(uint8_t* counts, int V, const int* tokens, int n, int per_row,
+void launch_count_tokens(uint8_t* counts, int64_t rows, int V, const int* tokens, int n, int per_row,
                          const int* count_row, cudaStream_t st) {
   if (n <= 0) return;
-  count_tokens_kernel<<<(n + 255) / 256, 256, 0, st>>>(counts, V, tokens, n, per_row, count_row);
+  count_tokens_kernel<<<(n + 255) / 256, 256, 0, st>>>(counts, rows, V, tokens, n, per_row, count_row);
 }
 
 }  // namespace air

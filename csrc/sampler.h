@@ -35,7 +35,7 @@ void launch_sampler_partial(const float* logits, int B, int V, int nch, int64_t 
                             cudaStream_t st);
 void launch_sampler_greedy_merge(const float4* part_all, int W, int B, int nch, int* out_tokens,
                                  float* out_prob, long long* step, cudaStream_t st);
-void launch_count_tokens(uint8_t* counts, int V, const int* tokens, int n, int per_row,
+void launch_count_tokens(uint8_t* counts, int64_t rows, int V, const int* tokens, int n, int per_row,
                          const int* count_row, cudaStream_t st);
 
 }  // namespace air
