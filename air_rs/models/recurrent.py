@@ -110,14 +110,19 @@ class RecurrentDecoder:
 
     def prefill(self, prompts: list[list[int]], slots: torch.Tensor, resume: torch.Tensor | None = None) -> torch.Tensor:
         """Runs the prompts packed together into the state rows ``slots`` (int32); ``resume`` (int32)
-        marks those that continue what their row holds. Returns the logits of each last token."""
+        marks those that continue what their row holds, the others start from a zero state and zero
+        counts. Returns the logits of each last token."""
         if any(not p for p in prompts):
             raise ValueError("prefill: a prompt has at least one token")
+        if slots.shape != (len(prompts),) or (resume is not None and resume.shape != slots.shape):
+            raise ValueError(f"prefill: one state row (and resume mark) for each of {len(prompts)} prompts")
         ids = torch.tensor([t for p in prompts for t in p], dtype=torch.int32, device=self.device)
         cu = torch.tensor([0] + [len(p) for p in prompts], dtype=torch.int32, device=self.device).cumsum(0, dtype=torch.int32)
-        for n, p in enumerate(prompts):
-            rows = slots[n:n + 1].expand(len(p)).contiguous()
-            ops.count_tokens(self.counts, ids[int(sum(map(len, prompts[:n]))):][:len(p)], count_row=rows, per_row=1)
+        fresh = torch.ones_like(slots, dtype=torch.bool) if resume is None else resume == 0
+        rows = torch.arange(self.max_seqs, device=self.device)
+        self.counts.masked_fill_(((rows[:, None] == slots) & fresh).any(1, keepdim=True), 0)
+        of_token = torch.tensor([n for n, p in enumerate(prompts) for _ in p], dtype=torch.int64, device=self.device)
+        ops.count_tokens(self.counts, ids, count_row=slots[of_token], per_row=1)
 
         def mixer(i, q, k, v, g):
             return ops.linear_attention(q, k, v, g, state=self.states[i], cu_seqlens=cu, slots=slots, has_state=resume,
@@ -140,7 +145,6 @@ class RecurrentDecoder:
         if B > self.max_seqs:
             raise ValueError(f"generate: {B} prompts, {self.max_seqs} state rows")
         slots = torch.arange(B, dtype=torch.int32, device=dev)
-        self.counts[:B].zero_()
         row = lambda v: torch.full((B,), float(v), dtype=torch.float32, device=dev)
         rules = dict(counts=self.counts, count_row=slots, repetition=row(repetition), frequency=row(frequency),
                      presence=row(presence), bias=ops.bias_lists(bias, dev) if bias else None, mask=mask, err=self.err)

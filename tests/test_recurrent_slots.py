@@ -23,3 +23,38 @@ def test_count_tokens_skips_rows_and_tokens_out_of_range():
     ops.count_tokens(buf[:2], _i32(5, 5, 5))                     # three tokens, two rows
     want[0, 5] = want[1, 5] = 1
     assert torch.equal(buf.cpu(), want)
+
+
+def _counts(m, prompts):
+    want = torch.zeros(m.max_seqs, m.cfg.vocab_size, dtype=torch.int64)
+    for slot, ids in prompts.items():
+        want[slot] = torch.bincount(torch.tensor(ids), minlength=m.cfg.vocab_size)
+    return want.clamp(max=255)
+
+
+@gpu
+def test_a_reused_slot_starts_with_its_own_counts():
+    m = RecurrentDecoder.random(RecurrentConfig(), max_seqs=4)
+    m.prefill([[1, 2, 2], [5] * 300], _i32(3, 1))
+    assert torch.equal(m.counts.cpu().long(), _counts(m, {3: [1, 2, 2], 1: [5] * 300}))
+    # slot 3 goes to another request, slot 1 continues, slot 0 is new
+    m.prefill([[7, 1], [5, 6], [9]], _i32(3, 1, 0), resume=_i32(0, 1, 0))
+    assert torch.equal(m.counts.cpu().long(), _counts(m, {3: [7, 1], 1: [5] * 302 + [6], 0: [9]}))
+    # rows out of range change nothing, and are reported
+    before = m.counts.clone()
+    m.prefill([[2], [3]], _i32(-1, 4))
+    assert torch.equal(m.counts, before) and int(m.err) == 1
+    for bad in (dict(slots=_i32(0)), dict(slots=_i32(0, 1), resume=_i32(1))):
+        with pytest.raises(ValueError):
+            m.prefill([[2], [3]], **bad)
+    assert torch.equal(m.counts, before)
+
+
+@gpu
+def test_generate_does_not_see_an_earlier_request():
+    cfg = RecurrentConfig()
+    m = RecurrentDecoder.random(cfg, max_seqs=2)
+    prompts = [[5, 6, 7], [11]]
+    first = m.generate(prompts, 6, presence=1e4)
+    m.generate([[1, 2, 3] * 50], 20, presence=1e4)
+    assert m.generate(prompts, 6, presence=1e4) == first
