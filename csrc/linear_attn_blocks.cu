@@ -16,7 +16,7 @@
 // whole state 32 times a block.
 //
 // A CTA has 20 warps, each with one task, that pass blocks on through mbarriers (every wait is bounded): copies;
-// decays (sums of log decays within 32 tokens, so that no difference of large sums is taken); the two groups
+// decays (sums of log decays within 32 tokens; a difference of sums is taken for two tokens of one 32 only); the two groups
 // of products, Q K^T / Q S / P V and W V, issued by one thread each; scores -> P and O -> output; keys -> W;
 // the state. The state's warps also look at V for NaN and infinities, while they wait for W V: P V, where 0 times
 // them would reach earlier tokens' outputs, gets them as zeros (W V does not), and the output's warps write NaN to
@@ -855,15 +855,15 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           if (!in) mbar_arrive(&b->qempty);
         }
         tc_fence_after();
-        float x = rs;                      // log2 of the decay from the end of 32 c to the row
         // rolled loops: the roles' code has to stay in the instruction cache together
 #pragma unroll 1
         for (int c = 0; c < q; ++c) {
           uint32_t pk[16];
           float v[32];
           tmem_ld32(trow + kSC + 32 * c, v);
-          x -= k.t2[c];
-          const float f = ex2(x) * a.scale;
+          // the decay from the end of 32 c to the row, of its own terms: taken off rs it would keep the rounding
+          // of whatever the earlier 32s decay by
+          const float f = ex2(gl + (c < 1 && q > 1 ? k.t2[1] : 0.f) + (c < 2 && q > 2 ? k.t2[2] : 0.f)) * a.scale;
           const uint64_t ff = f2(f, f);
           const float4* e4 = reinterpret_cast<const float4*>(&k.e[32 * c]);
 #pragma unroll

@@ -207,3 +207,26 @@ def test_nan_in_one_sequence_stays_there(d):
     co, cs = _c(max(lens), d, True)
     _near(torch.where(keep, got.double(), 0.0), torch.where(keep, out, 0.0), mag, co, True)
     _near(pool[[0, 3]], st[[0, 3]], sm[[0, 3]], cs, False)
+
+
+# ---------------------------------------------------------------------------------- decays
+@gpu
+def test_decays_after_strong_ones_keep_their_exponents():
+    """64 tokens that forget everything, then none that decay: row i's factor for a token of the third 32 is 1. Taken as a
+    difference of sums from the block's first token (9200 in log2, steps of 2^-10) it would be off by 2^-11 in the
+    exponent wherever the two strong 32s' sum rounds, 3.4e-4 relatively. The scores lie 1.2e-4 (2^-13) on either side of
+    the middle of two bf16 numbers, so each output is an exact number."""
+    T, H, d = 128, 16, 64
+    q, k, v = (torch.zeros(T, H, d) for _ in range(3))
+    k[70, :, :3] = torch.tensor([1.0, 2.0 ** -8 - 2.0 ** -13, 2.0 ** -8 + 2.0 ** -13])
+    q[:, :, 0] = 1
+    q[0::2, :, 1] = q[1::2, :, 2] = 1            # scores 1 + 2^-8 -+ 2^-13
+    v[70] = 1
+    g = torch.zeros(T, H)
+    g[:32] = -100.0 - 0.03 * torch.arange(H)
+    g[32:64] = -99.0
+    args = [x.to(torch.bfloat16).to(DEV) for x in (q, k, v)]
+    got = ops.linear_attention(*args, g.to(DEV), scale=1.0).float().cpu()
+    assert not got[:70].any()
+    assert bool((got[96::2] == 1).all()) and bool((got[97::2] == 1 + 2.0 ** -7).all())
+    assert bool((got[70:96:2] == 1).all()) and bool((got[71:96:2] == 1 + 2.0 ** -7).all())
