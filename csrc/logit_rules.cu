@@ -29,7 +29,7 @@ struct Entries {
 // 43 with one tile a CTA, 41 with 16 a stretch.
 template <bool VEC, bool BF16>
 __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const LogitRulesArgs a, int tiles) {
-  __shared__ float pw[2][kTable];
+  __shared__ float pw[kTable];
   __shared__ int ids[kThreads];
   __shared__ float vals[kThreads];
   __shared__ int wn[kThreads / 32];
@@ -81,11 +81,7 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const LogitRulesA
   load(first, next);
   const float rho = cnt && a.repetition ? a.repetition[row] : 1.f;
   const float fr = cnt && a.frequency ? a.frequency[row] : 0.f, pr = cnt && a.presence ? a.presence[row] : 0.f;
-  if (t < kTable && rho != 1.f) {
-    const float f = powf(rho, (float)t);
-    pw[0][t] = 1.f / f;
-    pw[1][t] = f;
-  }
+  if (t < kTable && rho != 1.f) pw[t] = powf(rho, (float)t);
   int b0 = 0, b1 = 0;
   if (a.bias_ptr) {
     b0 = a.bias_ptr[row];
@@ -142,12 +138,9 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const LogitRulesA
         if (k == 0) continue;
         float& v = x[g][j];
         if (rho != 1.f && v != 0.f) {        // 0 stays 0 even where rho^c overflows
-          if (k < kTable) {
-            v *= pw[v < 0.f][k];
-          } else {
-            const float f = powf(rho, (float)k);
-            v = v < 0.f ? v * f : v / f;
-          }
+          // a quotient: 1 / rho^c is rounded once more, and overflows where rho^c is below 2^-128
+          const float f = k < kTable ? pw[k] : powf(rho, (float)k);
+          v = v < 0.f ? v * f : v / f;
         }
         v = v - fr * (float)k - pr;
       }
