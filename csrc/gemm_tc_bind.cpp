@@ -112,10 +112,17 @@ void gemm_fp8(Tensor wq, Tensor wscale, int64_t row_bytes, int64_t N, int64_t K,
               int64_t mode, int64_t splits, optional<Tensor> ws, optional<Tensor> counters, Tensor err) {
   TORCH_CHECK(wq.is_cuda() && xq.is_cuda() && wscale.scalar_type() == at::kFloat && xs.scalar_type() == at::kFloat,
               "gemm_fp8: CUDA codes and f32 scales");
+  // the kernel reads all of them through bare pointers
+  for (const Tensor* t : {&wq, &wscale, &xs, &out, &err})
+    TORCH_CHECK(t->device() == xq.device(), "gemm_fp8: operands must be on the device of xq");
+  TORCH_CHECK(xq.scalar_type() == at::kByte || xq.scalar_type() == at::kFloat8_e4m3fn, "gemm_fp8: xq must be E4M3 codes (uint8)");
   TORCH_CHECK(K % 128 == 0 && xq.is_contiguous() && xq.dim() == 2 && xq.size(1) == K, "gemm_fp8: xq [T, K]");
   const int64_t T = xq.size(0);
-  TORCH_CHECK(wscale.numel() >= N * (K / 128) && xs.numel() >= T, "gemm_fp8: scale shapes");
-  TORCH_CHECK(out.stride(1) == 1 && out.size(0) >= T && out.size(1) >= N, "gemm_fp8: out [T, N] with contiguous rows");
+  TORCH_CHECK(xs.is_contiguous() && wscale.is_contiguous() && wscale.numel() >= N * (K / 128) && xs.numel() >= T,
+              "gemm_fp8: scale shapes");
+  TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) >= T && out.size(1) >= N && (T == 1 || out.stride(0) >= N),
+              "gemm_fp8: out [T, N] with contiguous rows");
+  TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() >= 1, "gemm_fp8: err must be int32");
   TORCH_CHECK(out.scalar_type() == (mode == air::kGemmStoreBF16 ? at::kBFloat16 : at::kFloat),
               "gemm_fp8: out must be bf16 for the bf16 store, else f32");
   air::GemmF8Args a{};
