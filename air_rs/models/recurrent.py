@@ -144,6 +144,8 @@ class RecurrentDecoder:
         B, dev = len(prompts), self.device
         if B > self.max_seqs:
             raise ValueError(f"generate: {B} prompts, {self.max_seqs} state rows")
+        if not prompts:
+            return []
         slots = torch.arange(B, dtype=torch.int32, device=dev)
         row = lambda v: torch.full((B,), float(v), dtype=torch.float32, device=dev)
         rules = dict(counts=self.counts, count_row=slots, repetition=row(repetition), frequency=row(frequency),

@@ -137,6 +137,8 @@ def linear_fp8(x: torch.Tensor, w: QWeight, out: torch.Tensor, *, residual: bool
     src/w8a8.rs:40-160)."""
     if w.fmt != FMT_FP8 or w.scales is None:
         raise ValueError("linear_fp8 needs block-scaled FP8 weights")
+    if x.shape[0] == 0:
+        return out
     xq, xs = quant_fp8_rows(x)
     return linear_fp8_rows(xq, xs, w, out, residual=residual, splits=splits, err=err)
 

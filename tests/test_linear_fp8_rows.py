@@ -54,3 +54,14 @@ def test_refusals():
     with pytest.raises(ValueError):
         gemm.linear_fp8_rows(xq, xs, ops.QWeight(ops.FMT_BF16, out.bfloat16(), None, T, N, GGMLType.F16), out)
     assert gemm.linear_fp8_rows(xq[:0], xs[:0], w, out[:0]).shape == (0, N)
+    assert gemm.linear_fp8(torch.empty(0, K, dtype=torch.bfloat16, device=DEV), w, out[:0]).shape == (0, N)
+
+
+@gpu
+def test_a_decoder_takes_no_prompts():
+    from air_rs.models.recurrent import RecurrentConfig, RecurrentDecoder
+    m = RecurrentDecoder.random(RecurrentConfig(), max_seqs=2)
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    assert m.prefill([], none).shape == (0, m.cfg.vocab_size) and m.decode(none, none).shape == (0, m.cfg.vocab_size)
+    assert m.generate([], 3) == [] and m.generate([[1]], 0) == [[]]
+    assert not m.counts[1].any() and int(m.err) == 0
