@@ -4,6 +4,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cmath>
+#include <utility>
 
 #include "linear_attn.h"
 #include "logit_rules.h"
@@ -24,6 +25,18 @@ void same_device(const Tensor& t, const Tensor& as, const char* what) {
 void post(const char* what) {
   cudaError_t e = cudaGetLastError();
   TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
+}
+// Rows of an output (two or three dimensions) share no memory: expanded or interleaved ones would be written by
+// several blocks at once.
+void distinct_rows(const Tensor& t, const char* op, const char* what) {
+  const auto sizes = t.sizes(), strides = t.strides();
+  const int last = (int)sizes.size() - 1;
+  int a = 0, b = last - 1;                            // the outer dimension and the next
+  if (sizes[b] > 1 && (sizes[a] <= 1 || strides[a] < strides[b])) std::swap(a, b);
+  const int64_t inner = sizes[b] > 1 && b != a ? (sizes[b] - 1) * strides[b] : 0;
+  const bool ok = (sizes[b] <= 1 || b == a || strides[b] >= sizes[last]) &&
+                  (sizes[a] <= 1 || strides[a] >= inner + sizes[last]);
+  TORCH_CHECK(ok || t.numel() == 0, op, ": the rows of ", what, " overlap or interleave in memory");
 }
 const int* int_row(const optional<Tensor>& t, int64_t n, const Tensor& as, const char* what) {
   if (!t.has_value()) return nullptr;
@@ -73,6 +86,7 @@ air::LinAttnArgs lin_args(const char* op, const Tensor& q, const Tensor& k, cons
     *div[i] = (int)(H / rows[i]->size(1));
   }
   TORCH_CHECK(out.size(1) == H && out.size(2) == dv, op, ": out must be [tokens, ", str(H), ", ", str(dv), "]");
+  distinct_rows(out, op, "out");
   a.q = q.data_ptr();
   a.k = k.data_ptr();
   a.v = v.data_ptr();
@@ -210,12 +224,14 @@ std::tuple<Tensor, Tensor> add_rmsnorm_fp8(Tensor x, optional<Tensor> y, Tensor 
   if (resid.has_value()) {
     rows(*resid, "resid_out");
     TORCH_CHECK(resid->scalar_type() == at::kFloat, "add_rmsnorm_fp8: resid_out float32");
+    distinct_rows(*resid, "add_rmsnorm_fp8", "resid_out");
     a.resid = resid->data_ptr<float>();
     a.ldr = resid->stride(0);
   }
   if (out_bf16.has_value()) {
     rows(*out_bf16, "out_bf16");
     TORCH_CHECK(out_bf16->scalar_type() == at::kBFloat16, "add_rmsnorm_fp8: out_bf16 bfloat16");
+    distinct_rows(*out_bf16, "add_rmsnorm_fp8", "out_bf16");
     a.out_bf16 = out_bf16->data_ptr();
     a.ldo = out_bf16->stride(0);
   }
@@ -251,6 +267,7 @@ void logit_rules(Tensor logits, Tensor out, optional<Tensor> counts, optional<Te
   same_device(out, logits, "out");
   TORCH_CHECK(out.scalar_type() == at::kFloat && out.sizes() == logits.sizes() && (V <= 1 || out.stride(1) == 1),
               "logit_rules: out must be float32 [rows, vocab] with contiguous rows");
+  distinct_rows(out, "logit_rules", "out");
   TORCH_CHECK(B <= 65535 && V < (1ll << 31) - 4096, "logit_rules: at most 65535 rows");
   same_device(err, logits, "err");
   TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() >= 1, "logit_rules: err must be int32");
