@@ -374,5 +374,6 @@ def gated_delta(q, k, v, alpha, beta, state=None):
     return out, state
 
 
+from .gemm import check_errors  # noqa: E402
 from .recurrent import (add_rmsnorm_fp8, bias_lists, linear_attention,  # noqa: E402
                         linear_attention_step, logit_rules)

@@ -70,6 +70,18 @@ def workspace(device) -> _Workspace:
     return w
 
 
+def check_errors(device=None) -> None:
+    """Raises RuntimeError, once, if an operator that was given no ``err`` reported an error on the device (None: the
+    current one) since the last check: an index out of range, or a bounded wait that ran out. Waits for the device.
+    The word is made by the first such call on the device, which is not to be one inside a graph capture."""
+    d = torch.device("cuda" if device is None else device)
+    w = workspace(d if d.index is not None else torch.device("cuda", torch.cuda.current_device()))
+    torch.cuda.synchronize(w.device)
+    if code := int(w.err):
+        w.err.zero_()
+        raise RuntimeError(f"device kernel reported error code {code} (1=index out of range, 2=wait timed out)")
+
+
 def linear(x: torch.Tensor, w: QWeight, out: torch.Tensor, runner=None, *, residual: bool = False,
            splits: int | None = None, err: torch.Tensor | None = None,
            dbg: torch.Tensor | None = None, row_count: torch.Tensor | None = None,

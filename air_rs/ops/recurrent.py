@@ -5,7 +5,7 @@ rows of the W8A8 projections, and the rules a request puts on its logits.
 All take CUDA tensors, run on the current stream without synchronising and can be captured in CUDA
 graphs. Arguments that the host can see are checked before the launch (RuntimeError); indices that
 live on the device are checked in the kernel, which skips the row and sets ``err`` (by default the
-device's shared error word). A state or count row out of range is reported and counts as -1.
+device's shared error word, which ``ops.check_errors`` reads and clears). A state or count row out of range is reported and counts as -1.
 Outputs whose rows overlap or interleave in memory are refused; an output shares no memory with other operands
 except where in-place use is named.
 """

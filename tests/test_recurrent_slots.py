@@ -58,3 +58,22 @@ def test_generate_does_not_see_an_earlier_request():
     first = m.generate(prompts, 6, presence=1e4)
     m.generate([[1, 2, 3] * 50], 20, presence=1e4)
     assert m.generate(prompts, 6, presence=1e4) == first
+
+
+@gpu
+def test_errors_without_a_word_of_ones_own_are_raised_once():
+    ops.check_errors()
+    q = torch.randn(1, 2, 64, device=DEV)
+    pool = torch.zeros(2, 2, 64, 64, device=DEV)
+    g = torch.zeros(2, device=DEV)
+    ops.linear_attention_step(q, q, q, g, pool, slots=_i32(1))
+    ops.check_errors(q.device)
+    ops.linear_attention_step(q, q, q, g, pool, slots=_i32(2))
+    with pytest.raises(RuntimeError, match="code 1"):
+        ops.check_errors(q.device)
+    ops.check_errors()
+    ops.linear_attention_step(q, q, q, g, pool, slots=_i32(2), err=_i32(0))     # a word of one's own
+    ops.check_errors("cuda:0")
+    ops.linear_attention_step(q, q, q, g, pool, slots=_i32(-3))
+    with pytest.raises(RuntimeError):
+        ops.check_errors("cuda")
