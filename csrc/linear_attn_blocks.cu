@@ -1296,7 +1296,10 @@ bool linear_blocks_supported(const LinAttnArgs& a, bool f32) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (heads == 1 || (sh % 8 == 0 && sh > 0)) &&
            (T == 1 || (st % 8 == 0 && st > 0)) && sh < (1ll << 38) && st < (1ll << 38);
   };
-  return !f32 && ((int64_t)a.T / C + a.N) * a.H < (1ll << 30) && (a.dk == 64 || a.dk == 128) && (a.dv == 64 || a.dv == 128) && a.T > 0 &&
+  // A CTA may step over all empty sequences between two blocks, one by one or 148th of the items by turns: up to 2^20 of
+  // them (some 100 clocks each) or 2^17 turns (250) stay far inside the 2^29 clocks after which waits give up.
+  const bool short_walk = (int64_t)a.N * (a.H > 16 ? a.H : 16) <= (1ll << 24);
+  return !f32 && short_walk && ((int64_t)a.T / C + a.N) * a.H < (1ll << 30) && (a.dk == 64 || a.dk == 128) && (a.dv == 64 || a.dv == 128) && a.T > 0 &&
          ok(a.q, a.qs_h, a.qs_t, a.H / a.q_div, a.T) && ok(a.k, a.ks_h, a.ks_t, a.H / a.k_div, a.T) &&
          ok(a.v, a.vs_h, a.vs_t, a.H / a.v_div, a.T) && ok(a.out, a.os_h, a.os_t, a.H, a.T) &&
          reinterpret_cast<uintptr_t>(a.state) % 16 == 0;
