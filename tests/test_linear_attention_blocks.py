@@ -230,3 +230,92 @@ def test_decays_after_strong_ones_keep_their_exponents():
     assert not got[:70].any()
     assert bool((got[96::2] == 1).all()) and bool((got[97::2] == 1 + 2.0 ** -7).all())
     assert bool((got[70:96:2] == 1).all()) and bool((got[71:96:2] == 1 + 2.0 ** -7).all())
+
+
+# ---------------------------------------------------------------------------------- precision and reach
+DIMS = [(128, 128), (128, 64), (64, 128), (64, 64)]
+# lengths, heads: whole items; two sequences that are cut, with an empty one between and a short one behind
+SHAPES = [([300, 129, 5], 4), ([1500, 0, 2100, 7], 3)]
+
+
+def _slow(T, H):
+    """Decays that keep the incoming state for thousands of tokens."""
+    return torch.tensor([3e-4, 7.77e-4, 0.0, 1.1e-3])[:H].neg().expand(T, H).contiguous()
+
+
+@gpu
+@pytest.mark.parametrize("dk,dv", DIMS)
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("slow", [False, True])
+@pytest.mark.parametrize("resume", [False, True])
+def test_state_keeps_32_bits(dk, dv, shape, slow, resume):
+    """Fresh and resumed sequences, whole and cut, for each pair of head sizes. A block's update is 32 accumulation steps
+    (8 times 16 tokens, 4 parts of the keys) that each drop at most 2^-23 of the running sum, half of that in the mean,
+    and the sum's size is 2/3 of its last in the mean: 32 x 2^-24 x 2/3 = 1.3e-6 of the state (2-norm). Exponents: 8
+    roundings of a sum G weigh G exp(-G) <= 0.37, 8 x 0.37 x 2^-24 = 1.8e-7; the updates of S 2^-24 a block, of random
+    sign: 17 blocks 2.5e-7. Without the last part of the decayed keys 3.4e-6 would be missing."""
+    lens, H = SHAPES[shape]
+    T, N = sum(lens), len(lens)
+    q, k, v, g = _inputs(dk + dv + shape, T, H, H, H, H, dk, dv, torch.bfloat16)
+    if slow:
+        g = _slow(T, H)
+    r = torch.Generator().manual_seed(shape)
+    pool = torch.randn(N + 2, H, dv, dk, generator=r)
+    slots = torch.randperm(N + 2, generator=r)[:N]
+    init = pool[slots] * float(resume)
+    out, st, mag, sm = _by_blocks(q, k, v, g, lens, init, 1.0)
+    dpool = pool.to(DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = ops.linear_attention(*(x.to(DEV) for x in (q, k, v, g)), state=dpool, cu_seqlens=_cu(lens), scale=1.0,
+                               slots=slots.to(torch.int32).to(DEV), err=err,
+                               has_state=torch.full((N,), int(resume), dtype=torch.int32, device=DEV))
+    assert int(err) == 0
+    _near(got, out, mag, _c(max(lens), dk, True)[0], True)
+    full = [n for n in range(N) if lens[n]]
+    off = (dpool.cpu()[slots].double() - st)[full].flatten(2).norm(dim=-1) / st[full].flatten(2).norm(dim=-1)
+    assert float(off.max()) < 1.3e-6 + 1.8e-7 + 2.5e-7, off
+    empty = [n for n in range(N) if not lens[n]]
+    assert torch.equal(dpool.cpu()[slots][empty], init[empty])
+    others = torch.ones(N + 2, dtype=torch.bool)
+    others[slots] = False
+    assert torch.equal(dpool.cpu()[others], pool[others])
+
+
+@gpu
+@pytest.mark.parametrize("H,T", [(64, 40), (2, 2100)])
+def test_block_form_with_state_offsets_beyond_32_bits(H, T):
+    """The last row of a pool of more than 2^31 numbers, for a whole sequence and for one that is cut."""
+    d = 128
+    rows = (1 << 31) // (H * d * d) + 2
+    if torch.cuda.mem_get_info()[0] < rows * H * d * d * 4 + (3 << 30):
+        pytest.skip("needs 12 GB of device memory")
+    pool = torch.empty(rows, H, d, d, device=DEV)
+    last = torch.tensor([rows - 1], dtype=torch.int32, device=DEV)
+    init = torch.randn(1, H, d, d, generator=torch.Generator().manual_seed(H))
+    pool[-1:] = init.to(DEV)
+    pool[0] = 0.25
+    q, k, v, _ = _inputs(H, T, H, 2, 2, 2, d, d, torch.bfloat16)
+    g = _slow(T, 2).repeat_interleave(H // 2, 1)
+    out, st, mag, sm = _by_blocks(q, k, v, g, [T], init, 1.0)
+    got = ops.linear_attention(*(x.to(DEV) for x in (q, k, v, g)), state=pool, slots=last, has_state=torch.ones_like(last), scale=1.0)
+    co, cs = _c(T, d, True)
+    _near(got, out, mag, co, True)
+    _near(pool[-1:], st, sm, cs, False)
+    assert bool((pool[0] == 0.25).all())
+
+
+@gpu
+def test_block_form_with_token_offsets_beyond_32_bits():
+    """Outputs of more than 2^31 numbers: the last of the packed sequences against the recurrence."""
+    T, H, d, L = 140000, 128, 128, 200
+    if torch.cuda.mem_get_info()[0] < 4 * T * H * d:
+        pytest.skip("needs 9 GB of device memory")
+    q, k, v, g = _inputs(3, L, 2, 1, 1, 1, d, d, torch.bfloat16)
+    ref, _, mag, _ = _by_blocks(q, k, v, g, [L], torch.zeros(1, 2, d, d), 1.0)
+    rows = lambda x: torch.cat([torch.zeros(T - L, *x.shape[1:], dtype=x.dtype, device=DEV), x.to(DEV)])
+    lens = [T // 2, T - L - T // 2, L]
+    out = ops.linear_attention(rows(q), rows(k), rows(v), rows(g.repeat_interleave(H // 2, 1)), cu_seqlens=_cu(lens), scale=1.0)
+    assert not out[: T - L: 997].any() and not out[T - L - 1].any()
+    co = _c(L, d, True)[0]
+    for h in (0, 63, 64, 127):
+        _near(out[T - L:, h], ref[:, h // 64], mag[:, h // 64], co, True)
