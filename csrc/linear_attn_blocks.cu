@@ -18,10 +18,10 @@
 // A CTA has 20 warps, each with one task, that pass blocks on through mbarriers (every wait is bounded): copies;
 // decays (sums of log decays within 32 tokens; a difference of sums is taken for two tokens of one 32 only); the two groups
 // of products, Q K^T / Q S / P V and W V, issued by one thread each; scores -> P and O -> output; keys -> W;
-// the state. The state's warps also look at V for NaN and infinities, while they wait for W V: P V, where 0 times
-// them would reach earlier tokens' outputs, gets them as zeros (W V does not), and the output's warps write NaN to
-// their columns from their token on. W goes through a ring of 16 tokens at a time, so that its production and W V overlap, and W V
-// of a block overlaps Q K^T, P and P V. The tasks' code is kept short (rolled loops, waits as a call): when
+// the state. NaN and infinities in V show in W V: there the state's warps turn them into zeros before P V, where 0
+// times them would reach earlier tokens' outputs, and the output's warps write NaN to their columns from their
+// token on. W goes through a ring of 16 tokens at a time, so that its production and W V overlap, and W V of a block
+// overlaps Q K^T and P. The tasks' code is kept short (rolled loops, waits as a call): when
 // it did not fit the instruction cache the same work took four times as long.
 //
 // Split over the length: the (sequence, head, block) triples form one list. Where a sequence is longer than
@@ -402,8 +402,8 @@ struct Bars {
   uint64_t kt_ready[4], kt_free[4];
   uint32_t tmem;
   int abort;
-  alignas(8) uint8_t odd[2][8];    // V's tile had NaN or infinities in its first, second, .. 16 rows
-  uint8_t first[2][8][128];        // then: the first row of each column that had (C: none)
+  alignas(8) uint8_t odd[2][8];    // V's tile had NaN or infinities: 4 times 32 rows of the left, of the right columns
+  uint8_t first[2][4][128];        // then: the first row of each column that had (C: none)
   Range range;
   int order[kSort];
   Block blk[kRing];
@@ -423,35 +423,16 @@ constexpr uint32_t kSC = 0, kP = 0, kKT = 128, kO = 256, kU = 384;
 // The state-only kernel has neither scores nor O and takes two regions for U in turn.
 template <bool STATE> AIR_DEVICE uint32_t u_cols(int i) { return STATE && (i & 1) ? kO : kU; }
 
-// NaN and infinities in rows [x0, x1) of V's tile (warp-wide, at most 16 rows): 0 x NaN and 0 x infinity are NaN, so a
-// sum of 0 x v is 0 or tells. 4 rows x 128 bytes of a panel an access.
-template <int DV>
-AIR_DEVICE bool odd_rows(const uint8_t* tile, int x0, int x1) {
-  const int lane = threadIdx.x & 31;
-  uint32_t sum[2] = {0u, 0u};
-#pragma unroll
-  for (int y = 0; y < 4; ++y) {
-    const int x = x0 + 4 * y + lane / 8;
-#pragma unroll
-    for (int p = 0; p < DV / 64; ++p) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (x < x1) v = *reinterpret_cast<const uint4*>(tile + p * C * 128 + x * 128 + 16 * (lane & 7));
-      sum[0] = bf2_fma(v.y, 0u, bf2_fma(v.x, 0u, sum[0]));
-      sum[1] = bf2_fma(v.w, 0u, bf2_fma(v.z, 0u, sum[1]));
-    }
-  }
-  return __any_sync(0xffffffffu, (sum[0] | sum[1]) != 0u);
-}
-// Turns them into zeros; the first row of each column that had one goes to first (C: none).
-template <int DV>
-__device__ __noinline__ void clear_odd_rows(uint8_t* tile, int x0, int x1, uint8_t* first) {
-  const int lane = threadIdx.x & 31;
-  if (lane < DV / 8) {                       // eight columns a lane
-    first += 8 * lane;
+// Turns NaN and infinities in rows [x0, x1) and columns [c0, c0 + n) of V's tile into zeros (warp-wide); the first row
+// of each column that had one goes to first (C: none). Eight columns a lane.
+__device__ __noinline__ void clear_odd(uint8_t* tile, int x0, int x1, int c0, int n, uint8_t* first) {
+  const int lane = threadIdx.x & 31, chunk = c0 / 8 + lane;
+  if (lane < n / 8) {
+    first += 8 * chunk;
     for (int e = 0; e < 8; ++e) first[e] = C;
 #pragma unroll 1
     for (int x = x0; x < x1; ++x) {
-      uint16_t* v = reinterpret_cast<uint16_t*>(tile + (lane >> 3) * C * 128 + x * 128 + (((lane ^ x) & 7) << 4));
+      uint16_t* v = reinterpret_cast<uint16_t*>(tile + (chunk >> 3) * C * 128 + x * 128 + (((chunk ^ x) & 7) << 4));
 #pragma unroll 1
       for (int e = 0; e < 8; ++e) {
         if ((v[e] & 0x7F80u) != 0x7F80u) continue;
@@ -987,9 +968,9 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         if (*reinterpret_cast<const uint64_t*>(b->odd[s]) != 0u) {
 #pragma unroll 1
-          for (int x = 0; x < 8 * DV; ++x) {
+          for (int x = 0; x < 4 * DV; ++x) {
             const int part = x / DV, c = x % DV;
-            if (!b->odd[s][part] || row < b->first[s][part][c] || row >= o_nt) continue;
+            if (!b->odd[s][4 * (c / (DV / 2)) + part] || row < b->first[s][part][c] || row >= o_nt) continue;
             if (full) *reinterpret_cast<uint16_t*>(stage + (c >> 6) * C * 128 + ((((c & 63) >> 3) ^ (lane & 7)) << 4) + 2 * (c & 7)) = 0x7FFF;
             else reinterpret_cast<uint16_t*>(out)[c] = 0x7FFF;
           }
@@ -1093,24 +1074,11 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         const Block& k = b->blk[i % kRing];
         const uint64_t ff = f2(k.f, k.f), one = f2(k.one, k.one);
         float* dst = k.dst;
-        uint8_t* vt = smem + M::kV + (i & 1) * M::kVTile;
-        const int x0 = 16 * (warp - 12), x1 = min(x0 + 16, k.nt);
-        bool odd = false;
-        if constexpr (!STATE) {
-          wait(&b->vfull[i & 1], i >> 1);
-          odd = odd_rows<DV>(vt, x0, x1);
-          if (lane == 0) {
-            b->odd[i & 1][warp - 12] = odd;
-            if (!odd) mbar_arrive(&b->v_clean[i & 1]);
-          }
-        }
+        const int nt = k.nt;
         wait(&b->u_done[i & 1], i >> 1);
         if (warp_aborted()) break;
-        if (!STATE && odd) {                     // W V has taken them as they are
-          clear_odd_rows<DV>(vt, x0, x1, b->first[i & 1][warp - 12]);
-          if (lane == 0) mbar_arrive(&b->v_clean[i & 1]);
-        }
         tc_fence_after();
+        uint64_t z = 0;                          // 0 x the update: not 0 where it has NaN or infinities
 #pragma unroll
         for (int c = 0; c < HV / 16; ++c) {
           float v[16];
@@ -1118,6 +1086,7 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const uint64_t x = f2(S[16 * c + j], S[16 * c + j + 1]);
+            if (!STATE) z = fma2(f2(v[j], v[j + 1]), 0, z);
             unf2(fma2(x, one, fma2(x, ff, f2(v[j], v[j + 1]))), S[16 * c + j], S[16 * c + j + 1]);
           }
         }
@@ -1126,6 +1095,15 @@ linear_blocks_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (lane == 0) {
           mbar_arrive(&b->u_free[i & 1]);
           mbar_arrive(&b->gempty[i % kRing]);
+        }
+        if constexpr (!STATE) {
+          // a column of the update is finite where V's column is: else this warp's 32 tokens of V are gone through
+          const bool odd = __any_sync(0xffffffffu, z != 0);
+          if (odd) clear_odd(smem + M::kV + (i & 1) * M::kVTile, 32 * q, min(32 * q + 32, nt), half * HV, HV, b->first[i & 1][q]);
+          if (lane == 0) {
+            b->odd[i & 1][warp - 12] = odd;
+            mbar_arrive(&b->v_clean[i & 1]);
+          }
         }
         if (dst && live) {
           float* d = dst + half * HV * DK + k0;
