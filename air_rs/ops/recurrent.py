@@ -45,10 +45,13 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     ``slots[n]`` (None: n; -1: starts from zeros and keeps nothing) and starts from that row where
     ``has_state[n]`` (int32; None: every sequence starts from zeros). Rows of one call are distinct.
     Returns out [T, H, dv] in q's type. bf16 prompts with head sizes 64 / 128 run on the tensor
-    cores in blocks of 128 tokens (P and the state's copy that the queries read are rounded to bf16,
-    the state itself stays f32). No token reaches the outputs of earlier ones, also where it holds NaN
-    or infinities; there an infinity in k or v may become NaN, in v it makes its column's outputs NaN
-    from its token on. Tokens outside every sequence are not written.
+    cores in blocks of 128 tokens, unless there are 12 tokens or fewer or less than 1.5 a sequence
+    (empty ones counted), which like all others run token by token. In blocks the decayed scores and
+    the state's copy that the queries read are rounded to bf16 (an output error of 2.35e-3 where one
+    rounding of exact outputs has 1.66e-3); the state itself stays f32. No token reaches the outputs of
+    earlier ones, also where it holds NaN or infinities; in blocks an infinity in k or v may become NaN,
+    and in v it makes its column's outputs NaN from its token on. Tokens outside every sequence are not
+    written.
     """
     out = require_ext().linear_attention(q, k, v, log_decay, state, cu_seqlens, slots, has_state, scale, out,
                                          _err(q) if err is None else err)

@@ -16,13 +16,13 @@
 // whole state 32 times a block.
 //
 // A CTA has 20 warps, each with one task, that pass blocks on through mbarriers (every wait is bounded): copies;
-// decays (sums of log decays within 32 tokens; a difference of sums is taken for two tokens of one 32 only); the two groups
-// of products, Q K^T / Q S / P V and W V, issued by one thread each; scores -> P and O -> output; keys -> W;
+// decays (sums of log decays within 32 tokens; a difference of sums is taken for two tokens of the same 32 only); the
+// two groups of products, Q K^T / Q S / P V and W V, issued by one thread each; scores -> P and O -> output; keys -> W;
 // the state. NaN and infinities in V show in W V: there the state's warps turn them into zeros before P V, where 0
 // times them would reach earlier tokens' outputs, and the output's warps write NaN to their columns from their
 // token on. W goes through a ring of 16 tokens at a time, so that its production and W V overlap, and W V of a block
-// overlaps Q K^T and P. The tasks' code is kept short (rolled loops, waits as a call): when
-// it did not fit the instruction cache the same work took four times as long.
+// overlaps Q K^T and P. The tasks' code is kept short (rolled loops, waits as a call): when it did not fit the
+// instruction cache the same work took four times as long.
 //
 // Split over the length: the (sequence, head, block) triples form one list. Where a sequence is longer than
 // two SMs' shares of it, the list is cut into one stretch per SM: a first kernel computes the state that each
@@ -30,10 +30,12 @@
 // starts each stretch from its incoming state. Otherwise whole sequences are dealt out, the longest first.
 // All sums have a fixed order.
 //
-// Measured (B200, 32 heads of 128): about 5600 clocks a block where tensor products need 3600 and the memory
-// 5400 with all SMs at it. One prompt of 16384 tokens: 183 us (64, 9 and 123 for each of the three kernels
-// alone; their ends overlap) of an 83 us floor; 13 ragged prompts of 8111 tokens together: 93 us; 77 tokens: 8.9 us. Bound by shared
-// memory: the products' operands (2300 clocks a block), the warps' accesses (2300) and the copies (1000) share it.
+// Measured (B200): 148 heads of 128, 2048 tokens each, one head per SM: 74.5 us, 7300 clocks a block (SM cycles over 16
+// blocks, set-up included). The tensor pipe is active 49 % of them, tensor memory 53 %, HBM 46 %, L1 and shared
+// memory 38 %: no unit is near its limit. What bounds it is the chain of a block's steps: Q K^T of the next block
+// starts behind P V of this one, because P lies over the scores and Q has one tile. One prompt of 16384 tokens, 32
+// heads: 186 us (71, 9.5 and 127 for each of the three kernels alone; their ends overlap) of an 83 us floor; 13 ragged
+// prompts of 8111 tokens together: 102 to 108 us; 77 tokens, 16 heads of 64: 9.2 us.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <string.h>
@@ -1266,7 +1268,8 @@ const char* launch_dims(const LinAttnArgs& a, float* ws, int sms, cudaStream_t s
 // Few tokens: the block kernel needs about 11 us for its first block whatever that holds, the token-by-token
 // one 2.5 us + 0.55 us a token (32 heads of 128, one sequence: 9.5 against 11.7 us at 12 tokens, 11.8 against
 // 11.7 at 16). Sequences of a token or two each: 16 x 32 heads 12.1 against 33 us at one token, 15.9 against 33
-// at two; 128 x 32 heads 108 against 152 and 154 against 153 (the states' traffic bounds both).
+// at two; 128 x 32 heads 108 against 152 and 154 against 153 (the states' traffic bounds both). Lengths are on the
+// device, so empty sequences count: one prompt of 1000 tokens in 700 slots goes token by token.
 bool linear_blocks_worth(const LinAttnArgs& a) { return a.T > 12 && 2 * (int64_t)a.T > 3 * (int64_t)a.N; }
 
 bool linear_blocks_supported(const LinAttnArgs& a, bool f32) {

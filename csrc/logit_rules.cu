@@ -25,7 +25,7 @@ struct Entries {
 
 // Four entries per thread and tile. VEC: four neighbouring ones in one access (rows and pointers aligned for it,
 // V a multiple of 4), so that a warp reads and writes whole lines; otherwise entries t, t + 128, ... one by one.
-// 192 x 128256 bf16 (175 MB): 37 us with 512-entry tiles and eight of them a stretch, 42 with 2048-entry tiles,
+// 192 x 128256 bf16 (175 MB): 38 us with 512-entry tiles and eight of them a stretch, 42 with 2048-entry tiles,
 // 43 with one tile a CTA, 41 with 16 a stretch.
 template <bool VEC, bool BF16>
 __global__ void __launch_bounds__(kThreads) logit_rules_kernel(const LogitRulesArgs a, int tiles) {
