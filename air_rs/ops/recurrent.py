@@ -102,7 +102,8 @@ def logit_rules(logits: torch.Tensor, *, out: torch.Tensor | None = None, counts
     ``bias`` (ptr int32 [B + 1], ids int32, values f32) as :func:`bias_lists` builds it, repeated ids
     add up in list order; ``mask`` int32 [B, ceil(V / 32)] allow bits. Writes f32 to ``out`` (None:
     in place for f32 logits, a new tensor for bf16) and returns it. A masked entry is -inf whatever
-    its logit was; a row whose mask allows nothing is all -inf."""
+    its logit was; a row whose mask allows nothing is all -inf. Penalties over different counts
+    (repetition over prompt and output, frequency and presence over the output) are two calls."""
     if out is None:
         out = logits if logits.dtype == torch.float32 else torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
     if err is None:

@@ -28,3 +28,21 @@ def test_repetition_powers_near_the_ends_of_the_range(V):
     assert not torch.isnan(got).any()
     over = (f > 3.5e38)
     assert not got[over & (x > 0)].any() and bool(torch.isinf(got[over & (x < 0)]).all())
+
+
+@pytest.mark.gpu
+def test_penalties_over_different_counts_are_two_calls():
+    B, V = 3, 500
+    r = torch.Generator().manual_seed(0)
+    x = torch.randn(B, V, generator=r)
+    out = torch.randint(0, 3, (B, V), generator=r).to(torch.uint8)
+    seen = out + torch.randint(0, 3, (B, V), generator=r).to(torch.uint8)
+    rho, fr, pr = 1.1 + torch.rand(B, generator=r), torch.rand(B, generator=r), torch.rand(B, generator=r)
+    d = lambda t: t.to(DEV)
+    got = ops.logit_rules(ops.logit_rules(d(x), counts=d(seen), repetition=d(rho)), counts=d(out), frequency=d(fr), presence=d(pr))
+    f = rho.double()[:, None] ** seen.double()
+    want = torch.where(x > 0, x.double() / f, x.double() * f)
+    mag = want.abs() + 4
+    want = want - fr.double()[:, None] * out - pr.double()[:, None] * (out > 0)
+    # powf 4 ulp (2^-21), the product or quotient, two differences of numbers up to mag
+    assert bool(((got.cpu().double() - want).abs() <= 2.0 ** -20 * mag).all())
