@@ -377,3 +377,5 @@ def gated_delta(q, k, v, alpha, beta, state=None):
 from .gemm import check_errors  # noqa: E402
 from .recurrent import (add_rmsnorm_fp8, bias_lists, linear_attention,  # noqa: E402
                         linear_attention_step, logit_rules)
+from .state_space import (TokenLogprobs, block_norm, causal_conv, causal_conv_step,  # noqa: E402
+                          selective_scan, selective_scan_step, token_logprobs)

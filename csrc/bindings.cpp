@@ -20,6 +20,7 @@ void register_gds(pybind11::module_& m);
 void register_kv_push(pybind11::module_& m);
 void register_ssm(pybind11::module_& m);
 void register_recurrent(pybind11::module_& m);
+void register_state_space(pybind11::module_& m);
 air::PeerPush peer_push_from_meta(const at::Tensor& meta);
 
 using at::Tensor;
@@ -399,6 +400,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_kv_push(m);
   register_ssm(m);
   register_recurrent(m);
+  register_state_space(m);
   register_comm(m);
   register_gds(m);
 }

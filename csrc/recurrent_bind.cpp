@@ -1,43 +1,16 @@
 // torch <-> kernel adapter of the recurrent-decoder operators: linear attention (prompts and single
 // tokens), residual add + RMSNorm + E4M3 rows, logit rules.
-#include <torch/extension.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
 #include <cmath>
-#include <utility>
 
+#include "bind_util.h"
 #include "linear_attn.h"
 #include "logit_rules.h"
 #include "norm_fp8.h"
 
-using at::Tensor;
-using c10::optional;
+using namespace air_bind;
 
 namespace {
 
-// Numbers enter messages through std::to_string: formatting them with a string stream inside the
-// extension crashed with this image's torch and libstdc++.
-std::string str(int64_t n) { return std::to_string(n); }
-
-void same_device(const Tensor& t, const Tensor& as, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.device() == as.device(), what, " must be on the same CUDA device as the first operand");
-}
-void post(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
-}
-// Rows of an output (two or three dimensions) share no memory: expanded or interleaved ones would be written by
-// several blocks at once.
-void distinct_rows(const Tensor& t, const char* op, const char* what) {
-  const auto sizes = t.sizes(), strides = t.strides();
-  const int last = (int)sizes.size() - 1;
-  int a = 0, b = last - 1;                            // the outer dimension and the next
-  if (sizes[b] > 1 && (sizes[a] <= 1 || strides[a] < strides[b])) std::swap(a, b);
-  const int64_t inner = sizes[b] > 1 && b != a ? (sizes[b] - 1) * strides[b] : 0;
-  const bool ok = (sizes[b] <= 1 || b == a || strides[b] >= sizes[last]) &&
-                  (sizes[a] <= 1 || strides[a] >= inner + sizes[last]);
-  TORCH_CHECK(ok || t.numel() == 0, op, ": the rows of ", what, " overlap or interleave in memory");
-}
 const int* int_row(const optional<Tensor>& t, int64_t n, const Tensor& as, const char* what) {
   if (!t.has_value()) return nullptr;
   same_device(*t, as, what);
@@ -114,12 +87,6 @@ air::LinAttnArgs lin_args(const char* op, const Tensor& q, const Tensor& k, cons
   return a;
 }
 
-// The caller's output, or a new one.
-Tensor or_new(const optional<Tensor>& out, at::IntArrayRef sizes, const Tensor& as, at::ScalarType type) {
-  if (out.has_value()) return *out;
-  TORCH_CHECK(as.is_cuda(), "the operands must be CUDA tensors");
-  return at::empty(sizes, as.options().dtype(type));
-}
 Tensor rows_or_new(const char* op, const optional<Tensor>& out, const Tensor& q, const Tensor& v, const Tensor& decay) {
   TORCH_CHECK(q.dim() == 3 && v.dim() == 3 && decay.dim() >= 1, op, ": q and v must be [tokens, heads, dim], log_decay [.., heads]");
   return or_new(out, {q.size(0), decay.size(-1), v.size(2)}, q, q.scalar_type());

@@ -1,0 +1,128 @@
+// Device helpers of the state-space operators.
+#pragma once
+#include "common.cuh"
+#include "state_space.h"
+
+namespace air {
+
+template <typename T>
+AIR_DEVICE float to_f(T v) {
+  if constexpr (sizeof(T) == 2) return bf2f(v);
+  else return v;
+}
+template <typename T>
+AIR_DEVICE T from_f(float v) {
+  if constexpr (sizeof(T) == 2) return f2bf(v);
+  else return v;
+}
+
+// V consecutive elements as f32: one 16- or 8-byte access, or single elements (V = 1).
+template <typename T, int V>
+AIR_DEVICE void load_v(const T* p, float* f) {
+  if constexpr (V == 1) f[0] = to_f(*p);
+  else if constexpr (sizeof(T) == 2 && V == 8) bf16x8_to_f32(*reinterpret_cast<const uint4*>(p), f);
+  else if constexpr (sizeof(T) == 2 && V == 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+    const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+    f[0] = lo.x; f[1] = lo.y; f[2] = hi.x; f[3] = hi.y;
+  } else {
+    static_assert(sizeof(T) == 4 && V % 4 == 0, "");
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 u = *reinterpret_cast<const float4*>(p + i);
+      f[i] = u.x; f[i + 1] = u.y; f[i + 2] = u.z; f[i + 3] = u.w;
+    }
+  }
+}
+template <typename T, int V>
+AIR_DEVICE void store_v(T* p, const float* f) {
+  if constexpr (V == 1) *p = from_f<T>(f[0]);
+  else if constexpr (sizeof(T) == 2 && V == 8) *reinterpret_cast<uint4*>(p) = f32_to_bf16x8(f);
+  else if constexpr (sizeof(T) == 2 && V == 4) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(f[0], f[1]), hi = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  } else {
+    static_assert(sizeof(T) == 4 && V % 4 == 0, "");
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  }
+}
+
+// 1 / (1 + exp(-x)) and x / (1 + exp(-x)); the division is exact to 2 ulp and 0 where exp(-x) passes 2^126.
+AIR_DEVICE float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+AIR_DEVICE float silu_f(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+
+// log(1 + exp(x)) = max(x, 0) + log(1 + u), u = exp(-|x|) in [0, 1]. The logarithm is u P(u) with P of degree 8 (equal
+// ripple of the relative error, computed for this interval: 3.0e-8, 1.7e-7 with the roundings): small steps keep their
+// relative accuracy, which the logarithm of the rounded sum 1 + u would lose, and it needs no special-function unit.
+AIR_DEVICE float softplus_f(float x) {
+  const float u = __expf(-fabsf(x));
+  float p = fmaf(0.00523269409f, u, -0.0295052398f);
+  p = fmaf(p, u, 0.0782259554f);
+  p = fmaf(p, u, -0.136632457f);
+  p = fmaf(p, u, 0.191060066f);
+  p = fmaf(p, u, -0.24842982f);
+  p = fmaf(p, u, 0.333190978f);
+  p = fmaf(p, u, -0.499994934f);
+  p = fmaf(p, u, 0.99999994f);
+  return x != x ? x : fmaf(p, u, fmaxf(x, 0.f));
+}
+
+// 2^u - 1 for the scan's decays, u = delta A log2(e). Added as h + (2^u - 1) h, a slow decay keeps its rate: 2^u itself,
+// rounded to 24 bits, would change a rate of 2^-10 by 2^-14 of itself at every token. For |u| <= log2(e) / 4 a quartic
+// (equal ripple of the relative error, computed for this interval: 8.5e-8), beyond it the exponential less one.
+AIR_DEVICE float decay_m1(float u) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
+  float p = fmaf(0.00133335532f, u, 0.00964317098f);
+  p = fmaf(p, u, 0.0555043519f);
+  p = fmaf(p, u, 0.240225688f);
+  p = fmaf(p, u, 0.693147182f);
+  return fabsf(u) <= 0.360673761f ? p * u : e - 1.f;
+}
+constexpr float kLog2e = 1.44269504f;
+
+struct SeqRange {
+  int t0, t1;        // tokens [t0, t1)
+  int64_t slot;      // state row, -1: none
+  bool init;         // the state row holds the incoming state
+};
+
+// Sequence n of the batch. Bad offsets: no tokens, and its state stays. A state row out of range: none.
+AIR_DEVICE SeqRange seq_range(const SeqArgs& a, int n, bool report = true) {
+  SeqRange s;
+  s.t0 = a.cu ? a.cu[n] : a.step ? n : 0;
+  s.t1 = a.cu ? a.cu[n + 1] : a.step ? n + 1 : a.T;
+  s.slot = a.S > 0 ? (a.slots ? (int64_t)a.slots[n] : (int64_t)n) : -1;
+  if (s.t0 < 0 || s.t1 < s.t0 || s.t1 > a.T) {
+    if (report) set_error(a.err, kErrBounds);
+    s.t0 = s.t1 = 0;
+    s.slot = -1;
+  }
+  if (s.slot < -1 || s.slot >= a.S) {
+    if (report) set_error(a.err, kErrBounds);
+    s.slot = -1;
+  }
+  s.init = s.slot >= 0 && (a.has_state ? a.has_state[n] != 0 : a.has_state_all != 0);
+  return s;
+}
+
+// The sequence that holds token t among rising offsets, by the whole warp: the last n with cu[n] <= t, in steps that
+// look at 32 offsets each. Whatever the offsets are, the result is in [0, N) and the caller checks its range.
+AIR_DEVICE int seq_of_token(const int* cu, int N, int t) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = N;                        // the sequence is in [lo, hi)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int i = lo + (lane + 1) * step;
+    const unsigned up = __ballot_sync(0xffffffffu, i < hi && cu[i] <= t);
+    const int run = __ffs(~up) - 1;          // lanes whose offset is not past t (32: ffs of 0 is 0)
+    const int k = up == 0xffffffffu ? 32 : run;
+    hi = min(hi, lo + (k + 1) * step);
+    lo += k * step;
+  }
+  return lo;
+}
+
+}  // namespace air
