@@ -111,23 +111,6 @@ AIR_DEVICE void conv_sequence(const ConvArgs& a, int n, int d) {
     if (i < len) taps.apply([&](int j) -> const float* { return ext[i + j]; }, a.silu, out + (int64_t)(s.t0 + i) * a.os);
 }
 
-// One bit for each of the 32 tokens from t0: whether its sequence is sound and holds its W - 1 predecessors.
-template <int W>
-AIR_DEVICE unsigned tokens_inside(const SeqArgs& a, int t0) {
-  const int t = t0 + (threadIdx.x & 31);
-  bool in = false;
-  if (a.cu) {
-    for (int n = seq_of_token(a.cu, a.N, t0); n < a.N; ++n) {
-      const int lo = a.cu[n], hi = a.cu[n + 1];
-      if (lo >= t0 + 32) break;
-      if (lo >= 0 && hi <= a.T) in |= t - lo >= W - 1 && t < hi;
-    }
-  } else {
-    in = t >= W - 1 && t < a.T;
-  }
-  return __ballot_sync(0xffffffffu, in);
-}
-
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const ConvArgs a, int blocks_d, int runs) {
   const int bd = blockIdx.x % blocks_d, unit = blockIdx.x / blocks_d;

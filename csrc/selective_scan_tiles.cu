@@ -1,0 +1,598 @@
+// Selective scan of packed prompts in tiles of tokens.
+//   h = exp(delta A) h + delta x B,   y = (C . h + D x) silu(z)
+//
+// What bounds it: one exponential per token, channel and state. At 16 states an element of x costs 16 exponentials (a
+// quarter of a warp's clock each per scheduler and 4 lanes: 4 clocks) against 8 bytes of bf16 rows, so the special-function
+// and instruction pipes, not memory. The recurrence itself is one chain of multiply-adds a state: independent chains in a thread keep
+// the pipes busy, not occupancy.
+//
+// A block has eight scan warps and four helper warps. L lanes share a pair of channels, each with two states of both: the
+// arithmetic runs on pairs of channels (f32x2), so the steps of a pair are one operand and B and C, stored twice, another,
+// and y of the pair comes out as one. Stage by stage of TS tokens, with one barrier a stage, the helpers turn dt and x of
+// the next stage into delta and delta x, and the lanes' parts of y of the last one into the output (sum, skip, gate,
+// rounding), so all global accesses are theirs: whole rows, copied asynchronously six stages ahead.
+//
+// The tokens of all sequences lie in one row of tiles of equal length; a block walks through its tile and loads or
+// stores a state where a sequence starts or ends, so ragged batches are balanced. With few channels there are several
+// tiles: a first pass then computes what each tile's last sequence adds to the next tile (the state from zero, or from the
+// sequence's initial state, and the sum of delta), and the second pass starts from exp(A sum) times those of the tiles before.
+// That pass doubles the exponentials of sequences that cross tiles, so the host cuts no more than fills the SMs.
+#include <algorithm>
+
+#include "state_space.cuh"
+
+namespace air {
+
+namespace {
+
+#ifndef LB
+#define LB 1
+#endif
+#ifndef KG
+#define KG 4
+#endif
+using f2 = unsigned long long;       // two floats, the operand of the paired instructions
+AIR_DEVICE f2 pack2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+AIR_DEVICE f2 dup2(float a) { return pack2(a, a); }
+AIR_DEVICE void unpack2(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+AIR_DEVICE f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+AIR_DEVICE f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+AIR_DEVICE f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// p = 2^u - 1 where |u| is past the cubic's interval: under a predicate, so lanes that need no exponential keep theirs
+AIR_DEVICE void far_decay(float& p, float u) {
+  asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %1;\n\tsetp.gt.f32 q, a, %2;\n\t"
+      "@q ex2.approx.ftz.f32 a, %1;\n\t@q add.f32 %0, a, 0fBF800000;\n\t}"
+      : "+f"(p) : "f"(u), "f"(kNearDecay));
+}
+// 2^u - 1 of M pairs (decay_m1), step by step over all of them: M independent chains
+template <int M>
+AIR_DEVICE void decays(const f2* u, f2* p) {
+  const f2 c3 = dup2(kDecay3), c2 = dup2(kDecay2), c1 = dup2(kDecay1), c0 = dup2(kDecay0);
+#pragma unroll
+  for (int m = 0; m < M; ++m) p[m] = fma2(c3, u[m], c2);
+#pragma unroll
+  for (int m = 0; m < M; ++m) p[m] = fma2(p[m], u[m], c1);
+#pragma unroll
+  for (int m = 0; m < M; ++m) p[m] = fma2(p[m], u[m], c0);
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    float a, b, ua, ub;
+    unpack2(mul2(p[m], u[m]), a, b);
+    unpack2(u[m], ua, ub);
+    far_decay(a, ua);
+    far_decay(b, ub);
+    p[m] = pack2(a, b);
+  }
+}
+// softplus_f of a pair
+AIR_DEVICE f2 softplus2(float a, float b) {
+  const f2 u = pack2(__expf(-fabsf(a)), __expf(-fabsf(b)));
+  f2 p = fma2(dup2(0.00523269409f), u, dup2(-0.0295052398f));
+  p = fma2(p, u, dup2(0.0782259554f));
+  p = fma2(p, u, dup2(-0.136632457f));
+  p = fma2(p, u, dup2(0.191060066f));
+  p = fma2(p, u, dup2(-0.24842982f));
+  p = fma2(p, u, dup2(0.333190978f));
+  p = fma2(p, u, dup2(-0.499994934f));
+  p = fma2(p, u, dup2(0.99999994f));
+  return fma2(p, u, pack2(fmaxf(a, 0.f), fmaxf(b, 0.f)));
+}
+
+#ifndef LB
+#define LB 1
+#endif
+#ifndef KG
+#define KG 4
+#endif
+constexpr int kGroup = KG;           // tokens whose decays are computed together
+constexpr int kScan = 256, kThreads = kScan + 128;   // eight scan warps, four helper warps
+AIR_DEVICE void stage_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
+template <int L>
+struct Shape {
+  static constexpr int CH = 512 / L, CP = CH / 2;        // channels a block, and pairs
+  static constexpr int TS = L <= 4 ? 8 : 16;             // tokens a stage
+  static constexpr int NP = 2 * L;                       // states, padded
+  static constexpr int E = CH * TS / 128;                // channels of a helper's access
+  static constexpr int HT = CH / E;                      // helpers a token
+};
+constexpr int kRing = 8, kAhead = 6; // stages of raw rows: `kAhead` being fetched, one prepared, one finished
+template <typename T, int L>
+struct Smem {
+  using S = Shape<L>;
+  static constexpr int BC = S::TS * S::NP * 2 / 4;       // groups of four values of B and C a stage
+  alignas(16) float4 step[2][S::TS][S::CP];              // delta of the pair, delta x of the pair
+  alignas(16) float2 bc[2][2][S::TS][S::NP];             // B, C, each value twice
+  alignas(16) float2 y[2][S::TS][S::CP * L];             // the lanes' parts of y of the pair
+  alignas(16) T rows[kRing][3][128][S::E];               // x, dt, z: each helper's own part
+  alignas(16) T raw_bc[kRing][BC][4];
+};
+// Where a pair lies in `step` and a lane's part in `y`: helpers write or read E channels each, and without the exchange
+// the eight helpers of a quarter of a warp would all go to the same banks.
+template <int E>
+AIR_DEVICE int step_slot(int cp) { return cp ^ (cp >> 3 & (E / 2 - 1)); }
+template <int L, int E>
+AIR_DEVICE int y_slot(int cp, int q) {
+  const int i = cp * L + q, helper = cp / (E / 2);
+  return i ^ (helper & 7) << 1;
+}
+
+// The part of a sequence from token t on: [t, hi) of sequence n, or tokens of no (sound) sequence (n = -1).
+struct Segment {
+  int n, lo, hi;
+};
+AIR_DEVICE Segment segment_at(const SeqArgs& a, int t) {
+  if (!a.cu) return {0, 0, a.T};
+  if (a.N == 0) return {-1, 0, a.T};
+  const int n = seq_of_token(a.cu, a.N, t);
+  const int lo = a.cu[n], hi = a.cu[n + 1];
+  if (t < lo) return {-1, t, min(lo, a.T)};
+  if (t >= hi) return {-1, t, a.T};                      // past the last sequence
+  if (lo < 0 || hi > a.T) return {-1, t, min(hi, a.T)};
+  return {n, lo, hi};
+}
+
+struct TileArgs {
+  int tiles, tile;         // tiles, tokens of each (the last one may have fewer)
+  int blocks_g;            // blocks of channels a group
+  float* h;                // [tiles][D][N] what the tile's last sequence leaves for the next tile
+  float* init;             // [tiles][D][N] that sequence's initial state, if it starts in the tile
+  float* sum;              // [tiles][D] sum of delta over its tokens in the tile
+};
+
+// B bytes from global to shared memory (4, 8 or a multiple of 16), zeros instead where `in` is false.
+template <int B>
+AIR_DEVICE void copy_async(void* dst, const void* src, bool in) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (B >= 16) {
+#pragma unroll
+    for (int i = 0; i < B; i += 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                   ::"r"(d + i), "l"(static_cast<const char*>(src) + i), "r"(in ? 16 : 0) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(B), "r"(in ? B : 0) : "memory");
+  }
+}
+
+// ---- helpers: delta and delta x of a stage, B and C, and the output from y. A helper fetches, prepares and finishes the
+// same E channels of the same token of each stage, and the same groups of four values of B and C.
+template <typename T, int L, bool FIRST>
+struct Helper {
+  using S = Shape<L>;
+  using M = Smem<T, L>;
+  static constexpr int E = S::E, NB = (M::BC + 127) / 128;
+  const ScanArgs& a;
+  M& sm;
+  const int tid, tok, c;            // of 128 helpers: token of the stage, first channel in the block
+  const int live;                   // channels there are from c on, up to E
+  const int64_t d, g;               // channel and group in the tensors
+  const bool vec, vec_bc;           // rows (B and C) can be copied in whole accesses
+  const int t0, t1;
+  float bias[E], skip[E];
+
+  AIR_DEVICE Helper(const ScanArgs& a_, M& s, int64_t d0, int64_t group, int left, int v, int start, int end)
+      : a(a_), sm(s), tid(threadIdx.x - kScan), tok(tid / S::HT), c(tid % S::HT * E), live(min(E, left - c)), d(d0 + c), g(group),
+        vec(v & 1), vec_bc(v & 2), t0(start), t1(end) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      bias[i] = a.dt_bias && i < live ? a.dt_bias[d + i] : 0.f;
+      skip[i] = a.skip && i < live ? a.skip[d + i] : 0.f;
+    }
+  }
+  AIR_DEVICE void row(T* dst, const void* base, int64_t stride, int t) {
+    const bool in = t < t1 && live > 0;
+    const T* p = static_cast<const T*>(base) + (in ? (int64_t)t * stride + d : 0);
+    if (vec) copy_async<E * (int)sizeof(T)>(dst, p, in);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) dst[i] = in && i < live ? p[i] : from_f<T>(0.f);
+    }
+  }
+  // Stage k's rows, complete for this helper after arrived() with at most kAhead - 1 stages fetched after it
+  AIR_DEVICE void fetch(int k) {
+    const int t = t0 + k * S::TS + tok, slot = k % kRing;
+    row(sm.rows[slot][0][tid], a.x, a.xs, t);
+    row(sm.rows[slot][1][tid], a.dt, a.ds, t);
+    if (!FIRST && a.z) row(sm.rows[slot][2][tid], a.z, a.zs, t);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int i = tid + 128 * j, which = i / (M::BC / 2), at = i % (M::BC / 2) * 4;
+      if (i >= (FIRST ? M::BC / 2 : M::BC)) break;
+      const int n = at % S::NP, t_ = t0 + k * S::TS + at / S::NP;
+      const bool in = t_ < t1 && n < a.N;
+      const T* p = which ? static_cast<const T*>(a.C) + (in ? t_ * a.cs_t + g * a.cs_g + n : 0)
+                         : static_cast<const T*>(a.B) + (in ? t_ * a.bs_t + g * a.bs_g + n : 0);
+      if (vec_bc) copy_async<4 * (int)sizeof(T)>(sm.raw_bc[slot][i], p, in);
+      else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sm.raw_bc[slot][i][e] = in && n + e < a.N ? p[e] : from_f<T>(0.f);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  AIR_DEVICE void arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
+  // Tokens past the end change nothing: their step is zero.
+  AIR_DEVICE void prepare(int k) {
+    const int slot = k % kRing;
+    const bool in = t0 + k * S::TS + tok < t1;
+    float x[E], dt[E];
+    load_v<T, E>(sm.rows[slot][0][tid], x);
+    load_v<T, E>(sm.rows[slot][1][tid], dt);
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      float v = dt[i] + bias[i], w = dt[i + 1] + bias[i + 1];
+      if (a.softplus) unpack2(softplus2(v, w), v, w);
+      if (!in) v = w = 0.f;
+      sm.step[k & 1][tok][step_slot<E>((c + i) / 2)] = make_float4(v, w, v * x[i], w * x[i + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int i = tid + 128 * j;
+      if (i >= (FIRST ? M::BC / 2 : M::BC)) break;
+      float f[4];
+      load_v<T, 4>(sm.raw_bc[slot][i], f);
+      float4* p = reinterpret_cast<float4*>(&sm.bc[k & 1][0][0][0] + i * 4);
+      p[0] = make_float4(f[0], f[0], f[1], f[1]);
+      p[1] = make_float4(f[2], f[2], f[3], f[3]);
+    }
+  }
+  AIR_DEVICE void finish(int k, unsigned mask) {
+    if (live <= 0 || !(mask >> tok & 1)) return;
+    const int t = t0 + k * S::TS + tok, slot = k % kRing;
+    float y[E], f[E];
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      f2 sum = 0ull;
+#pragma unroll
+      for (int q = 0; q < L; q += 2) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.y[k & 1][tok][y_slot<L, E>((c + i) / 2, q)]);
+        sum = q ? add2(sum, add2(v.x, v.y)) : add2(v.x, v.y);
+      }
+      unpack2(sum, y[i], y[i + 1]);
+    }
+    if (a.skip) {
+      load_v<T, E>(sm.rows[slot][0][tid], f);
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = fmaf(skip[i], f[i], y[i]);
+    }
+    if (a.z) {
+      load_v<T, E>(sm.rows[slot][2][tid], f);
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] *= silu_f(f[i]);
+    }
+    T* o = static_cast<T*>(a.out) + (int64_t)t * a.os + d;
+    if (vec) store_v<T, E>(o, y);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i < live) o[i] = from_f<T>(y[i]);
+    }
+  }
+};
+
+// ---- scan warps: two states of two channels a lane, as pairs over the channels
+template <typename T, int L>
+struct Scan {
+  using S = Shape<L>;
+  const ScanArgs& a;
+  Smem<T, L>& sm;
+  const int q, cp;                  // lane among the pair's L, pair in the block
+  const int64_t d;                  // first channel
+  const int left;                   // channels there are from it on
+  const int slot, part;             // of the pair in `step`, of the lane in `y`
+  const bool whole;
+  f2 A[2], h[2];
+
+  AIR_DEVICE Scan(const ScanArgs& a_, Smem<T, L>& s, int64_t d0, int left_)
+      : a(a_), sm(s), q(threadIdx.x % L), cp(threadIdx.x / L), d(d0 + cp * 2), left(left_ - cp * 2), slot(step_slot<S::E>(cp)),
+        part(y_slot<L, S::E>(cp, q)), whole(a_.N % 2 == 0 && reinterpret_cast<uintptr_t>(a_.state) % 8 == 0) {
+    float v[2][2];
+    rows(a.A, v, false);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) A[i] = pack2(v[0][i] * kLog2e, v[1][i] * kLog2e);
+    zero();
+  }
+  AIR_DEVICE void zero() { h[0] = h[1] = 0ull; }
+  // v[channel][state] of [D][N] rows; `al`: the two states of a lane are one aligned access
+  AIR_DEVICE void rows(const float* base, float (&v)[2][2], bool al) const {
+#pragma unroll
+    for (int s_ = 0; s_ < 2; ++s_) {
+      const float* p = base + (d + s_) * a.N + q * 2;
+      v[s_][0] = v[s_][1] = 0.f;
+      if (s_ >= left) continue;
+      if (al && q * 2 < a.N) load_v<float, 2>(p, v[s_]);
+      else if (!al) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (q * 2 + i < a.N) v[s_][i] = p[i];
+      }
+    }
+  }
+  AIR_DEVICE void load(const float* base, bool al) {      // one sequence's rows (of the pool or scratch)
+    float v[2][2];
+    rows(base, v, al);
+    h[0] = pack2(v[0][0], v[1][0]);
+    h[1] = pack2(v[0][1], v[1][1]);
+  }
+  AIR_DEVICE void store(float* base, bool al) const {
+    float v[2][2];
+    unpack2(h[0], v[0][0], v[1][0]);
+    unpack2(h[1], v[0][1], v[1][1]);
+#pragma unroll
+    for (int s_ = 0; s_ < 2; ++s_) {
+      float* p = base + (d + s_) * a.N + q * 2;
+      if (s_ >= left) continue;
+      if (al && q * 2 < a.N) store_v<float, 2>(p, v[s_]);
+      else if (!al) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (q * 2 + i < a.N) p[i] = v[s_][i];
+      }
+    }
+  }
+  // K tokens from i on: first all their decays (K independent chains a state), then the chain through h. `sum`: of delta.
+  template <bool OUT, int K>
+  AIR_DEVICE void tokens(int buf, int i, f2& sum) {
+    f2 u[K * 2], p[K * 2], dx[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(&sm.step[buf][i + k][slot]);
+      dx[k] = st.y;
+      if (!OUT) sum = add2(sum, st.x);
+      u[k * 2] = mul2(st.x, A[0]);
+      u[k * 2 + 1] = mul2(st.x, A[1]);
+    }
+    decays<K * 2>(u, p);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sm.bc[buf][0][i + k][q * 2]);
+      h[0] = fma2(p[k * 2], h[0], fma2(dx[k], B.x, h[0]));
+      h[1] = fma2(p[k * 2 + 1], h[1], fma2(dx[k], B.y, h[1]));
+      if (OUT) {
+        const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sm.bc[buf][1][i + k][q * 2]);
+        *reinterpret_cast<f2*>(&sm.y[buf][i + k][part]) = fma2(C.y, h[1], mul2(C.x, h[0]));
+      }
+    }
+  }
+};
+
+AIR_DEVICE bool starts_from(const SeqArgs& a, int n, int64_t& slot) {
+  const SeqRange s = seq_range(a, n, false);
+  slot = s.slot;
+  return s.init;
+}
+
+template <typename T, int L, bool FIRST>
+__global__ void __launch_bounds__(kThreads, LB) scan_tiles_kernel(const __grid_constant__ ScanArgs a, const __grid_constant__ TileArgs ta, int vec) {
+  using S = Shape<L>;
+  extern __shared__ __align__(16) uint8_t raw_smem[];
+  Smem<T, L>& sm = *reinterpret_cast<Smem<T, L>*>(raw_smem);
+  const int blocks = ta.blocks_g * a.G;
+  const int tile = blockIdx.x / blocks, blk = blockIdx.x % blocks;
+  const int per_group = a.D / a.G, grp = blk / ta.blocks_g, first_ch = blk % ta.blocks_g * S::CH;
+  const int left = per_group - first_ch;                     // channels of the group from here on
+  const int64_t d0 = (int64_t)grp * per_group + first_ch;
+  int t0 = tile * ta.tile;
+  const int t1 = (int)min((int64_t)a.seq.T, (int64_t)t0 + ta.tile);
+  Segment seg;
+  if (FIRST) {
+    seg = segment_at(a.seq, t1 - 1);
+    if (seg.n < 0 || seg.hi <= t1) return;                   // nothing goes on in the next tile
+    t0 = max(t0, seg.lo);
+  } else {
+    seg = segment_at(a.seq, t0);
+  }
+  const bool idle = !FIRST && seg.n < 0 && seg.hi >= t1;      // no token of the tile is in a sequence
+  const int stages = idle ? 0 : (t1 - t0 + S::TS - 1) / S::TS;
+  const int64_t row = (int64_t)a.D * a.N;
+
+  if (threadIdx.x >= kScan) {
+    Helper<T, L, FIRST> w(a, sm, d0, grp, left, vec, t0, t1);
+    if (stages > 0) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) w.fetch(k);
+      w.arrived();
+      w.prepare(0);
+    }
+    stage_barrier();
+    if (!FIRST && tile < ta.tiles && a.seq.S > 0) {
+      // offsets and rows that are not sound are reported once, empty sequences without a state start one of zeros
+      for (int n = tile * 128 + w.tid; n < a.seq.N; n += ta.tiles * 128) {
+        const SeqRange s = seq_range(a.seq, n, blk == 0);
+        if (a.seq.cu && s.slot >= 0 && s.t0 == s.t1 && !s.init)
+          for (int64_t i = d0 * a.N; i < (d0 + min(left, S::CH)) * a.N; ++i) a.state[s.slot * row + i] = 0.f;
+      }
+    } else if (!FIRST && blk == 0) {
+      for (int n = tile * 128 + w.tid; n < a.seq.N; n += ta.tiles * 128) seq_range(a.seq, n);
+    }
+    for (int k = 0; k < stages; ++k) {
+      w.fetch(k + kAhead);
+      w.arrived();
+      if (k + 1 < stages) w.prepare(k + 1);
+      if (!FIRST && k > 0) {
+        const int t = t0 + (k - 1) * S::TS;
+        unsigned mask = ~0u;
+        if (seg.n < 0 || t < seg.lo || t + S::TS > seg.hi) {
+          mask = tokens_inside<1>(a.seq, t);
+          seg = segment_at(a.seq, min(t + S::TS, a.seq.T - 1));
+        }
+        w.finish(k - 1, mask & (t + S::TS <= t1 ? ~0u : (1u << (t1 - t)) - 1));
+      }
+      stage_barrier();
+    }
+    if (!FIRST && stages > 0) {
+      const int t = t0 + (stages - 1) * S::TS;
+      w.finish(stages - 1, tokens_inside<1>(a.seq, t) & (t + S::TS <= t1 ? ~0u : (1u << (t1 - t)) - 1));
+    }
+    return;
+  }
+
+  Scan<T, L> w(a, sm, d0, left);
+  const bool al = a.N % 2 == 0;                              // scratch is aligned
+  auto enter = [&](int t) {                                  // the state before token t of seg
+    w.zero();
+    if (seg.n < 0) return;
+    int64_t slot;
+    if (seg.lo == t) {
+      if (!starts_from(a.seq, seg.n, slot)) {
+        if (FIRST) w.store(ta.init + tile * row, al);
+        return;
+      }
+      // where the sequence ends in another tile, that tile's block may have replaced the pool's row already
+      if (!FIRST && ta.tiles > 1 && seg.hi > t1) w.load(ta.init + tile * row, al);
+      else w.load(a.state + slot * row, w.whole);
+      if (FIRST) w.store(ta.init + tile * row, al);
+    } else if (!FIRST && t == tile * ta.tile && tile > 0) {
+      f2 acc[2] = {0ull, 0ull};
+      float sum[2] = {0.f, 0.f};
+      for (int j = tile - 1; j >= 0; --j) {
+        w.load(ta.h + j * row, al);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float u, v;
+          unpack2(mul2(w.A[i], pack2(sum[0], sum[1])), u, v);
+          acc[i] = fma2(pack2(exp2f(u), exp2f(v)), w.h[i], acc[i]);
+        }
+#pragma unroll
+        for (int s_ = 0; s_ < 2; ++s_)
+          if (s_ < w.left) sum[s_] += ta.sum[(int64_t)j * a.D + w.d + s_];
+        if (j * ta.tile <= seg.lo) break;
+      }
+      w.h[0] = acc[0];
+      w.h[1] = acc[1];
+    }
+  };
+  auto leave = [&]() {
+    int64_t slot;
+    if (seg.n < 0) return;
+    starts_from(a.seq, seg.n, slot);
+    if (slot >= 0) w.store(a.state + slot * row, w.whole);
+  };
+  enter(t0);
+  float total[2] = {0.f, 0.f}, low[2] = {0.f, 0.f};          // the sum of delta and what its roundings lost
+  stage_barrier();
+  for (int k = 0; k < stages; ++k) {
+    const int t = t0 + k * S::TS;
+    f2 sum2 = 0ull;
+    if (FIRST || t + S::TS <= seg.hi) {
+#pragma unroll
+      for (int i = 0; i < S::TS; i += kGroup) w.template tokens<!FIRST, kGroup>(k & 1, i, sum2);
+    } else {
+      for (int i = 0; i < S::TS && t + i < t1; ++i) {
+        while (t + i >= seg.hi) {
+          leave();
+          seg = segment_at(a.seq, t + i);
+          enter(t + i);
+        }
+        w.template tokens<!FIRST, 1>(k & 1, i, sum2);
+      }
+    }
+    float sum[2];
+    unpack2(sum2, sum[0], sum[1]);
+    if (FIRST) {
+#pragma unroll
+      for (int s_ = 0; s_ < 2; ++s_) {
+        const float n = total[s_] + sum[s_], back = n - total[s_];
+        low[s_] += (total[s_] - (n - back)) + (sum[s_] - back);
+        total[s_] = n;
+      }
+    }
+    stage_barrier();
+  }
+  if (FIRST) {
+    w.store(ta.h + tile * row, al);
+#pragma unroll
+    for (int s_ = 0; s_ < 2; ++s_)
+      if (w.q == 0 && s_ < w.left) ta.sum[(int64_t)tile * a.D + w.d + s_] = total[s_] + low[s_];
+  } else if (seg.hi <= t1) {
+    leave();
+  }
+}
+
+template <int L>
+int channel_blocks(const ScanArgs& a) {
+  const int per_group = a.D / a.G;
+  return (per_group + Shape<L>::CH - 1) / Shape<L>::CH;
+}
+
+int lanes_of(int N) { return N <= 8 ? 4 : N <= 16 ? 8 : N <= 32 ? 16 : 32; }
+
+template <typename T, int L>
+const char* launch(const ScanArgs& a, const ScanPlan& p, float* ws, cudaStream_t st) {
+  using S = Shape<L>;
+  const int64_t row = (int64_t)a.D * a.N;
+  TileArgs ta{p.tiles, p.tile, channel_blocks<L>(a), ws, ws + p.tiles * row, ws + 2 * p.tiles * row};
+  const int64_t blocks = (int64_t)ta.blocks_g * a.G;
+  if (blocks * p.tiles >= (1ll << 31)) return "selective_scan: too many channels and tokens for one call";
+  auto ok = [](const void* q, int64_t stride, int bytes) {
+    return reinterpret_cast<uintptr_t>(q) % bytes == 0 && stride * (int64_t)sizeof(T) % bytes == 0;
+  };
+  const bool rows = a.D / a.G % 8 == 0 && ok(a.x, a.xs, 16) && ok(a.dt, a.ds, 16) && ok(a.out, a.os, 16) && (!a.z || ok(a.z, a.zs, 16));
+  constexpr int four = 4 * sizeof(T);
+  const bool bc = a.N % 4 == 0 && ok(a.B, a.bs_t, four) && ok(a.C, a.cs_t, four) && (a.G == 1 || (ok(a.B, a.bs_g, four) && ok(a.C, a.cs_g, four)));
+  const int vec = rows + 2 * bc;
+  constexpr int bytes = sizeof(Smem<T, L>);
+  static unsigned long long done1 = 0, done2 = 0;
+  if (!set_max_smem_per_device(scan_tiles_kernel<T, L, true>, bytes, done1) ||
+      !set_max_smem_per_device(scan_tiles_kernel<T, L, false>, bytes, done2))
+    return "selective_scan: the device has too little shared memory";
+  if (p.tiles > 1) scan_tiles_kernel<T, L, true><<<(unsigned)(blocks * (p.tiles - 1)), kThreads, bytes, st>>>(a, ta, vec);
+  scan_tiles_kernel<T, L, false><<<(unsigned)(blocks * p.tiles), kThreads, bytes, st>>>(a, ta, vec);
+  return nullptr;
+}
+
+}  // namespace
+
+ScanPlan scan_plan(const ScanArgs& a, int sms) {
+  const int L = lanes_of(a.N);
+  const int64_t per_group = a.D / a.G, ch = 512 / L;
+  const int64_t blocks = (per_group + ch - 1) / ch * a.G;
+  // Blocks of a wave run at one speed per SM. A cut adds a first pass of 0.8 of the work over what crosses tiles: all of
+  // a long sequence, less of short ones.
+  ScanPlan best{1, a.seq.T, 0};
+  double cost = (double)a.seq.T * ((blocks + sms - 1) / sms);
+  for (int64_t n = 2; n <= 64 && a.seq.T / n >= 64; ++n) {
+    const int64_t tile = ((a.seq.T + n - 1) / n + 15) / 16 * 16;
+    const int64_t tiles = (a.seq.T + tile - 1) / tile;
+    if (tiles < 2) break;
+    const double crossing = std::min(1.0, (double)tiles / std::max(1, a.seq.N));
+    const double c = tile * (double)((blocks * tiles + sms - 1) / sms) +
+                     0.8 * crossing * tile * (double)((blocks * (tiles - 1) + sms - 1) / sms) + 24.0 + tiles;
+    if (c < cost) {
+      cost = c;
+      best = {(int)tiles, (int)tile, (int64_t)tiles * a.D * (2 * a.N + 1)};
+    }
+  }
+  return best;
+}
+
+bool scan_tiles_supported(const ScanArgs& a) { return a.N <= 64; }
+
+const char* launch_scan_tiles(const ScanArgs& a, const ScanPlan& p, float* ws, bool f32, cudaStream_t st) {
+#define AIR_SCAN_L(n) \
+  if (lanes_of(a.N) == n) return f32 ? launch<float, n>(a, p, ws, st) : launch<__nv_bfloat16, n>(a, p, ws, st);
+  AIR_SCAN_L(4)
+  AIR_SCAN_L(8)
+  AIR_SCAN_L(16)
+  AIR_SCAN_L(32)
+#undef AIR_SCAN_L
+  return "selective_scan: too many states";
+}
+
+}  // namespace air

@@ -26,6 +26,12 @@ AIR_DEVICE void load_v(const T* p, float* f) {
     const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
     const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
     f[0] = lo.x; f[1] = lo.y; f[2] = hi.x; f[3] = hi.y;
+  } else if constexpr (sizeof(T) == 2 && V == 2) {
+    const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+    f[0] = lo.x; f[1] = lo.y;
+  } else if constexpr (V == 2) {
+    const float2 lo = *reinterpret_cast<const float2*>(p);
+    f[0] = lo.x; f[1] = lo.y;
   } else {
     static_assert(sizeof(T) == 4 && V % 4 == 0, "");
 #pragma unroll
@@ -42,6 +48,10 @@ AIR_DEVICE void store_v(T* p, const float* f) {
   else if constexpr (sizeof(T) == 2 && V == 4) {
     const __nv_bfloat162 lo = __floats2bfloat162_rn(f[0], f[1]), hi = __floats2bfloat162_rn(f[2], f[3]);
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  } else if constexpr (sizeof(T) == 2 && V == 2) {
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(f[0], f[1]);
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
   } else {
     static_assert(sizeof(T) == 4 && V % 4 == 0, "");
 #pragma unroll
@@ -70,16 +80,16 @@ AIR_DEVICE float softplus_f(float x) {
 }
 
 // 2^u - 1 for the scan's decays, u = delta A log2(e). Added as h + (2^u - 1) h, a slow decay keeps its rate: 2^u itself,
-// rounded to 24 bits, would change a rate of 2^-10 by 2^-14 of itself at every token. For |u| <= log2(e) / 4 a quartic
-// (equal ripple of the relative error, computed for this interval: 8.5e-8), beyond it the exponential less one.
+// rounded to 24 bits, would change a rate of 2^-10 by 2^-14 of itself at every token. For |u| <= log2(e) / 10 a cubic
+// (equal ripple of the relative error, computed for this interval: 1.0e-7, 2.2e-7 with the roundings), beyond it the
+// exponential less one, whose error is then at most 2.4e-6 of the rate.
+constexpr float kNearDecay = 0.144269504f, kDecay0 = 0.693147123f, kDecay1 = 0.240226552f, kDecay2 = 0.0555318594f,
+                kDecay3 = 0.00961812865f;
 AIR_DEVICE float decay_m1(float u) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
-  float p = fmaf(0.00133335532f, u, 0.00964317098f);
-  p = fmaf(p, u, 0.0555043519f);
-  p = fmaf(p, u, 0.240225688f);
-  p = fmaf(p, u, 0.693147182f);
-  return fabsf(u) <= 0.360673761f ? p * u : e - 1.f;
+  const float p = fmaf(fmaf(fmaf(kDecay3, u, kDecay2), u, kDecay1), u, kDecay0);
+  return fabsf(u) <= kNearDecay ? p * u : e - 1.f;
 }
 constexpr float kLog2e = 1.44269504f;
 
@@ -123,6 +133,24 @@ AIR_DEVICE int seq_of_token(const int* cu, int N, int t) {
     lo += k * step;
   }
   return lo;
+}
+
+// One bit for each of the 32 tokens from t0: whether its sequence is sound and holds its W - 1 predecessors. By the
+// whole warp.
+template <int W>
+AIR_DEVICE unsigned tokens_inside(const SeqArgs& a, int t0) {
+  const int t = t0 + (threadIdx.x & 31);
+  bool in = false;
+  if (a.cu) {
+    for (int n = a.N ? seq_of_token(a.cu, a.N, t0) : 0; n < a.N; ++n) {
+      const int lo = a.cu[n], hi = a.cu[n + 1];
+      if (lo >= t0 + 32) break;
+      if (lo >= 0 && hi <= a.T) in |= t - lo >= W - 1 && t < hi;
+    }
+  } else {
+    in = t >= W - 1 && t < a.T;
+  }
+  return __ballot_sync(0xffffffffu, in);
 }
 
 }  // namespace air

@@ -46,6 +46,15 @@ constexpr int kScanMaxStates = 256;
 // Sequences token by token, a few threads per channel: any shape.
 void launch_scan_tokens(const ScanArgs& a, bool f32, cudaStream_t st);
 
+// Prompts in tiles of tokens, at most 64 states: the number of tiles, their tokens and the floats of scratch.
+struct ScanPlan {
+  int tiles, tile;
+  int64_t floats;
+};
+bool scan_tiles_supported(const ScanArgs& a);
+ScanPlan scan_plan(const ScanArgs& a, int sms);
+const char* launch_scan_tiles(const ScanArgs& a, const ScanPlan& p, float* ws, bool f32, cudaStream_t st);
+
 struct BlockNormArgs {
   const void* y;           // [T, K] bf16 or f32
   const void* gate;        // [T, K] of y's type (null: none); ldg = 0: one row for all tokens

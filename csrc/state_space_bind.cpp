@@ -99,7 +99,7 @@ Tensor output(const optional<Tensor>& out, at::IntArrayRef sizes, const Tensor& 
   return out.has_value() ? *out : at::empty(sizes, as.options().dtype(type));
 }
 
-constexpr int64_t kMaxTokens = (1ll << 31) - 64;
+constexpr int64_t kMaxTokens = (1ll << 31) - 4096;   // room for the tokens that blocks look ahead
 
 // Sequences of a prompt call (step = 0) or one token each (step = 1).
 air::SeqArgs sequences(Operands& c, int64_t T, int64_t S, bool has_pool, const optional<Tensor>& cu, const optional<Tensor>& slots,
@@ -234,7 +234,17 @@ Tensor scan(const char* op, const Tensor& x, const Tensor& dt, const Tensor& A, 
   a.N = (int)N;
   a.softplus = softplus;
   TORCH_CHECK(a.seq.N <= (1ll << 31) / (D / 4 + 1), op, ": too many sequences");
-  air::launch_scan_tokens(a, type == at::kFloat, at::cuda::getCurrentCUDAStream());
+  const bool f32 = type == at::kFloat;
+  auto st = at::cuda::getCurrentCUDAStream();
+  if (!step && air::scan_tiles_supported(a)) {
+    const air::ScanPlan p = air::scan_plan(a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+    Tensor ws;                                     // from the allocator's pool of this stream
+    if (p.floats) ws = at::empty({p.floats}, x.options().dtype(at::kFloat));
+    const char* e = air::launch_scan_tiles(a, p, p.floats ? ws.data_ptr<float>() : nullptr, f32, st);
+    TORCH_CHECK(e == nullptr, e ? e : "");
+  } else {
+    air::launch_scan_tokens(a, f32, st);
+  }
   post(op);
   return out;
 }

@@ -7,7 +7,7 @@ logarithm's polynomial 3.0 u with its roundings, the sum dt + bias u (|dt| + |bi
 relatively in softplus: delta is off by (2 |v| + |dt| + |bias| + 10) u relatively.
 
 The scan's bound is carried along the recurrence, one step's new errors at a time: h' = h + (2^g' - 1) h + delta x B has the
-decay's own error (relatively 5 u of 2^g' - 1 for |g| <= 1/4, else 6 u absolutely), the error of g = delta A (relatively that of delta
+decay's own error (relatively 5 u of 2^g' - 1 for |g| <= 1/10, else 6 u absolutely), the error of g = delta A (relatively that of delta
 and 3 u), two roundings of terms of |h| + |b| (each sum is at most that) and those of delta x B.
 """
 import math
@@ -151,7 +151,7 @@ def _scan_ref(x, dt, A, B, C, D, z, bias, softplus, lens, init):
             b, c = B[t].double()[per], C[t].double()[per]
             inp = (delta[t] * x64[t])[:, None] * b
             eg = (ed[t] + 3 * U * delta[t].abs())[:, None] * A.abs()
-            own = torch.where(g.abs() <= 0.249, 5 * U * torch.expm1(g).abs(), 6 * U * torch.maximum(torch.exp(g), torch.ones(())))
+            own = torch.where(g.abs() <= 0.0999, 5 * U * torch.expm1(g).abs(), 6 * U * torch.maximum(torch.exp(g), torch.ones(())))
             a = torch.exp(g)
             e = a * e + (a * eg + own) * h.abs() + 2 * U * (2 * h.abs() + inp.abs()) + \
                 inp.abs() * 2 * U + (ed[t] * x64[t].abs())[:, None] * b.abs()
