@@ -6,7 +6,7 @@
 // and instruction pipes, not memory. The recurrence itself is one chain of multiply-adds a state: independent chains in a thread keep
 // the pipes busy, not occupancy.
 //
-// A block has eight scan warps and four helper warps. L lanes share a pair of channels, each with two states of both: the
+// A block has eight scan warps and eight helper warps. L lanes share a pair of channels, each with two states of both: the
 // arithmetic runs on pairs of channels (f32x2), so the steps of a pair are one operand and B and C, stored twice, another,
 // and y of the pair comes out as one. Stage by stage of TS tokens, with one barrier a stage, the helpers turn dt and x of
 // the next stage into delta and delta x, and the lanes' parts of y of the last one into the output (sum, skip, gate,
@@ -54,29 +54,41 @@ AIR_DEVICE f2 add2(f2 a, f2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// p = 2^u - 1 where |u| is past the cubic's interval: under a predicate, so lanes that need no exponential keep theirs
-AIR_DEVICE void far_decay(float& p, float u) {
-  asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %1;\n\tsetp.gt.f32 q, a, %2;\n\t"
-      "@q ex2.approx.ftz.f32 a, %1;\n\t@q add.f32 %0, a, 0fBF800000;\n\t}"
-      : "+f"(p) : "f"(u), "f"(kNearDecay));
+AIR_DEVICE float exp2_fast(float u) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
+  return e;
 }
-// 2^u - 1 of M pairs (decay_m1), step by step over all of them: M independent chains
+// p = e - 1 where |u| is past the polynomial's interval
+AIR_DEVICE void far_decay(float& p, float u, float e) {
+  asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %1;\n\tsetp.gt.f32 q, a, %2;\n\t@q add.f32 %0, %3, 0fBF800000;\n\t}"
+      : "+f"(p) : "f"(u), "f"(kNearDecay), "f"(e));
+}
+// 2^u - 1 of M pairs (decay_m1), step by step over all of them: M independent chains, and the exponentials beside them
 template <int M>
 AIR_DEVICE void decays(const f2* u, f2* p) {
-  const f2 c3 = dup2(kDecay3), c2 = dup2(kDecay2), c1 = dup2(kDecay1), c0 = dup2(kDecay0);
+  const f2 c2 = dup2(kDecay2), c1 = dup2(kDecay1), c0 = dup2(kDecay0);
+  float e[2 * M];
 #pragma unroll
-  for (int m = 0; m < M; ++m) p[m] = fma2(c3, u[m], c2);
+  for (int m = 0; m < M; ++m) {
+    float ua, ub;
+    unpack2(u[m], ua, ub);
+    e[2 * m] = exp2_fast(ua);
+    e[2 * m + 1] = exp2_fast(ub);
+  }
 #pragma unroll
-  for (int m = 0; m < M; ++m) p[m] = fma2(p[m], u[m], c1);
+  for (int m = 0; m < M; ++m) p[m] = fma2(c2, u[m], c1);
 #pragma unroll
   for (int m = 0; m < M; ++m) p[m] = fma2(p[m], u[m], c0);
 #pragma unroll
+  for (int m = 0; m < M; ++m) p[m] = mul2(p[m], u[m]);
+#pragma unroll
   for (int m = 0; m < M; ++m) {
     float a, b, ua, ub;
-    unpack2(mul2(p[m], u[m]), a, b);
+    unpack2(p[m], a, b);
     unpack2(u[m], ua, ub);
-    far_decay(a, ua);
-    far_decay(b, ub);
+    far_decay(a, ua, e[2 * m]);
+    far_decay(b, ub, e[2 * m + 1]);
     p[m] = pack2(a, b);
   }
 }
@@ -94,14 +106,11 @@ AIR_DEVICE f2 softplus2(float a, float b) {
   return fma2(p, u, pack2(fmaxf(a, 0.f), fmaxf(b, 0.f)));
 }
 
-#ifndef LB
-#define LB 1
-#endif
 #ifndef KG
-#define KG 4
+#define KG 2
 #endif
 constexpr int kGroup = KG;           // tokens whose decays are computed together
-constexpr int kScan = 256, kThreads = kScan + 128;   // eight scan warps, four helper warps
+constexpr int kScan = 256, kHelp = 256, kThreads = kScan + kHelp;   // eight scan warps, eight helper warps
 AIR_DEVICE void stage_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
 template <int L>
@@ -109,7 +118,7 @@ struct Shape {
   static constexpr int CH = 512 / L, CP = CH / 2;        // channels a block, and pairs
   static constexpr int TS = L <= 4 ? 8 : 16;             // tokens a stage
   static constexpr int NP = 2 * L;                       // states, padded
-  static constexpr int E = CH * TS / 128;                // channels of a helper's access
+  static constexpr int E = CH * TS / kHelp > 1 ? CH * TS / kHelp : 2;   // channels of a helper's access
   static constexpr int HT = CH / E;                      // helpers a token
 };
 constexpr int kRing = 8, kAhead = 6; // stages of raw rows: `kAhead` being fetched, one prepared, one finished
@@ -118,9 +127,9 @@ struct Smem {
   using S = Shape<L>;
   static constexpr int BC = S::TS * S::NP * 2 / 4;       // groups of four values of B and C a stage
   alignas(16) float4 step[2][S::TS][S::CP];              // delta of the pair, delta x of the pair
-  alignas(16) float2 bc[2][2][S::TS][S::NP];             // B, C, each value twice
+  alignas(16) float4 bc[2][S::TS][L];                    // B and C of a lane's two states
   alignas(16) float2 y[2][S::TS][S::CP * L];             // the lanes' parts of y of the pair
-  alignas(16) T rows[kRing][3][128][S::E];               // x, dt, z: each helper's own part
+  alignas(16) T rows[kRing][3][kHelp][S::E];               // x, dt, z: each helper's own part
   alignas(16) T raw_bc[kRing][BC][4];
 };
 // Where a pair lies in `step` and a lane's part in `y`: helpers write or read E channels each, and without the exchange
@@ -176,85 +185,110 @@ template <typename T, int L, bool FIRST>
 struct Helper {
   using S = Shape<L>;
   using M = Smem<T, L>;
-  static constexpr int E = S::E, NB = (M::BC + 127) / 128;
+  static constexpr int E = S::E, NB = (M::BC + kHelp - 1) / kHelp;
   const ScanArgs& a;
   M& sm;
-  const int tid, tok, c;            // of 128 helpers: token of the stage, first channel in the block
+  const int tid, tok, c;            // helper: token of the stage, first channel in the block
   const int live;                   // channels there are from c on, up to E
-  const int64_t d, g;               // channel and group in the tensors
   const bool vec, vec_bc;           // rows (B and C) can be copied in whole accesses
-  const int t0, t1;
+  const int t1;
+  int tf, tb[NB];                   // tokens of the next fetch
+  const T *x, *dt, *z, *bc[NB];     // and its rows
+  T* out;                           // row of the next output
+  int64_t bc_stride[NB];
+  bool has_bc[NB];                  // padded states have none
+  int ring;                         // stages fetched, as a place in the ring
   float bias[E], skip[E];
 
-  AIR_DEVICE Helper(const ScanArgs& a_, M& s, int64_t d0, int64_t group, int left, int v, int start, int end)
-      : a(a_), sm(s), tid(threadIdx.x - kScan), tok(tid / S::HT), c(tid % S::HT * E), live(min(E, left - c)), d(d0 + c), g(group),
-        vec(v & 1), vec_bc(v & 2), t0(start), t1(end) {
+  AIR_DEVICE Helper(const ScanArgs& a_, M& s, int64_t d0, int64_t g, int left, int v, int t0, int end)
+      : a(a_), sm(s), tid(threadIdx.x - kScan), tok(tid / S::HT), c(tid % S::HT * E),
+        live(tok < S::TS ? max(0, min(E, left - c)) : 0), vec(v & 1), vec_bc(v & 2), t1(end), tf(t0 + tok), ring(0) {
+    const int64_t d = d0 + c;
+    x = static_cast<const T*>(a.x) + (int64_t)tf * a.xs + d;
+    dt = static_cast<const T*>(a.dt) + (int64_t)tf * a.ds + d;
+    z = a.z ? static_cast<const T*>(a.z) + (int64_t)tf * a.zs + d : nullptr;
+    out = static_cast<T*>(a.out) + (int64_t)tf * a.os + d;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       bias[i] = a.dt_bias && i < live ? a.dt_bias[d + i] : 0.f;
       skip[i] = a.skip && i < live ? a.skip[d + i] : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {  // four states of a token of B (the first half of the groups) or C
+      const int i = tid + kHelp * j, at = i % (M::BC / 2) * 4, n = at % S::NP;
+      const bool is_c = i >= M::BC / 2;
+      tb[j] = t0 + at / S::NP;
+      bc_stride[j] = is_c ? a.cs_t : a.bs_t;
+      bc[j] = static_cast<const T*>(is_c ? a.C : a.B) + tb[j] * bc_stride[j] + g * (is_c ? a.cs_g : a.bs_g) + n;
+      has_bc[j] = n < a.N;
+    }
   }
-  AIR_DEVICE void row(T* dst, const void* base, int64_t stride, int t) {
-    const bool in = t < t1 && live > 0;
-    const T* p = static_cast<const T*>(base) + (in ? (int64_t)t * stride + d : 0);
-    if (vec) copy_async<E * (int)sizeof(T)>(dst, p, in);
+  AIR_DEVICE void row(T* dst, const T* p, const void* any, bool in) {
+    if (vec) copy_async<E * (int)sizeof(T)>(dst, in ? p : any, in);
     else {
 #pragma unroll
       for (int i = 0; i < E; ++i) dst[i] = in && i < live ? p[i] : from_f<T>(0.f);
     }
   }
-  // Stage k's rows, complete for this helper after arrived() with at most kAhead - 1 stages fetched after it
-  AIR_DEVICE void fetch(int k) {
-    const int t = t0 + k * S::TS + tok, slot = k % kRing;
-    row(sm.rows[slot][0][tid], a.x, a.xs, t);
-    row(sm.rows[slot][1][tid], a.dt, a.ds, t);
-    if (!FIRST && a.z) row(sm.rows[slot][2][tid], a.z, a.zs, t);
+  // The next stage's rows, complete for this helper after arrived() with at most kAhead - 1 stages fetched after it
+  AIR_DEVICE void fetch() {
+    const bool in = tf < t1 && live > 0;
+    row(sm.rows[ring][0][tid], x, a.x, in);
+    row(sm.rows[ring][1][tid], dt, a.dt, in);
+    if (!FIRST && a.z) row(sm.rows[ring][2][tid], z, a.z, in);
+    tf += S::TS;
+    x += S::TS * a.xs;
+    dt += S::TS * a.ds;
+    z += S::TS * a.zs;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int i = tid + 128 * j, which = i / (M::BC / 2), at = i % (M::BC / 2) * 4;
-      if (i >= (FIRST ? M::BC / 2 : M::BC)) break;
-      const int n = at % S::NP, t_ = t0 + k * S::TS + at / S::NP;
-      const bool in = t_ < t1 && n < a.N;
-      const T* p = which ? static_cast<const T*>(a.C) + (in ? t_ * a.cs_t + g * a.cs_g + n : 0)
-                         : static_cast<const T*>(a.B) + (in ? t_ * a.bs_t + g * a.bs_g + n : 0);
-      if (vec_bc) copy_async<4 * (int)sizeof(T)>(sm.raw_bc[slot][i], p, in);
+      const int i = tid + kHelp * j;
+      if (i >= (FIRST ? M::BC / 2 : M::BC)) continue;
+      const bool in_ = tb[j] < t1 && has_bc[j];
+      if (vec_bc) copy_async<4 * (int)sizeof(T)>(sm.raw_bc[ring][i], in_ ? bc[j] : a.B, in_);
       else {
+        const int n = i % (M::BC / 2) * 4 % S::NP;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sm.raw_bc[slot][i][e] = in && n + e < a.N ? p[e] : from_f<T>(0.f);
+        for (int e = 0; e < 4; ++e) sm.raw_bc[ring][i][e] = in_ && n + e < a.N ? bc[j][e] : from_f<T>(0.f);
       }
+      tb[j] += S::TS;
+      bc[j] += S::TS * bc_stride[j];
     }
+    ring = (ring + 1) % kRing;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   AIR_DEVICE void arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
-  // Tokens past the end change nothing: their step is zero.
-  AIR_DEVICE void prepare(int k) {
+  // Stage k, `in`: this helper's token is one of the tile's. Tokens past the end change nothing: their step is zero.
+  AIR_DEVICE void prepare(int k, bool in) {
     const int slot = k % kRing;
-    const bool in = t0 + k * S::TS + tok < t1;
-    float x[E], dt[E];
-    load_v<T, E>(sm.rows[slot][0][tid], x);
-    load_v<T, E>(sm.rows[slot][1][tid], dt);
+    float xv[E], dv[E];
+    load_v<T, E>(sm.rows[slot][0][tid], xv);
+    load_v<T, E>(sm.rows[slot][1][tid], dv);
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      float v = dt[i] + bias[i], w = dt[i + 1] + bias[i + 1];
+    for (int i = 0; i < E && (S::HT * S::TS == kHelp || tok < S::TS); i += 2) {
+      float v = dv[i] + bias[i], w = dv[i + 1] + bias[i + 1];
       if (a.softplus) unpack2(softplus2(v, w), v, w);
       if (!in) v = w = 0.f;
-      sm.step[k & 1][tok][step_slot<E>((c + i) / 2)] = make_float4(v, w, v * x[i], w * x[i + 1]);
+      sm.step[k & 1][tok][step_slot<E>((c + i) / 2)] = make_float4(v, w, v * xv[i], w * xv[i + 1]);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int i = tid + 128 * j;
-      if (i >= (FIRST ? M::BC / 2 : M::BC)) break;
+      const int i = tid + kHelp * j;
+      if (i >= (FIRST ? M::BC / 2 : M::BC)) continue;
       float f[4];
       load_v<T, 4>(sm.raw_bc[slot][i], f);
-      float4* p = reinterpret_cast<float4*>(&sm.bc[k & 1][0][0][0] + i * 4);
-      p[0] = make_float4(f[0], f[0], f[1], f[1]);
-      p[1] = make_float4(f[2], f[2], f[3], f[3]);
+      const int which = i / (M::BC / 2), at = i % (M::BC / 2) * 4;
+      float2* p = reinterpret_cast<float2*>(&sm.bc[k & 1][at / S::NP][at % S::NP / 2]) + which;
+      p[0] = make_float2(f[0], f[1]);
+      p[2] = make_float2(f[2], f[3]);
     }
   }
+  // The outputs of stage k, for the tokens of the mask
   AIR_DEVICE void finish(int k, unsigned mask) {
+    T* o = out;
+    out += S::TS * a.os;
     if (live <= 0 || !(mask >> tok & 1)) return;
-    const int t = t0 + k * S::TS + tok, slot = k % kRing;
+    const int slot = k % kRing;
     float y[E], f[E];
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
@@ -276,7 +310,6 @@ struct Helper {
 #pragma unroll
       for (int i = 0; i < E; ++i) y[i] *= silu_f(f[i]);
     }
-    T* o = static_cast<T*>(a.out) + (int64_t)t * a.os + d;
     if (vec) store_v<T, E>(o, y);
     else {
 #pragma unroll
@@ -346,29 +379,46 @@ struct Scan {
       }
     }
   }
-  // K tokens from i on: first all their decays (K independent chains a state), then the chain through h. `sum`: of delta.
+  AIR_DEVICE ulonglong2 step(int buf, int i) const { return *reinterpret_cast<const ulonglong2*>(&sm.step[buf][i][slot]); }
+  // K tokens from i on, whose steps are in st: first all their decays (K independent chains a state), then the chains
+  // through h. What the chains read, and the next tokens' steps, are loaded before. `sum`: of delta.
   template <bool OUT, int K>
-  AIR_DEVICE void tokens(int buf, int i, f2& sum) {
+  AIR_DEVICE void tokens(int buf, int i, ulonglong2* st, int next, f2& sum) {
     f2 u[K * 2], p[K * 2], dx[K];
+    float4 c[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(&sm.step[buf][i + k][slot]);
-      dx[k] = st.y;
-      if (!OUT) sum = add2(sum, st.x);
-      u[k * 2] = mul2(st.x, A[0]);
-      u[k * 2 + 1] = mul2(st.x, A[1]);
+      u[k * 2] = mul2(st[k].x, A[0]);
+      u[k * 2 + 1] = mul2(st[k].x, A[1]);
+      dx[k] = st[k].y;
+      if (!OUT) sum = add2(sum, st[k].x);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) c[k] = sm.bc[buf][i + k][q];             // B, B', C, C'
+    if (next >= 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) st[k] = step(buf, next + k);
     }
     decays<K * 2>(u, p);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sm.bc[buf][0][i + k][q * 2]);
-      h[0] = fma2(p[k * 2], h[0], fma2(dx[k], B.x, h[0]));
-      h[1] = fma2(p[k * 2 + 1], h[1], fma2(dx[k], B.y, h[1]));
-      if (OUT) {
-        const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sm.bc[buf][1][i + k][q * 2]);
-        *reinterpret_cast<f2*>(&sm.y[buf][i + k][part]) = fma2(C.y, h[1], mul2(C.x, h[0]));
-      }
+      h[0] = fma2(p[k * 2], h[0], fma2(dx[k], dup2(c[k].x), h[0]));
+      h[1] = fma2(p[k * 2 + 1], h[1], fma2(dx[k], dup2(c[k].y), h[1]));
+      if (OUT) *reinterpret_cast<f2*>(&sm.y[buf][i + k][part]) = fma2(dup2(c[k].w), h[1], mul2(dup2(c[k].z), h[0]));
     }
+  }
+  template <bool OUT>
+  AIR_DEVICE void stage(int buf, f2& sum) {
+    ulonglong2 st[kGroup];
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) st[k] = step(buf, k);
+#pragma unroll
+    for (int i = 0; i < S::TS; i += kGroup) tokens<OUT, kGroup>(buf, i, st, i + kGroup < S::TS ? i + kGroup : -1, sum);
+  }
+  template <bool OUT>
+  AIR_DEVICE void token(int buf, int i, f2& sum) {
+    ulonglong2 st = step(buf, i);
+    tokens<OUT, 1>(buf, i, &st, -1, sum);
   }
 };
 
@@ -379,7 +429,7 @@ AIR_DEVICE bool starts_from(const SeqArgs& a, int n, int64_t& slot) {
 }
 
 template <typename T, int L, bool FIRST>
-__global__ void __launch_bounds__(kThreads, LB) scan_tiles_kernel(const __grid_constant__ ScanArgs a, const __grid_constant__ TileArgs ta, int vec) {
+__global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_constant__ ScanArgs a, const __grid_constant__ TileArgs ta, int vec) {
   using S = Shape<L>;
   extern __shared__ __align__(16) uint8_t raw_smem[];
   Smem<T, L>& sm = *reinterpret_cast<Smem<T, L>*>(raw_smem);
@@ -406,25 +456,25 @@ __global__ void __launch_bounds__(kThreads, LB) scan_tiles_kernel(const __grid_c
     Helper<T, L, FIRST> w(a, sm, d0, grp, left, vec, t0, t1);
     if (stages > 0) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) w.fetch(k);
+      for (int k = 0; k < kAhead; ++k) w.fetch();
       w.arrived();
-      w.prepare(0);
+      w.prepare(0, t0 + w.tok < t1);
     }
     stage_barrier();
     if (!FIRST && tile < ta.tiles && a.seq.S > 0) {
       // offsets and rows that are not sound are reported once, empty sequences without a state start one of zeros
-      for (int n = tile * 128 + w.tid; n < a.seq.N; n += ta.tiles * 128) {
+      for (int n = tile * kHelp + w.tid; n < a.seq.N; n += ta.tiles * kHelp) {
         const SeqRange s = seq_range(a.seq, n, blk == 0);
         if (a.seq.cu && s.slot >= 0 && s.t0 == s.t1 && !s.init)
           for (int64_t i = d0 * a.N; i < (d0 + min(left, S::CH)) * a.N; ++i) a.state[s.slot * row + i] = 0.f;
       }
     } else if (!FIRST && blk == 0) {
-      for (int n = tile * 128 + w.tid; n < a.seq.N; n += ta.tiles * 128) seq_range(a.seq, n);
+      for (int n = tile * kHelp + w.tid; n < a.seq.N; n += ta.tiles * kHelp) seq_range(a.seq, n);
     }
     for (int k = 0; k < stages; ++k) {
-      w.fetch(k + kAhead);
+      w.fetch();
       w.arrived();
-      if (k + 1 < stages) w.prepare(k + 1);
+      if (k + 1 < stages) w.prepare(k + 1, t0 + (k + 1) * S::TS + w.tok < t1);
       if (!FIRST && k > 0) {
         const int t = t0 + (k - 1) * S::TS;
         unsigned mask = ~0u;
@@ -491,8 +541,7 @@ __global__ void __launch_bounds__(kThreads, LB) scan_tiles_kernel(const __grid_c
     const int t = t0 + k * S::TS;
     f2 sum2 = 0ull;
     if (FIRST || t + S::TS <= seg.hi) {
-#pragma unroll
-      for (int i = 0; i < S::TS; i += kGroup) w.template tokens<!FIRST, kGroup>(k & 1, i, sum2);
+      w.template stage<!FIRST>(k & 1, sum2);
     } else {
       for (int i = 0; i < S::TS && t + i < t1; ++i) {
         while (t + i >= seg.hi) {
@@ -500,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, LB) scan_tiles_kernel(const __grid_c
           seg = segment_at(a.seq, t + i);
           enter(t + i);
         }
-        w.template tokens<!FIRST, 1>(k & 1, i, sum2);
+        w.template token<!FIRST>(k & 1, i, sum2);
       }
     }
     float sum[2];

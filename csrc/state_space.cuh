@@ -80,15 +80,14 @@ AIR_DEVICE float softplus_f(float x) {
 }
 
 // 2^u - 1 for the scan's decays, u = delta A log2(e). Added as h + (2^u - 1) h, a slow decay keeps its rate: 2^u itself,
-// rounded to 24 bits, would change a rate of 2^-10 by 2^-14 of itself at every token. For |u| <= log2(e) / 10 a cubic
-// (equal ripple of the relative error, computed for this interval: 1.0e-7, 2.2e-7 with the roundings), beyond it the
-// exponential less one, whose error is then at most 2.4e-6 of the rate.
-constexpr float kNearDecay = 0.144269504f, kDecay0 = 0.693147123f, kDecay1 = 0.240226552f, kDecay2 = 0.0555318594f,
-                kDecay3 = 0.00961812865f;
+// rounded to 24 bits, would change a rate of 2^-10 by 2^-14 of itself at every token. For |u| <= log2(e) / 32 a quadratic
+// times u (equal ripple of the relative error, computed for this interval: 3.2e-7, 4.2e-7 with the roundings), beyond it
+// the exponential less one, whose error is then at most 7.6e-6 of the rate.
+constexpr float kNearDecay = 0.0450842196f, kDecay0 = 0.693147182f, kDecay1 = 0.24024117f, kDecay2 = 0.0555041097f;
 AIR_DEVICE float decay_m1(float u) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
-  const float p = fmaf(fmaf(fmaf(kDecay3, u, kDecay2), u, kDecay1), u, kDecay0);
+  const float p = fmaf(fmaf(kDecay2, u, kDecay1), u, kDecay0);
   return fabsf(u) <= kNearDecay ? p * u : e - 1.f;
 }
 constexpr float kLog2e = 1.44269504f;
