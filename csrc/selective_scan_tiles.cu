@@ -31,34 +31,6 @@ namespace {
 #ifndef KG
 #define KG 4
 #endif
-using f2 = unsigned long long;       // two floats, the operand of the paired instructions
-AIR_DEVICE f2 pack2(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-AIR_DEVICE f2 dup2(float a) { return pack2(a, a); }
-AIR_DEVICE void unpack2(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-AIR_DEVICE f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-AIR_DEVICE f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-AIR_DEVICE f2 add2(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-AIR_DEVICE float exp2_fast(float u) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
-  return e;
-}
 // p = e - 1 where |u| is past the polynomial's interval
 AIR_DEVICE void far_decay(float& p, float u, float e) {
   asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %1;\n\tsetp.gt.f32 q, a, %2;\n\t@q add.f32 %0, %3, 0fBF800000;\n\t}"

@@ -16,6 +16,36 @@ AIR_DEVICE T from_f(float v) {
   else return v;
 }
 
+// ---- paired f32 arithmetic
+using f2 = unsigned long long;       // two floats, the operand of the paired instructions
+AIR_DEVICE f2 pack2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+AIR_DEVICE f2 dup2(float a) { return pack2(a, a); }
+AIR_DEVICE void unpack2(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+AIR_DEVICE f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+AIR_DEVICE f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+AIR_DEVICE f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+AIR_DEVICE float exp2_fast(float u) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
+  return e;
+}
+
 // V consecutive elements as f32: one 16- or 8-byte access, or single elements (V = 1).
 template <typename T, int V>
 AIR_DEVICE void load_v(const T* p, float* f) {
@@ -85,9 +115,7 @@ AIR_DEVICE float softplus_f(float x) {
 // the exponential less one, whose error is then at most 7.6e-6 of the rate.
 constexpr float kNearDecay = 0.0450842196f, kDecay0 = 0.693147182f, kDecay1 = 0.24024117f, kDecay2 = 0.0555041097f;
 AIR_DEVICE float decay_m1(float u) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
-  const float p = fmaf(fmaf(kDecay2, u, kDecay1), u, kDecay0);
+  const float e = exp2_fast(u), p = fmaf(fmaf(kDecay2, u, kDecay1), u, kDecay0);
   return fabsf(u) <= kNearDecay ? p * u : e - 1.f;
 }
 constexpr float kLog2e = 1.44269504f;

@@ -1,54 +1,185 @@
-// Log probabilities from logits, one pass a row:
+// Log probabilities from logits, one pass over a row:
 //   lse = log sum_v exp(x_v),  logprob = x_token - lse,  entropy = lse - sum_v p_v x_v,
-// and the k most likely tokens (ties: the lowest index first). Sums stay f32 around the row's maximum.
+// and the k most likely tokens (ties: the lowest index first).
+//
+// A block (or a cluster of blocks, with few rows) streams its row in 16-byte accesses. Each thread keeps s = sum exp(d) and
+// e = sum d exp(d) for d = x - ref and moves its reference only when a logit passes it by more than 16, so the exponential
+// and four paired operations are what two elements cost; sums are f32, joined around the row's maximum:
+// entropy = log s - e / s. Infinities below count as -1e30, whose exponential is an exact zero.
+//
+// The alternatives need no second pass over the row: the k-th largest of the threads' maxima is at most the k-th largest
+// logit, so only the k threads whose maximum reaches it can hold one. Their elements (k / threads of the row, from L2) are
+// read again by the whole block, the few that reach the bound are collected and ordered. Memory-bound.
+#include <cooperative_groups.h>
 #include "state_space.cuh"
 
 namespace air {
 
 namespace {
 
-constexpr int kLpThreads = 256;
+namespace cg = cooperative_groups;
 
+constexpr float kMasked = -1e30f;          // stands for -inf in the sums
+constexpr float kAllLow = -1e29f;          // a row whose maximum is below takes the plain path
+constexpr float kMargin = 16.f;
+
+using Key = unsigned long long;
 // Order of the alternatives as one number: the value's bits mapped to rising unsigned ones, then the index inverted.
-AIR_DEVICE unsigned long long rank_key(float v, int i) {
-  const uint32_t b = __float_as_uint(v);
-  return (unsigned long long)(b ^ (b >> 31 ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~i;
+// Zeros of both signs are alike.
+AIR_DEVICE uint32_t rank_bits(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
-AIR_DEVICE float key_value(unsigned long long k) {
+AIR_DEVICE Key rank_key(float v, int i) { return (Key)rank_bits(v) << 32 | (uint32_t)~i; }
+AIR_DEVICE float key_value(Key k) {
   const uint32_t b = (uint32_t)(k >> 32);
   return __uint_as_float(b ^ (b >> 31 ? 0x80000000u : 0xffffffffu));
 }
+AIR_DEVICE int key_index(Key k) { return (int)~(uint32_t)k; }
 
-AIR_DEVICE unsigned long long block_max_key(unsigned long long v, unsigned long long* red) {
+// 16 bytes of a row as f32, infinities below as kMasked, NaN kept.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int E = 8;
+  __nv_bfloat162 v[4];
+  AIR_DEVICE void load(const __nv_bfloat16* p) {
+    const uint4 u = ld_stream(p);
+    v[0] = *reinterpret_cast<const __nv_bfloat162*>(&u.x);
+    v[1] = *reinterpret_cast<const __nv_bfloat162*>(&u.y);
+    v[2] = *reinterpret_cast<const __nv_bfloat162*>(&u.z);
+    v[3] = *reinterpret_cast<const __nv_bfloat162*>(&u.w);
+  }
+  AIR_DEVICE void load_part(const __nv_bfloat16* p, int lo, int hi) {
+    __nv_bfloat16 t[8];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
+    for (int i = 0; i < 8; ++i) t[i] = i >= lo && i < hi ? p[i] : __float2bfloat16_rn(-INFINITY);
 #pragma unroll
-  for (int w = 1; w < kLpThreads / 32; ++w) v = max(v, red[w]);
-  return v;
+    for (int i = 0; i < 4; ++i) v[i] = __nv_bfloat162(t[2 * i], t[2 * i + 1]);
+  }
+  AIR_DEVICE void clamp() {
+    const __nv_bfloat162 m = __float2bfloat162_rn(kMasked);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __hmax2_nan(v[i], m);
+  }
+  AIR_DEVICE float max() const {
+    const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  AIR_DEVICE void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(&v[i]);
+      f[2 * i] = __uint_as_float(u << 16);
+      f[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
+    }
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int E = 4;
+  float v[4];
+  AIR_DEVICE void load(const float* p) {
+    const uint4 u = ld_stream(p);
+    v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
+  }
+  AIR_DEVICE void load_part(const float* p, int lo, int hi) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i >= lo && i < hi ? p[i] : -INFINITY;
+  }
+  AIR_DEVICE void clamp() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(v[i]) : "f"(kMasked));
+  }
+  AIR_DEVICE float max() const { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
+  AIR_DEVICE void get(float (&f)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = v[i];
+  }
+};
+
+// A row as aligned vectors: vector i holds elements i E - off .. of the row.
+template <typename T>
+struct Row {
+  static constexpr int E = Vec<T>::E;
+  const T* base;                           // 16-byte aligned, at or before the first element
+  int off, V, vectors;
+  AIR_DEVICE Row(const T* x, int n) : V(n) {
+    off = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+    base = x - off;
+    vectors = (int)(((int64_t)n + off + E - 1) / E);
+  }
+  AIR_DEVICE Vec<T> operator()(int i) const {
+    Vec<T> r;
+    const int64_t first = (int64_t)i * E - off;
+    if (first >= 0 && first + E <= V) r.load(base + (int64_t)i * E);
+    else r.load_part(base + (int64_t)i * E, first < 0 ? off : 0, (int)min((int64_t)E, V - first));
+    return r;
+  }
+};
+
+struct Sums {
+  float ref, s, e;                         // s = sum exp(d), e = sum d exp(d) for d = x - ref
+  AIR_DEVICE void move(float to) {         // to >= ref
+    const float d = ref - to, f = ref == -INFINITY ? 0.f : exp2f(d * kLog2e);
+    e = ref == -INFINITY ? 0.f : f * fmaf(d, s, e);
+    s *= f;
+    ref = to;
+  }
+};
+
+template <typename T, int NT>
+struct LpSmem {
+  static constexpr int Keep = 1024, Cap = Keep + NT * Vec<T>::E;   // a round adds at most a vector a thread
+  Key keys[Cap], best[kLogprobMaxTop];
+  float maxima[NT];
+  short chosen[NT];
+  float red[3][32];
+  Sums total;
+  float bound;
+  int count, n_chosen;
+};
+
+// keys[0 .. n) -> the k largest in order in best (0 where there are fewer)
+template <int NT>
+AIR_DEVICE void largest(const Key* keys, int n, int k, Key* best) {
+  if (threadIdx.x < k) best[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const Key mine = keys[i];
+    int above = 0;
+    for (int j = 0; j < n && above < k; ++j) above += keys[j] > mine;
+    if (above < k) best[above] = mine;
+  }
+  __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const TokenLogprobArgs a) {
-  __shared__ float red[32];
-  __shared__ unsigned long long redk[kLpThreads / 32];
-  const int64_t t = blockIdx.x;
-  const T* x = static_cast<const T*>(a.logits) + t * a.ld;
-  float m = -INFINITY;
-  bool nan = false;
-  for (int i = threadIdx.x; i < a.V; i += kLpThreads) {
-    const float v = to_f(x[i]);
-    nan |= v != v || v == INFINITY;
-    m = fmaxf(m, v);
+// The k-th largest of NT values, by the first warp: the largest bound that at least k of them reach, bit by bit.
+template <int NT>
+AIR_DEVICE float kth_largest(const float* v, int k) {
+  uint32_t mine[NT / 32], bound = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) mine[i] = rank_bits(v[threadIdx.x + 32 * i]);
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t t = bound | 1u << b;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) n += mine[i] >= t;
+    if (__reduce_add_sync(0xffffffffu, n) >= k) bound = t;
   }
+  return __uint_as_float(bound ^ (bound >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// The sums of a row by one block, element by element around its true maximum, for rows that the stand-in for -inf would
+// change: all logits below -1e29.
+template <typename T, int NT>
+__device__ Sums low_row(const T* x, int V, float* red) {
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < V; i += NT) m = fmaxf(m, to_f(x[i]));
   m = block_max(m, red);
-  nan = __syncthreads_or(nan);
-  const bool none = m == -INFINITY;
   float s = 0.f, e = 0.f;
-  for (int i = threadIdx.x; i < a.V; i += kLpThreads) {
+  for (int i = threadIdx.x; i < V && m > -INFINITY; i += NT) {
     const float u = to_f(x[i]) - m, p = expf(u);
     s += p;
     if (p > 0.f) e = fmaf(p, u, e);
@@ -56,36 +187,199 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const TokenL
   s = block_sum(s, red);
   __syncthreads();
   e = block_sum(e, red);
-  const float ls = logf(s);
-  auto logprob = [&](float v) { return nan ? NAN : v == -INFINITY ? -INFINITY : v - m - ls; };
+  return {m, s, e};
+}
+
+// Collects the elements of the vectors at(0 .. items) that `take` wants into sm.keys; never more than the k largest and a
+// round's worth at a time. By the whole block.
+template <typename T, int NT, class At, class Take>
+AIR_DEVICE void collect(LpSmem<T, NT>& sm, const Row<T>& row, int k, int items, At at, Take take) {
+  constexpr int E = Vec<T>::E;
+  Key above = 0;
+  for (int w0 = 0; w0 < items; w0 += NT) {
+    const int i = w0 + (int)threadIdx.x < items ? at(w0 + threadIdx.x) : -1;
+    if (i >= 0) {
+      float f[E];
+      row(i).get(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const Key key = rank_key(f[j], i * E - row.off + j);
+        if (take(f[j]) && key > above) sm.keys[atomicAdd(&sm.count, 1)] = key;
+      }
+    }
+    __syncthreads();
+    const int n = sm.count;
+    if (n > LpSmem<T, NT>::Keep) {                   // keep the k largest, and look for larger ones only
+      largest<NT>(sm.keys, n, k, sm.best);
+      above = sm.best[k - 1];
+      if (threadIdx.x < k) sm.keys[threadIdx.x] = sm.best[threadIdx.x];
+      if (threadIdx.x == 0) sm.count = k;
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int NT, int CS>
+__global__ void __launch_bounds__(NT) token_logprobs_kernel(const TokenLogprobArgs a) {
+  using V = Vec<T>;
+  constexpr int E = V::E, U = 4;                     // vectors in flight
+  extern __shared__ __align__(16) uint8_t raw_smem[];
+  LpSmem<T, NT>& sm = *reinterpret_cast<LpSmem<T, NT>*>(raw_smem);
+  const int rank = CS > 1 ? (int)cg::this_cluster().block_rank() : 0;
+  const int64_t t = blockIdx.x / CS;
+  const Row<T> row(static_cast<const T*>(a.logits) + t * a.ld, a.V);
+  const int per = (row.vectors + CS - 1) / CS;
+  const int v0 = min(row.vectors, rank * per), v1 = min(row.vectors, v0 + per);
+
+  float ref = -INFINITY, top = -INFINITY;
+  f2 s2 = 0ull, e2 = 0ull, back = 0ull;              // the sums in two halves; -ref twice
+  auto join = [&]() {
+    float s0, s1, e0, e1;
+    unpack2(s2, s0, s1);
+    unpack2(e2, e0, e1);
+    return Sums{ref, s0 + s1, e0 + e1};
+  };
+  auto add = [&](V& v) {
+    v.clamp();
+    const float m = v.max();
+    top = fmaxf(top, m);
+    if (m > ref + kMargin || ref == -INFINITY) {
+      Sums r = join();
+      r.move(m);
+      ref = m;
+      s2 = pack2(r.s, 0.f);
+      e2 = pack2(r.e, 0.f);
+      back = dup2(-m);
+    }
+    float f[E];
+    v.get(f);
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      const f2 d = add2(pack2(f[i], f[i + 1]), back);
+      float u0, u1;
+      unpack2(mul2(d, dup2(kLog2e)), u0, u1);
+      const f2 p = pack2(exp2_fast(u0), exp2_fast(u1));
+      s2 = add2(s2, p);
+      e2 = fma2(d, p, e2);
+    }
+  };
+  int i = v0 + threadIdx.x;
+  for (; i + (U - 1) * NT < v1; i += U * NT) {
+    V v[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) v[j] = row(i + j * NT);
+#pragma unroll
+    for (int j = 0; j < U; ++j) add(v[j]);
+  }
+  for (; i < v1; i += NT) {
+    V v = row(i);
+    add(v);
+  }
+
+  // ---- the block's maximum and sums
+  Sums r = join();
+  const float big = block_max(top, sm.red[0]);
+  if (big > r.ref) r.move(big);                      // (no element: s = e = 0)
+  const float s = block_sum(r.s, sm.red[1]), e = block_sum(r.e, sm.red[2]);
+  if (threadIdx.x == 0) sm.total = {big, s, e};
+
+  // ---- the block's k largest
+  if (a.k) {
+    sm.maxima[threadIdx.x] = top;
+    if (threadIdx.x == 0) sm.n_chosen = sm.count = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const float b = kth_largest<NT>(sm.maxima, a.k);
+      if (threadIdx.x == 0) sm.bound = fmaxf(b, kAllLow);
+    }
+    __syncthreads();
+    const float bound = sm.bound;
+    if (top >= bound) sm.chosen[atomicAdd(&sm.n_chosen, 1)] = (short)threadIdx.x;
+    __syncthreads();
+    const int each = (v1 - v0 + NT - 1) / NT;
+    collect<T, NT>(sm, row, a.k, sm.n_chosen * each,
+                   [&](int w) { const int at = v0 + sm.chosen[w / each] + w % each * NT; return at < v1 ? at : -1; },
+                   [&](float f) { return f >= bound; });
+    const int found = sm.count;
+    __syncthreads();
+    if (found < a.k)                                 // fewer than k: what is finite and lower still, if there is any
+      collect<T, NT>(sm, row, a.k, v1 - v0, [&](int w) { return v0 + w; }, [&](float f) { return f < bound && f > -INFINITY; });
+    largest<NT>(sm.keys, sm.count, a.k, sm.best);
+  }
+
+  // ---- the cluster's
+  Sums all = {big, s, e};
+  if constexpr (CS > 1) {
+    auto cluster = cg::this_cluster();
+    cluster.sync();
+    if (rank == 0) {
+      for (int c = 1; c < CS; ++c) {
+        Sums o = cluster.map_shared_rank(&sm, c)->total;
+        const float m = fmaxf(all.ref, o.ref);
+        if (m > all.ref) all.move(m);
+        if (m > o.ref) o.move(m);
+        all.s += o.s;
+        all.e += o.e;
+      }
+      if (a.k) {
+        __syncthreads();
+        for (int w = threadIdx.x; w < CS * a.k; w += NT) sm.keys[w] = cluster.map_shared_rank(&sm, w / a.k)->best[w % a.k];
+        __syncthreads();
+        largest<NT>(sm.keys, CS * a.k, a.k, sm.best);
+      }
+    }
+    cluster.sync();                                  // the others' memory was read until here
+    if (rank != 0) return;
+  }
+  const bool nan = !(all.s < INFINITY);
+  const int tok = a.tokens ? a.tokens[t] : -1;
+  if (threadIdx.x == 0 && (tok < -1 || tok >= a.V)) set_error(a.err, kErrBounds);
+  if (!nan && all.ref <= kAllLow) all = low_row<T, NT>(row.base + row.off, a.V, sm.red[0]);
+  const bool none = all.ref == -INFINITY;            // nothing is allowed
+  const float ls = logf(all.s);
+  auto logprob = [&](float v) { return nan ? NAN : v == -INFINITY ? -INFINITY : v - all.ref - ls; };
   if (threadIdx.x == 0) {
-    const int tok = a.tokens ? a.tokens[t] : -1;
-    if (tok < -1 || tok >= a.V) set_error(a.err, kErrBounds);
-    a.logprob[t] = tok < 0 || tok >= a.V ? 0.f : logprob(to_f(x[tok]));
-    a.entropy[t] = nan ? NAN : none ? 0.f : ls - e / s;
+    a.logprob[t] = tok < 0 || tok >= a.V ? 0.f : logprob(to_f(row.base[row.off + (int64_t)tok]));
+    a.entropy[t] = nan ? NAN : none ? 0.f : ls - all.e / all.s;
   }
-  unsigned long long below = ~0ull;
-  for (int r = 0; r < a.k; ++r) {
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < a.V && !nan; i += kLpThreads) {
-      const float v = to_f(x[i]);
-      const unsigned long long key = v == -INFINITY ? 0 : rank_key(v == 0.f ? 0.f : v, i);
-      if (key < below) best = max(best, key);
-    }
-    below = best = block_max_key(best, redk);
-    if (threadIdx.x == 0) {
-      a.top_id[t * a.k + r] = best ? (int)~(uint32_t)best : -1;
-      a.top_lp[t * a.k + r] = nan ? NAN : best ? logprob(key_value(best)) : -INFINITY;
-    }
+  if (threadIdx.x < a.k) {
+    const Key b = nan ? 0 : sm.best[threadIdx.x];
+    a.top_id[t * a.k + threadIdx.x] = b ? key_index(b) : -1;
+    a.top_lp[t * a.k + threadIdx.x] = nan ? NAN : b ? logprob(key_value(b)) : -INFINITY;
   }
+}
+
+template <typename T, int NT, int CS>
+void launch(const TokenLogprobArgs& a, cudaStream_t st) {
+  static unsigned long long done = 0;
+  constexpr int bytes = sizeof(LpSmem<T, NT>);
+  set_max_smem_per_device(token_logprobs_kernel<T, NT, CS>, bytes, done);
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)a.T * CS);
+  c.blockDim = dim3(NT);
+  c.dynamicSmemBytes = bytes;
+  c.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim = {CS, 1, 1};
+  c.attrs = &at;
+  c.numAttrs = CS > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&c, token_logprobs_kernel<T, NT, CS>, a);
+}
+
+template <typename T>
+void choose(const TokenLogprobArgs& a, cudaStream_t st) {
+  if ((int64_t)a.T * 8 <= 148 * 4 && a.V >= 16384) launch<T, 512, 8>(a, st);
+  else if ((int64_t)a.T * 2 <= 148 * 4 && a.V >= 16384) launch<T, 256, 2>(a, st);
+  else launch<T, 256, 1>(a, st);
 }
 
 }  // namespace
 
 void launch_token_logprobs(const TokenLogprobArgs& a, bool f32, cudaStream_t st) {
   if (a.T == 0) return;
-  if (f32) token_logprobs_kernel<float><<<a.T, kLpThreads, 0, st>>>(a);
-  else token_logprobs_kernel<__nv_bfloat16><<<a.T, kLpThreads, 0, st>>>(a);
+  if (f32) choose<float>(a, st);
+  else choose<__nv_bfloat16>(a, st);
 }
 
 }  // namespace air
