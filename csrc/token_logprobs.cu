@@ -11,6 +11,7 @@
 // logit, so only the k threads whose maximum reaches it can hold one. Their elements (k / threads of the row, from L2) are
 // read again by the whole block, the few that reach the bound are collected and ordered. Memory-bound.
 #include <cooperative_groups.h>
+
 #include "state_space.cuh"
 
 namespace air {
@@ -131,17 +132,17 @@ struct Sums {
 
 template <typename T, int NT>
 struct LpSmem {
-  static constexpr int Keep = 1024, Cap = Keep + NT * Vec<T>::E;   // a round adds at most a vector a thread
+  static constexpr int Keep = 256, Cap = Keep + NT * Vec<T>::E;    // a round of collect_rounds adds at most a vector a thread
   Key keys[Cap], best[kLogprobMaxTop];
   float maxima[NT];
   short chosen[NT];
-  float red[3][32];
-  Sums total;
+  Sums warp[NT / 32], total, joined;
+  float red[32];
   float bound;
   int count, n_chosen;
 };
 
-// keys[0 .. n) -> the k largest in order in best (0 where there are fewer)
+// keys[0 .. n) -> the k largest in order in best (0 where there are fewer): each key's place is the number of larger ones
 template <int NT>
 AIR_DEVICE void largest(const Key* keys, int n, int k, Key* best) {
   if (threadIdx.x < k) best[threadIdx.x] = 0;
@@ -149,19 +150,20 @@ AIR_DEVICE void largest(const Key* keys, int n, int k, Key* best) {
   for (int i = threadIdx.x; i < n; i += NT) {
     const Key mine = keys[i];
     int above = 0;
-    for (int j = 0; j < n && above < k; ++j) above += keys[j] > mine;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) above += keys[j] > mine;
     if (above < k) best[above] = mine;
   }
   __syncthreads();
 }
 
-// The k-th largest of NT values, by the first warp: the largest bound that at least k of them reach, bit by bit.
+// A bound that at least k of NT values reach and hardly more: the k-th largest, rounded down to 16 bits. By one warp.
 template <int NT>
 AIR_DEVICE float kth_largest(const float* v, int k) {
   uint32_t mine[NT / 32], bound = 0;
 #pragma unroll
-  for (int i = 0; i < NT / 32; ++i) mine[i] = rank_bits(v[threadIdx.x + 32 * i]);
-  for (int b = 31; b >= 0; --b) {
+  for (int i = 0; i < NT / 32; ++i) mine[i] = rank_bits(v[(threadIdx.x & 31) + 32 * i]);
+  for (int b = 31; b >= 16; --b) {
     const uint32_t t = bound | 1u << b;
     int n = 0;
 #pragma unroll
@@ -169,6 +171,13 @@ AIR_DEVICE float kth_largest(const float* v, int k) {
     if (__reduce_add_sync(0xffffffffu, n) >= k) bound = t;
   }
   return __uint_as_float(bound ^ (bound >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// The sums of up to 32 lanes, in all lanes.
+AIR_DEVICE Sums warp_join(Sums r) {
+  const float m = warp_max(r.ref);
+  if (m > r.ref) r.move(m);
+  return {m, warp_sum(r.s), warp_sum(r.e)};
 }
 
 // The sums of a row by one block, element by element around its true maximum, for rows that the stand-in for -inf would
@@ -190,10 +199,10 @@ __device__ Sums low_row(const T* x, int V, float* red) {
   return {m, s, e};
 }
 
-// Collects the elements of the vectors at(0 .. items) that `take` wants into sm.keys; never more than the k largest and a
-// round's worth at a time. By the whole block.
+// Collects the elements of the vectors at(0 .. items) that `take` wants into sm.keys, which may hold some already; never
+// more than the k largest and a round's worth at a time. By the whole block.
 template <typename T, int NT, class At, class Take>
-AIR_DEVICE void collect(LpSmem<T, NT>& sm, const Row<T>& row, int k, int items, At at, Take take) {
+__device__ __noinline__ void collect_rounds(LpSmem<T, NT>& sm, const Row<T>& row, int k, int items, At at, Take take) {
   constexpr int E = Vec<T>::E;
   Key above = 0;
   for (int w0 = 0; w0 < items; w0 += NT) {
@@ -216,6 +225,46 @@ AIR_DEVICE void collect(LpSmem<T, NT>& sm, const Row<T>& row, int k, int items, 
       if (threadIdx.x == 0) sm.count = k;
     }
     __syncthreads();
+  }
+}
+// The same in one go, several vectors in flight and no barriers, and in rounds only if there are too many to hold.
+template <typename T, int NT, class At, class Take>
+AIR_DEVICE void collect(LpSmem<T, NT>& sm, const Row<T>& row, int k, int items, At at, Take take) {
+  constexpr int E = Vec<T>::E, U = 4;
+  const int before = sm.count;
+  __syncthreads();
+  for (int w0 = threadIdx.x; w0 < items; w0 += NT * U) {
+    Vec<T> v[U];
+    int i[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      i[u] = w0 + u * NT < items ? at(w0 + u * NT) : -1;
+      if (i[u] >= 0) v[u] = row(i[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i[u] < 0) continue;
+      float f[E];
+      v[u].get(f);
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < E; ++j) any |= take(f[j]);
+      if (!any) continue;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        if (!take(f[j])) continue;
+        const int n = atomicAdd(&sm.count, 1);
+        if (n < LpSmem<T, NT>::Cap) sm.keys[n] = rank_key(f[j], i[u] * E - row.off + j);
+      }
+    }
+  }
+  __syncthreads();
+  const int n = sm.count;
+  __syncthreads();
+  if (n > LpSmem<T, NT>::Cap) {
+    if (threadIdx.x == 0) sm.count = before;
+    __syncthreads();
+    collect_rounds<T, NT>(sm, row, k, items, at, take);
   }
 }
 
@@ -263,78 +312,90 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const TokenLogprobAr
       e2 = fma2(d, p, e2);
     }
   };
-  int i = v0 + threadIdx.x;
-  for (; i + (U - 1) * NT < v1; i += U * NT) {
+  // whole vectors, several in flight, then the two at the row's ends, which may hold fewer elements
+  const int w0 = v0 + (v0 == 0), w1 = v1 - (v1 == row.vectors && v1 > w0);
+  const T* p = row.base + (int64_t)(w0 + threadIdx.x) * E;
+  int i = w0 + threadIdx.x;
+  for (; i + (U - 1) * NT < w1; i += U * NT, p += U * NT * E) {
     V v[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) v[j] = row(i + j * NT);
+    for (int j = 0; j < U; ++j) v[j].load(p + j * NT * E);
 #pragma unroll
     for (int j = 0; j < U; ++j) add(v[j]);
   }
-  for (; i < v1; i += NT) {
-    V v = row(i);
+  for (; i < w1; i += NT, p += NT * E) {
+    V v;
+    v.load(p);
+    add(v);
+  }
+  if (threadIdx.x == 0 && w0 > v0 && v1 > v0) {
+    V v = row(v0);
+    add(v);
+  }
+  if (threadIdx.x == NT - 1 && w1 < v1) {
+    V v = row(w1);
     add(v);
   }
 
-  // ---- the block's maximum and sums
-  Sums r = join();
-  const float big = block_max(top, sm.red[0]);
-  if (big > r.ref) r.move(big);                      // (no element: s = e = 0)
-  const float s = block_sum(r.s, sm.red[1]), e = block_sum(r.e, sm.red[2]);
-  if (threadIdx.x == 0) sm.total = {big, s, e};
+  // ---- the block's maximum and sums, and a bound of its k largest
+  {
+    const Sums w = warp_join(join());
+    if ((threadIdx.x & 31) == 0) sm.warp[threadIdx.x >> 5] = w;
+    sm.maxima[threadIdx.x] = top;
+    if (threadIdx.x == 0) sm.n_chosen = sm.count = 0;
+  }
+  __syncthreads();
+  if (a.k && threadIdx.x < 32) {
+    const float b = kth_largest<NT>(sm.maxima, a.k);
+    if (threadIdx.x == 0) sm.bound = fmaxf(b, kAllLow);
+  } else if (threadIdx.x >= NT - 32) {
+    const int lane = threadIdx.x & 31;
+    const Sums w = warp_join(lane < NT / 32 ? sm.warp[lane] : Sums{-INFINITY, 0.f, 0.f});
+    if (lane == 0) sm.total = w;
+  }
+  __syncthreads();
 
   // ---- the block's k largest
   if (a.k) {
-    sm.maxima[threadIdx.x] = top;
-    if (threadIdx.x == 0) sm.n_chosen = sm.count = 0;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      const float b = kth_largest<NT>(sm.maxima, a.k);
-      if (threadIdx.x == 0) sm.bound = fmaxf(b, kAllLow);
-    }
-    __syncthreads();
     const float bound = sm.bound;
     if (top >= bound) sm.chosen[atomicAdd(&sm.n_chosen, 1)] = (short)threadIdx.x;
     __syncthreads();
-    const int each = (v1 - v0 + NT - 1) / NT;
+    const int each = (w1 - w0 + NT - 1) / NT + 1;    // a thread's vectors; the last place is for one of the row's ends
     collect<T, NT>(sm, row, a.k, sm.n_chosen * each,
-                   [&](int w) { const int at = v0 + sm.chosen[w / each] + w % each * NT; return at < v1 ? at : -1; },
-                   [&](float f) { return f >= bound; });
-    const int found = sm.count;
-    __syncthreads();
-    if (found < a.k)                                 // fewer than k: what is finite and lower still, if there is any
-      collect<T, NT>(sm, row, a.k, v1 - v0, [&](int w) { return v0 + w; }, [&](float f) { return f < bound && f > -INFINITY; });
+                   [=, &sm](int w) {
+                     const int who = sm.chosen[w / each], j = w % each, at = w0 + who + j * NT;
+                     if (j < each - 1) return at < w1 ? at : -1;
+                     return who == 0 && w0 > v0 && v1 > v0 ? v0 : who == NT - 1 && w1 < v1 ? w1 : -1;
+                   },
+                   [=](float f) { return f >= bound; });
+    if (sm.count < a.k)                              // fewer than k: what is finite and lower still, if there is any
+      collect<T, NT>(sm, row, a.k, v1 - v0, [=](int w) { return v0 + w; }, [=](float f) { return f < bound && f > -INFINITY; });
     largest<NT>(sm.keys, sm.count, a.k, sm.best);
   }
 
   // ---- the cluster's
-  Sums all = {big, s, e};
+  Sums all = sm.total;
   if constexpr (CS > 1) {
     auto cluster = cg::this_cluster();
     cluster.sync();
     if (rank == 0) {
-      for (int c = 1; c < CS; ++c) {
-        Sums o = cluster.map_shared_rank(&sm, c)->total;
-        const float m = fmaxf(all.ref, o.ref);
-        if (m > all.ref) all.move(m);
-        if (m > o.ref) o.move(m);
-        all.s += o.s;
-        all.e += o.e;
+      if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        const Sums w = warp_join(lane < CS ? cluster.map_shared_rank(&sm, lane % CS)->total : Sums{-INFINITY, 0.f, 0.f});
+        if (lane == 0) sm.joined = w;
       }
-      if (a.k) {
-        __syncthreads();
-        for (int w = threadIdx.x; w < CS * a.k; w += NT) sm.keys[w] = cluster.map_shared_rank(&sm, w / a.k)->best[w % a.k];
-        __syncthreads();
-        largest<NT>(sm.keys, CS * a.k, a.k, sm.best);
-      }
+      for (int w = threadIdx.x; w < CS * a.k; w += NT) sm.keys[w] = cluster.map_shared_rank(&sm, w / a.k)->best[w % a.k];
+      __syncthreads();
+      all = sm.joined;
     }
     cluster.sync();                                  // the others' memory was read until here
     if (rank != 0) return;
+    if (a.k) largest<NT>(sm.keys, CS * a.k, a.k, sm.best);
   }
   const bool nan = !(all.s < INFINITY);
   const int tok = a.tokens ? a.tokens[t] : -1;
   if (threadIdx.x == 0 && (tok < -1 || tok >= a.V)) set_error(a.err, kErrBounds);
-  if (!nan && all.ref <= kAllLow) all = low_row<T, NT>(row.base + row.off, a.V, sm.red[0]);
+  if (!nan && all.ref <= kAllLow) all = low_row<T, NT>(row.base + row.off, a.V, sm.red);
   const bool none = all.ref == -INFINITY;            // nothing is allowed
   const float ls = logf(all.s);
   auto logprob = [&](float v) { return nan ? NAN : v == -INFINITY ? -INFINITY : v - all.ref - ls; };
@@ -369,8 +430,18 @@ void launch(const TokenLogprobArgs& a, cudaStream_t st) {
 
 template <typename T>
 void choose(const TokenLogprobArgs& a, cudaStream_t st) {
-  if ((int64_t)a.T * 8 <= 148 * 4 && a.V >= 16384) launch<T, 512, 8>(a, st);
-  else if ((int64_t)a.T * 2 <= 148 * 4 && a.V >= 16384) launch<T, 256, 2>(a, st);
+  // Blocks of 256 threads fill the device at five an SM. Rows that leave room are cut among clusters of up to 8 blocks (1 row
+  // of 128256: 9.8 us against 16.4 by one block; 100 rows: 19 against 38), or taken by larger blocks (400 rows: 46
+  // against 53). Many short rows leave most threads of a block idle in the selection: 20000 x 5000 takes 101 us
+  // with 64 threads, 128 with 128 and 233 with 256, 4000 x 16000 takes 64, 56 and 70; 300 x 10000 20, 13 and 10.
+  const int64_t room = 148 * 5, vectors = a.V / Vec<T>::E;
+  if (vectors <= 1024 && a.T > 1024) launch<T, 64, 1>(a, st);
+  else if (vectors <= 2048 && a.T > 1024) launch<T, 128, 1>(a, st);
+  else if (vectors <= 2048) launch<T, 256, 1>(a, st);
+  else if (a.T * 8 <= room) launch<T, 256, 8>(a, st);
+  else if (a.T * 4 <= room) launch<T, 256, 4>(a, st);
+  else if (a.T * 2 <= room) launch<T, 256, 2>(a, st);
+  else if (a.T <= 148 * 3) launch<T, 512, 1>(a, st);
   else launch<T, 256, 1>(a, st);
 }
 
