@@ -3,11 +3,11 @@
 // where the W - 1 inputs before a sequence's first token are those of its state row (or zeros); the row then gets the
 // sequence's last W - 1 inputs. Sums stay f32 and are rounded once; the state holds inputs, unrounded.
 //
-// One launch has two kinds of blocks. Token runs: R consecutive packed tokens of a block of channels slide a window
+// A prompt launch has two kinds of blocks. Token runs: R consecutive packed tokens of a block of channels slide a window
 // over x; they write the tokens that have their W - 1 predecessors in their own sequence, so they need no state.
 // Sequences: the first W - 1 tokens and the state row, read and replaced by the same threads, so no block reads a row
 // that another writes. x is read once but for W - 1 rows a run. Memory-bound: two element sizes of traffic for
-// 2 W + 5 operations and two special functions.
+// 2 W + 5 operations and two special functions; the arithmetic runs on pairs of channels (f32x2).
 #include "state_space.cuh"
 
 namespace air {
@@ -16,55 +16,81 @@ namespace {
 
 constexpr int kConvThreads = 128;
 constexpr int kConvRun = 32;       // tokens a run, a bit each of a warp's vote
+constexpr int kGroups = 4;         // groups of rows in the ring
+
+// V channels of a row as they lie in memory, and as pairs of f32 (one channel: a pair whose second half is unused).
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Raw {
+  T v[V];
+};
+template <int V>
+struct Chan {
+  static constexpr int P = (V + 1) / 2;
+  f2 p[P];
+  AIR_DEVICE void zero() {
+#pragma unroll
+    for (int i = 0; i < P; ++i) p[i] = 0ull;
+  }
+  template <typename T>
+  AIR_DEVICE void from(const Raw<T, V>& r) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) p[i] = pack2(to_f(r.v[2 * i]), V > 1 ? to_f(r.v[V > 1 ? 2 * i + 1 : 0]) : 0.f);
+  }
+};
+template <typename T, int V>
+AIR_DEVICE Raw<T, V> no_row() {
+  Raw<T, V> r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.v[v] = from_f<T>(0.f);
+  return r;
+}
 
 template <typename T, int W, int V>
 struct Taps {
-  float w[W][V], b[V];
+  Chan<V> w[W], b;
   AIR_DEVICE Taps(const ConvArgs& a, int d) {
-    float flat[V * W];
-    if constexpr (V == 1) {
+    float flat[V * W], bias[V];
+    if constexpr (V * W % 4 == 0) load_v<float, V * W>(a.w + (int64_t)d * W, flat);
+    else {
 #pragma unroll
-      for (int i = 0; i < W; ++i) flat[i] = a.w[(int64_t)d * W + i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V * W; i += 4) load_v<float, 4>(a.w + (int64_t)d * W + i, flat + i);
+      for (int i = 0; i < V * W; ++i) flat[i] = a.w[(int64_t)d * W + i];
     }
 #pragma unroll
-    for (int j = 0; j < W; ++j)
+    for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[d + v] : 0.f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) w[j][v] = flat[v * W + j];
-    if (a.bias) {
-      if constexpr (V == 1) b[0] = a.bias[d];
-      else {
+    for (int i = 0; i < Chan<V>::P; ++i) {
+      const int c0 = 2 * i, c1 = V > 1 ? 2 * i + 1 : 0;
 #pragma unroll
-        for (int i = 0; i < V; i += 4) load_v<float, 4>(a.bias + d + i, b + i);
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) b[v] = 0.f;
+      for (int j = 0; j < W; ++j) w[j].p[i] = pack2(flat[c0 * W + j], flat[c1 * W + j]);
+      b.p[i] = pack2(bias[c0], bias[c1]);
     }
   }
-  // rows[0 .. W - 1]: the token's window, oldest first
-  template <class Row>
-  AIR_DEVICE void apply(Row rows, int silu, T* out) const {
-    float y[V];
+  // win(0 .. W - 1): the token's window, oldest first
+  template <class Win>
+  AIR_DEVICE void apply(Win win, int silu, T* out) const {
+    Raw<T, V> r;
 #pragma unroll
-    for (int v = 0; v < V; ++v) y[v] = b[v];
+    for (int i = 0; i < Chan<V>::P; ++i) {
+      f2 y = b.p[i];
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-#pragma unroll
-      for (int v = 0; v < V; ++v) y[v] = fmaf(w[j][v], rows(j)[v], y[v]);
-    if (silu) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) y[v] = silu_f(y[v]);
+      for (int j = 0; j < W; ++j) y = fma2(w[j].p[i], win(j).p[i], y);
+      float y0, y1;
+      unpack2(y, y0, y1);
+      if (silu) {
+        y0 = silu_f(y0);
+        if (V > 1) y1 = silu_f(y1);
+      }
+      r.v[2 * i] = from_f<T>(y0);
+      if (V > 1) r.v[V > 1 ? 2 * i + 1 : 0] = from_f<T>(y1);
     }
-    store_v<T, V>(out, y);
+    *reinterpret_cast<Raw<T, V>*>(out) = r;
   }
 };
 
 // The first W - 1 tokens of sequence n and its state row, V channels a thread.
 template <typename T, int W, int V>
 AIR_DEVICE void conv_sequence(const ConvArgs& a, int n, int d) {
+  using R = Raw<T, V>;
   constexpr int H = W - 1;
   const SeqRange s = seq_range(a.seq, n);
   if (d >= a.D) return;
@@ -72,83 +98,101 @@ AIR_DEVICE void conv_sequence(const ConvArgs& a, int n, int d) {
   T* out = static_cast<T*>(a.out) + d;
   T* row = s.slot >= 0 ? static_cast<T*>(a.state) + s.slot * H * (int64_t)a.D + d : nullptr;
   if (a.seq.step && !row) {
-    float zero[V] = {};
-    for (int t = s.t0; t < s.t1; ++t) store_v<T, V>(out + t * a.os, zero);
+    for (int t = s.t0; t < s.t1; ++t) *reinterpret_cast<R*>(out + t * a.os) = no_row<T, V>();
     return;
   }
   const int len = s.t1 - s.t0;
+  const Taps<T, W, V> taps(a, d);
   // ext: the state's rows, then the first H tokens
-  float ext[2 * H][V], last[H][V];
+  R ext[2 * H];
 #pragma unroll
   for (int i = 0; i < 2 * H; ++i) {
     const T* p = i < H ? (s.init ? row + (int64_t)i * a.D : nullptr) : i - H < len ? x + (int64_t)(s.t0 + i - H) * a.xs : nullptr;
-    if (p) load_v<T, V>(p, ext[i]);
-    else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) ext[i][v] = 0.f;
-    }
+    ext[i] = p ? *reinterpret_cast<const R*>(p) : no_row<T, V>();
   }
   if (row) {
+    R last[H];
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      if (len >= H) load_v<T, V>(x + (int64_t)(s.t1 - H + i) * a.xs, last[i]);
+      if (len >= H) last[i] = *reinterpret_cast<const R*>(x + (int64_t)(s.t1 - H + i) * a.xs);
       else {
 #pragma unroll
-        for (int k = 0; k < H; ++k) {                 // ext[len + i], with the index known to the compiler
-          if (len == k) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) last[i][v] = ext[k + i][v];
-          }
-        }
+        for (int k = 0; k < H; ++k)                   // ext[len + i], with the index known to the compiler
+          if (len == k) last[i] = ext[k + i];
       }
     }
 #pragma unroll
-    for (int i = 0; i < H; ++i) store_v<T, V>(row + (int64_t)i * a.D, last[i]);
+    for (int i = 0; i < H; ++i) *reinterpret_cast<R*>(row + (int64_t)i * a.D) = last[i];
   }
-  const Taps<T, W, V> taps(a, d);
+  Chan<V> f[2 * H];
+#pragma unroll
+  for (int i = 0; i < 2 * H; ++i) f[i].from(ext[i]);
 #pragma unroll
   for (int i = 0; i < H; ++i)
-    if (i < len) taps.apply([&](int j) -> const float* { return ext[i + j]; }, a.silu, out + (int64_t)(s.t0 + i) * a.os);
+    if (i < len) taps.apply([&](int j) -> const Chan<V>& { return f[i + j]; }, a.silu, out + (int64_t)(s.t0 + i) * a.os);
+}
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvArgs a, int blocks_d) {
+  conv_sequence<T, W, V>(a, blockIdx.x / blocks_d, (blockIdx.x % blocks_d * kConvThreads + threadIdx.x) * V);
 }
 
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const ConvArgs a, int blocks_d, int runs) {
+  using R = Raw<T, V>;
   const int bd = blockIdx.x % blocks_d, unit = blockIdx.x / blocks_d;
   const int d = (bd * kConvThreads + threadIdx.x) * V;
   if (unit >= runs) {
     conv_sequence<T, W, V>(a, unit - runs, d);
     return;
   }
-  constexpr int H = W - 1, B = 4;                 // rows in flight
+  // B rows a group. Whole 16-byte parts of rows are copied asynchronously, kGroups - 1 groups ahead, into a ring of shared
+  // memory that is each thread's own, so nothing waits for other threads; narrower parts go through registers.
+  constexpr bool async = V * sizeof(T) == 16;
+  constexpr int H = W - 1, B = async ? 4 : 8, groups = kConvRun / B;
+  __shared__ R ring[async ? kGroups : 1][async ? B : 1][kConvThreads];
   const int t0 = unit * kConvRun;
-  const unsigned mask = tokens_inside<W>(a.seq, t0);
-  if (d >= a.D || !mask) return;
-  const T* x = static_cast<const T*>(a.x) + d;
-  T* out = static_cast<T*>(a.out) + d;
-  const Taps<T, W, V> taps(a, d);
-  float win[H + B][V];
-  auto row = [&](int t, float* f) {
-    if (t >= 0 && t < a.seq.T) load_v<T, V>(x + (int64_t)t * a.xs, f);
-    else {
+  const T* x = static_cast<const T*>(a.x) + d + (int64_t)t0 * a.xs;
+  auto row = [&](int i) { return t0 + i >= 0 && t0 + i < a.seq.T ? *reinterpret_cast<const R*>(x + i * a.xs) : no_row<T, V>(); };
+  R next[async ? 1 : B];
+  Chan<V> win[H + B];
+  auto fetch = [&](int g) {
+    if constexpr (async) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) f[v] = 0.f;
+      for (int i = 0; i < B; ++i)
+        if (g < groups && t0 + g * B + i < a.seq.T) copy_async<16>(&ring[g % kGroups][i][threadIdx.x], x + (g * B + i) * a.xs, true);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    } else if (g < groups) {
+#pragma unroll
+      for (int i = 0; i < B; ++i) next[i] = row(g * B + i);
     }
   };
+  if (d < a.D) {
 #pragma unroll
-  for (int i = 0; i < H; ++i) row(t0 - H + i, win[i]);
-  for (int r = 0; r < kConvRun; r += B) {
-    if (!(mask >> r)) return;
+    for (int g = 0; g < (async ? kGroups - 1 : 1); ++g) fetch(g);
 #pragma unroll
-    for (int i = 0; i < B; ++i) row(t0 + r + i, win[H + i]);
+    for (int i = 0; i < H; ++i) win[i].from(row(i - H));
+  }
+  const unsigned mask = tokens_inside<W>(a.seq, t0);
+  if (d >= a.D) return;
+  T* out = static_cast<T*>(a.out) + d + (int64_t)t0 * a.os;
+  const Taps<T, W, V> taps(a, d);
+  for (int g = 0; g < groups && mask >> g * B; ++g) {
+    if constexpr (async) {
+      fetch(g + kGroups - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kGroups - 1) : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) win[H + i].from(async ? ring[g % kGroups][i][threadIdx.x] : next[async ? 0 : i]);
+    if constexpr (!async) fetch(g + 1);
 #pragma unroll
     for (int i = 0; i < B; ++i)
-      if (mask >> (r + i) & 1)
-        taps.apply([&](int j) -> const float* { return win[i + j]; }, a.silu, out + (int64_t)(t0 + r + i) * a.os);
+      if (mask >> (g * B + i) & 1)
+        taps.apply([&](int j) -> const Chan<V>& { return win[i + j]; }, a.silu, out + (int64_t)(g * B + i) * a.os);
 #pragma unroll
-    for (int i = 0; i < H; ++i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) win[i][v] = win[B + i][v];
+    for (int i = 0; i < H; ++i) win[i] = win[B + i];
   }
+  if constexpr (async) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename T, int W, int V>
@@ -157,20 +201,26 @@ const char* launch(const ConvArgs& a, cudaStream_t st) {
   const int64_t runs = a.seq.step ? 0 : (a.seq.T + (int64_t)kConvRun - 1) / kConvRun;
   const int64_t grid = blocks_d * (runs + a.seq.N);
   if (grid >= (1ll << 31)) return "causal_conv: too many tokens, sequences or channels for one call";
-  if (grid) causal_conv_kernel<T, W, V><<<(unsigned)grid, kConvThreads, 0, st>>>(a, (int)blocks_d, (int)runs);
+  if (!grid) return nullptr;
+  if (a.seq.step) conv_step_kernel<T, W, V><<<(unsigned)grid, kConvThreads, 0, st>>>(a, (int)blocks_d);
+  else causal_conv_kernel<T, W, V><<<(unsigned)grid, kConvThreads, 0, st>>>(a, (int)blocks_d, (int)runs);
   return nullptr;
 }
 
 }  // namespace
 
-const char* launch_causal_conv(const ConvArgs& a, bool f32, bool vec, cudaStream_t st) {
-#define AIR_CONV(N)                                                                               \
-  if (a.W == N) return f32 ? (vec ? launch<float, N, 4>(a, st) : launch<float, N, 1>(a, st))      \
-                           : (vec ? launch<__nv_bfloat16, N, 8>(a, st) : launch<__nv_bfloat16, N, 1>(a, st));
+const char* launch_causal_conv(const ConvArgs& a, bool f32, int vec, cudaStream_t st) {
+#define AIR_CONV_V(N, T) return vec * sizeof(T) >= 16 && !a.seq.step ? launch<T, N, 16 / sizeof(T)>(a, st) : vec >= 4 ? launch<T, N, 4>(a, st) : vec == 2 ? launch<T, N, 2>(a, st) : launch<T, N, 1>(a, st)
+#define AIR_CONV(N)                     \
+  if (a.W == N) {                       \
+    if (f32) AIR_CONV_V(N, float);      \
+    AIR_CONV_V(N, __nv_bfloat16);       \
+  }
   AIR_CONV(2)
   AIR_CONV(3)
   AIR_CONV(4)
 #undef AIR_CONV
+#undef AIR_CONV_V
   return "causal_conv: 2 to 4 taps";
 }
 

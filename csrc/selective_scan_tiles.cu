@@ -137,20 +137,6 @@ struct TileArgs {
   float* sum;              // [tiles][D] sum of delta over its tokens in the tile
 };
 
-// B bytes from global to shared memory (4, 8 or a multiple of 16), zeros instead where `in` is false.
-template <int B>
-AIR_DEVICE void copy_async(void* dst, const void* src, bool in) {
-  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-  if constexpr (B >= 16) {
-#pragma unroll
-    for (int i = 0; i < B; i += 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                   ::"r"(d + i), "l"(static_cast<const char*>(src) + i), "r"(in ? 16 : 0) : "memory");
-  } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(B), "r"(in ? B : 0) : "memory");
-  }
-}
-
 // ---- helpers: delta and delta x of a stage, B and C, and the output from y. A helper fetches, prepares and finishes the
 // same E channels of the same token of each stage, and the same groups of four values of B and C.
 template <typename T, int L, bool FIRST>

@@ -89,6 +89,20 @@ AIR_DEVICE void store_v(T* p, const float* f) {
   }
 }
 
+// B bytes from global to shared memory (4, 8 or a multiple of 16), zeros instead where `in` is false.
+template <int B>
+AIR_DEVICE void copy_async(void* dst, const void* src, bool in) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (B >= 16) {
+#pragma unroll
+    for (int i = 0; i < B; i += 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                   ::"r"(d + i), "l"(static_cast<const char*>(src) + i), "r"(in ? 16 : 0) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(B), "r"(in ? B : 0) : "memory");
+  }
+}
+
 // 1 / (1 + exp(-x)) and x / (1 + exp(-x)); the division is exact to 2 ulp and 0 where exp(-x) passes 2^126.
 AIR_DEVICE float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 AIR_DEVICE float silu_f(float x) { return __fdividef(x, 1.f + __expf(-x)); }

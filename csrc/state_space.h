@@ -27,8 +27,8 @@ struct ConvArgs {
   void* state;             // [S, W - 1, D], the type of x: the last inputs, the newest in the last row (null: none)
   int D, W, silu;
 };
-// 2 <= W <= 4. `vec`: x, out, state, w and bias are 16-byte aligned and so are their rows (D a multiple of 8).
-const char* launch_causal_conv(const ConvArgs& a, bool f32, bool vec, cudaStream_t st);
+// 2 <= W <= 4. vec = 8, 4, 2 or 1 divides D, the rows of x, out and state are aligned to vec elements, w to 16 bytes.
+const char* launch_causal_conv(const ConvArgs& a, bool f32, int vec, cudaStream_t st);
 
 struct ScanArgs {
   SeqArgs seq;

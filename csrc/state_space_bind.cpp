@@ -158,8 +158,13 @@ Tensor conv(const char* op, const Tensor& x, const Tensor& w, const optional<Ten
   a.D = (int)D;
   a.W = (int)W;
   a.silu = silu;
-  const bool vec = D % 8 == 0 && aligned(x, 16) && aligned(out, 16) && aligned(w, 16) && (!bias.has_value() || aligned(*bias, 16)) &&
-                   (!state.has_value() || aligned(*state, 16));
+  int vec = !aligned(w, 16) ? 1 : x.scalar_type() == at::kFloat ? 4 : 8;
+  auto rows = [&](const Tensor& t) {
+    while (vec > 1 && (D % vec || !aligned(t, vec * t.element_size()))) vec /= 2;
+  };
+  rows(x);
+  rows(out);
+  if (state.has_value()) rows(*state);
   const char* e = air::launch_causal_conv(a, x.scalar_type() == at::kFloat, vec, at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(e == nullptr, e ? e : "");
   post(op);
