@@ -66,7 +66,7 @@ AIR_DEVICE void decays(const f2* u, f2* p) {
 }
 // softplus_f of a pair
 AIR_DEVICE f2 softplus2(float a, float b) {
-  const f2 u = pack2(__expf(-fabsf(a)), __expf(-fabsf(b)));
+  const f2 u = pack2(exp2_fast(fabsf(a) * -kLog2e), exp2_fast(fabsf(b) * -kLog2e));
   f2 p = fma2(dup2(0.00523269409f), u, dup2(-0.0295052398f));
   p = fma2(p, u, dup2(0.0782259554f));
   p = fma2(p, u, dup2(-0.136632457f));
@@ -247,7 +247,9 @@ struct Helper {
     out += S::TS * a.os;
     if (live <= 0 || !(mask >> tok & 1)) return;
     const int slot = k % kRing;
-    float y[E], f[E];
+    float y[E], f[E], g[E];
+    if (a.skip) load_v<T, E>(sm.rows[slot][0][tid], f);
+    if (a.z) load_v<T, E>(sm.rows[slot][2][tid], g);
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
       f2 sum = 0ull;
@@ -256,17 +258,9 @@ struct Helper {
         const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.y[k & 1][tok][y_slot<L, E>((c + i) / 2, q)]);
         sum = q ? add2(sum, add2(v.x, v.y)) : add2(v.x, v.y);
       }
+      if (a.skip) sum = fma2(pack2(skip[i], skip[i + 1]), pack2(f[i], f[i + 1]), sum);
+      if (a.z) sum = mul2(sum, silu2(pack2(g[i], g[i + 1])));
       unpack2(sum, y[i], y[i + 1]);
-    }
-    if (a.skip) {
-      load_v<T, E>(sm.rows[slot][0][tid], f);
-#pragma unroll
-      for (int i = 0; i < E; ++i) y[i] = fmaf(skip[i], f[i], y[i]);
-    }
-    if (a.z) {
-      load_v<T, E>(sm.rows[slot][2][tid], f);
-#pragma unroll
-      for (int i = 0; i < E; ++i) y[i] *= silu_f(f[i]);
     }
     if (vec) store_v<T, E>(o, y);
     else {

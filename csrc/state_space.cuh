@@ -16,6 +16,8 @@ AIR_DEVICE T from_f(float v) {
   else return v;
 }
 
+constexpr float kLog2e = 1.44269504f;
+
 // ---- paired f32 arithmetic
 using f2 = unsigned long long;       // two floats, the operand of the paired instructions
 AIR_DEVICE f2 pack2(float a, float b) {
@@ -103,15 +105,27 @@ AIR_DEVICE void copy_async(void* dst, const void* src, bool in) {
   }
 }
 
-// 1 / (1 + exp(-x)) and x / (1 + exp(-x)); the division is exact to 2 ulp and 0 where exp(-x) passes 2^126.
-AIR_DEVICE float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-AIR_DEVICE float silu_f(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+// 1 / (1 + exp(-x)) and x / (1 + exp(-x)). Subnormals count as zero in the exponential and the reciprocal: without that
+// each of them costs three to four instructions more, for values below 2^-126.
+AIR_DEVICE float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+AIR_DEVICE float sigmoid_f(float x) { return rcp_fast(1.f + exp2_fast(x * -kLog2e)); }
+AIR_DEVICE float silu_f(float x) { return x * sigmoid_f(x); }
+AIR_DEVICE f2 silu2(f2 x) {
+  float a, b;
+  unpack2(mul2(x, dup2(-kLog2e)), a, b);
+  unpack2(add2(pack2(exp2_fast(a), exp2_fast(b)), dup2(1.f)), a, b);
+  return mul2(x, pack2(rcp_fast(a), rcp_fast(b)));
+}
 
 // log(1 + exp(x)) = max(x, 0) + log(1 + u), u = exp(-|x|) in [0, 1]. The logarithm is u P(u) with P of degree 8 (equal
 // ripple of the relative error, computed for this interval: 3.0e-8, 1.7e-7 with the roundings): small steps keep their
 // relative accuracy, which the logarithm of the rounded sum 1 + u would lose, and it needs no special-function unit.
 AIR_DEVICE float softplus_f(float x) {
-  const float u = __expf(-fabsf(x));
+  const float u = exp2_fast(fabsf(x) * -kLog2e);
   float p = fmaf(0.00523269409f, u, -0.0295052398f);
   p = fmaf(p, u, 0.0782259554f);
   p = fmaf(p, u, -0.136632457f);
@@ -132,7 +146,6 @@ AIR_DEVICE float decay_m1(float u) {
   const float e = exp2_fast(u), p = fmaf(fmaf(kDecay2, u, kDecay1), u, kDecay0);
   return fabsf(u) <= kNearDecay ? p * u : e - 1.f;
 }
-constexpr float kLog2e = 1.44269504f;
 
 struct SeqRange {
   int t0, t1;        // tokens [t0, t1)
@@ -157,6 +170,14 @@ AIR_DEVICE SeqRange seq_range(const SeqArgs& a, int n, bool report = true) {
   }
   s.init = s.slot >= 0 && (a.has_state ? a.has_state[n] != 0 : a.has_state_all != 0);
   return s;
+}
+
+// State row of single token n (SeqArgs with `step`), -1: none.
+AIR_DEVICE int64_t state_row(const SeqArgs& a, int n, bool report) {
+  const int64_t slot = a.slots ? (int64_t)a.slots[n] : (int64_t)n;
+  if (slot >= 0 && slot < a.S) return slot;
+  if (slot != -1 && report) set_error(a.err, kErrBounds);
+  return -1;
 }
 
 // The sequence that holds token t among rising offsets, by the whole warp: the last n with cu[n] <= t, in steps that
