@@ -15,6 +15,7 @@ which is the reference's Candle-CPU path.
 """
 from __future__ import annotations
 
+import math
 import dataclasses
 import itertools
 import time
@@ -846,20 +847,34 @@ class Engine:
         """Per-token log-probabilities of ``ids`` under the model, each given everything before
         it (BOS included when added): one forward over all rows on the GPU, teacher forcing
         on the CPU oracle. Used by the eval harness."""
+        return self.token_scores(ids, add_bos).logprobs.tolist()
+
+    def token_scores(self, ids: list[int], add_bos: bool | None = None, top: int = 0):
+        """:meth:`token_logprobs` with the entropy at each position and its ``top`` most likely tokens (at most 32), as
+        ``ops.TokenLogprobs`` of CPU tensors."""
+        from .. import ops
+        if not 0 <= top <= 32:
+            raise ValueError(f"token_scores: 0 to 32 alternatives, not {top}")
         bos = self.add_bos if add_bos is None else add_bos
         ids = ([self.cfg.bos_token_id] if bos else []) + list(ids)
         T = len(ids)
         if T < 2:
-            return []
+            return ops.TokenLogprobs(torch.empty(0), torch.empty(0), torch.empty(0, top), torch.empty(0, top, dtype=torch.int32))
         if self.runner is None:
             self.oracle.reset()
-            out = []
+            lps, ents, tops, order = [], [], torch.full((T - 1, top), -math.inf), torch.full((T - 1, top), -1, dtype=torch.int32)
             logits = self.oracle.forward(ids[:1], 0)
             for i in range(1, T):
-                out.append(float(torch.log_softmax(logits.float(), -1)[ids[i]]))
+                lp = torch.log_softmax(logits.float(), -1)
+                p = lp.exp()
+                lps.append(lp[ids[i]])
+                ents.append(-torch.where(p > 0, p * lp, torch.zeros(())).sum())
+                best = torch.sort(lp, descending=True, stable=True)
+                k = min(top, lp.numel())
+                tops[i - 1, :k], order[i - 1, :k] = best.values[:k], best.indices[:k].to(torch.int32)
                 logits = self.oracle.forward([ids[i]], i)
             self.oracle.reset()
-            return out
+            return ops.TokenLogprobs(torch.stack(lps), torch.stack(ents), tops, order.masked_fill(tops == -math.inf, -1))
         rn = self.runner
         dev = rn.device
         seq = self.seqs.create_sequence()
@@ -867,15 +882,15 @@ class Engine:
             slots = self.seqs.append(seq, T)
             tab = torch.full((1, rn.max_blocks), -1, dtype=torch.int32)
             self.seqs.fill_table([seq], tab)
-            lg = rn.prefill(torch.tensor(ids, dtype=torch.int32, device=dev),
+            tok = torch.tensor(ids, dtype=torch.int32, device=dev)
+            lg = rn.prefill(tok,
                             torch.arange(T, dtype=torch.int32, device=dev),
                             torch.tensor(slots, dtype=torch.int64, device=dev),
                             torch.zeros(T, dtype=torch.int32, device=dev), tab.to(dev),
                             torch.arange(T - 1, dtype=torch.int64, device=dev), None, None, None, None,
                             None, return_logits=True)
-            lp = torch.log_softmax(lg.float(), -1)
-            tgt = torch.tensor(ids[1:], dtype=torch.long, device=dev)
-            return lp.gather(1, tgt[:, None]).squeeze(1).tolist()
+            r = ops.token_logprobs(lg, tok[1:], top=top)
+            return ops.TokenLogprobs(*(t.cpu() for t in r))
         finally:
             self.seqs.free_sequence(seq)
 

@@ -8,8 +8,8 @@
 //
 // A block has eight scan warps and eight helper warps. L lanes share a pair of channels, each with two states of both: the
 // arithmetic runs on pairs of channels (f32x2), so the steps of a pair are one operand and B and C, stored twice, another,
-// and y of the pair comes out as one. Stage by stage of TS tokens, with one barrier a stage, the helpers turn dt and x of
-// the next stage into delta and delta x, and the lanes' parts of y of the last one into the output (sum, skip, gate,
+// and y of the pair comes out as one. Stage by stage of TS tokens, through two sets of buffers, the helpers turn dt and x of the
+// next stages into delta and delta x, and the lanes' parts of y of the last one into the output (sum, skip, gate,
 // rounding), so all global accesses are theirs: whole rows, copied asynchronously six stages ahead.
 //
 // The tokens of all sequences lie in one row of tiles of equal length; a block walks through its tile and loads or
@@ -83,7 +83,12 @@ AIR_DEVICE f2 softplus2(float a, float b) {
 #endif
 constexpr int kGroup = KG;           // tokens whose decays are computed together
 constexpr int kScan = 256, kHelp = 256, kThreads = kScan + kHelp;   // eight scan warps, eight helper warps
-AIR_DEVICE void stage_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+// Hand-over of a stage's buffers: each has a barrier for "prepared" and one for "scanned"; the side that gives arrives,
+// the side that takes waits.
+AIR_DEVICE void give(int barrier) { asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
+AIR_DEVICE void take(int barrier) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
+AIR_DEVICE int prepared(int k) { return 1 + (k & 1); }
+AIR_DEVICE int scanned(int k) { return 3 + (k & 1); }
 
 template <int L>
 struct Shape {
@@ -93,7 +98,7 @@ struct Shape {
   static constexpr int E = CH * TS / kHelp > 1 ? CH * TS / kHelp : 2;   // channels of a helper's access
   static constexpr int HT = CH / E;                      // helpers a token
 };
-constexpr int kRing = 8, kAhead = 6; // stages of raw rows: `kAhead` being fetched, one prepared, one finished
+constexpr int kRing = 8, kAhead = 6; // stages of raw rows: up to `kAhead` being fetched, two prepared
 template <typename T, int L>
 struct Smem {
   using S = Shape<L>;
@@ -406,14 +411,19 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
 
   if (threadIdx.x >= kScan) {
     Helper<T, L, FIRST> w(a, sm, d0, grp, left, vec, t0, t1);
+    auto next = [&](int k) {                                 // stage k's buffers
+      if (k > 0) w.fetch();
+      w.arrived();
+      w.prepare(k, t0 + k * S::TS + w.tok < t1);
+      give(prepared(k));
+    };
     if (stages > 0) {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) w.fetch();
-      w.arrived();
-      w.prepare(0, t0 + w.tok < t1);
+      next(0);
+      if (stages > 1) next(1);
     }
-    stage_barrier();
-    if (!FIRST && tile < ta.tiles && a.seq.S > 0) {
+    if (!FIRST && a.seq.S > 0) {
       // offsets and rows that are not sound are reported once, empty sequences without a state start one of zeros
       for (int n = tile * kHelp + w.tid; n < a.seq.N; n += ta.tiles * kHelp) {
         const SeqRange s = seq_range(a.seq, n, blk == 0);
@@ -424,23 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
       for (int n = tile * kHelp + w.tid; n < a.seq.N; n += ta.tiles * kHelp) seq_range(a.seq, n);
     }
     for (int k = 0; k < stages; ++k) {
-      w.fetch();
-      w.arrived();
-      if (k + 1 < stages) w.prepare(k + 1, t0 + (k + 1) * S::TS + w.tok < t1);
-      if (!FIRST && k > 0) {
-        const int t = t0 + (k - 1) * S::TS;
-        unsigned mask = ~0u;
-        if (seg.n < 0 || t < seg.lo || t + S::TS > seg.hi) {
-          mask = tokens_inside<1>(a.seq, t);
-          seg = segment_at(a.seq, min(t + S::TS, a.seq.T - 1));
-        }
-        w.finish(k - 1, mask & (t + S::TS <= t1 ? ~0u : (1u << (t1 - t)) - 1));
+      const int t = t0 + k * S::TS;
+      unsigned mask = ~0u;
+      if (!FIRST && (seg.n < 0 || t < seg.lo || t + S::TS > seg.hi)) {
+        mask = tokens_inside<1>(a.seq, t);
+        seg = segment_at(a.seq, min(t + S::TS, a.seq.T - 1));
       }
-      stage_barrier();
-    }
-    if (!FIRST && stages > 0) {
-      const int t = t0 + (stages - 1) * S::TS;
-      w.finish(stages - 1, tokens_inside<1>(a.seq, t) & (t + S::TS <= t1 ? ~0u : (1u << (t1 - t)) - 1));
+      take(scanned(k));
+      if (!FIRST) w.finish(k, mask & (t + S::TS <= t1 ? ~0u : (1u << (t1 - t)) - 1));
+      if (k + 2 < stages) next(k + 2);
     }
     return;
   }
@@ -488,9 +490,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
   };
   enter(t0);
   float total[2] = {0.f, 0.f}, low[2] = {0.f, 0.f};          // the sum of delta and what its roundings lost
-  stage_barrier();
   for (int k = 0; k < stages; ++k) {
     const int t = t0 + k * S::TS;
+    take(prepared(k));
     f2 sum2 = 0ull;
     if (FIRST || t + S::TS <= seg.hi) {
       w.template stage<!FIRST>(k & 1, sum2);
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
         total[s_] = n;
       }
     }
-    stage_barrier();
+    give(scanned(k));
   }
   if (FIRST) {
     w.store(ta.h + tile * row, al);
