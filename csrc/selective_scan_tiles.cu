@@ -78,27 +78,28 @@ AIR_DEVICE f2 softplus2(float a, float b) {
   return fma2(p, u, pack2(fmaxf(a, 0.f), fmaxf(b, 0.f)));
 }
 
-#ifndef KG
-#define KG 2
-#endif
-constexpr int kGroup = KG;           // tokens whose decays are computed together
-constexpr int kScan = 256, kHelp = 256, kThreads = kScan + kHelp;   // eight scan warps, eight helper warps
+constexpr int kGroup = 2;           // tokens whose decays are computed together
 // Hand-over of a stage's buffers: each has a barrier for "prepared" and one for "scanned"; the side that gives arrives,
 // the side that takes waits.
-AIR_DEVICE void give(int barrier) { asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
-AIR_DEVICE void take(int barrier) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kThreads) : "memory"); }
+template <int THREADS>
+AIR_DEVICE void give(int barrier) { asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "n"(THREADS) : "memory"); }
+template <int THREADS>
+AIR_DEVICE void take(int barrier) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(THREADS) : "memory"); }
 AIR_DEVICE int prepared(int k) { return 1 + (k & 1); }
 AIR_DEVICE int scanned(int k) { return 3 + (k & 1); }
 
 template <int L>
 struct Shape {
-  static constexpr int CH = 512 / L, CP = CH / 2;        // channels a block, and pairs
+  // Threads that scan, and as many helpers. Two blocks an SM of 128 + 128, or, where many lanes share a pair and a block of
+  // that size would have few channels to share B and C, one of 256 + 256 (8000 x 2048 with 64 states: 607 against 765 us).
+  static constexpr int SCAN = L <= 16 ? 128 : 256, HELP = SCAN, THREADS = SCAN + HELP, BLOCKS = 256 / SCAN;
+  static constexpr int CH = 2 * SCAN / L, CP = CH / 2;   // channels a block, and pairs
   static constexpr int TS = L <= 4 ? 8 : 16;             // tokens a stage
   static constexpr int NP = 2 * L;                       // states, padded
-  static constexpr int E = CH * TS / kHelp > 1 ? CH * TS / kHelp : 2;   // channels of a helper's access
+  static constexpr int E = CH * TS / HELP > 1 ? CH * TS / HELP : 2;   // channels of a helper's access
   static constexpr int HT = CH / E;                      // helpers a token
 };
-constexpr int kRing = 8, kAhead = 6; // stages of raw rows: up to `kAhead` being fetched, two prepared
+constexpr int kRing = 4, kAhead = 3; // stages of raw rows: up to `kAhead` being fetched, two prepared
 template <typename T, int L>
 struct Smem {
   using S = Shape<L>;
@@ -106,7 +107,9 @@ struct Smem {
   alignas(16) float4 step[2][S::TS][S::CP];              // delta of the pair, delta x of the pair
   alignas(16) float4 bc[2][S::TS][L];                    // B and C of a lane's two states
   alignas(16) float2 y[2][S::TS][S::CP * L];             // the lanes' parts of y of the pair
-  alignas(16) T rows[kRing][3][kHelp][S::E];               // x, dt, z: each helper's own part
+  // x, dt, z: each helper's own part, with room for the words that rows of bf16 at odd addresses start and end in
+  static constexpr int W = sizeof(T) == 2 ? 2 * S::E : S::E;
+  alignas(16) T rows[kRing][3][S::HELP][W];
   alignas(16) T raw_bc[kRing][BC][4];
 };
 // Where a pair lies in `step` and a lane's part in `y`: helpers write or read E channels each, and without the exchange
@@ -144,16 +147,17 @@ struct TileArgs {
 
 // ---- helpers: delta and delta x of a stage, B and C, and the output from y. A helper fetches, prepares and finishes the
 // same E channels of the same token of each stage, and the same groups of four values of B and C.
-template <typename T, int L, bool FIRST>
+// VEC: its part of a row is one aligned access.
+template <typename T, int L, bool FIRST, bool VEC>
 struct Helper {
   using S = Shape<L>;
   using M = Smem<T, L>;
-  static constexpr int E = S::E, NB = (M::BC + kHelp - 1) / kHelp;
+  static constexpr int E = S::E, NB = (M::BC + S::HELP - 1) / S::HELP;
   const ScanArgs& a;
   M& sm;
   const int tid, tok, c;            // helper: token of the stage, first channel in the block
   const int live;                   // channels there are from c on, up to E
-  const bool vec, vec_bc;           // rows (B and C) can be copied in whole accesses
+  const bool vec_bc;                // B and C can be copied in whole accesses
   const int t1;
   int tf, tb[NB];                   // tokens of the next fetch
   const T *x, *dt, *z, *bc[NB];     // and its rows
@@ -162,15 +166,19 @@ struct Helper {
   bool has_bc[NB];                  // padded states have none
   int ring;                         // stages fetched, as a place in the ring
   float bias[E], skip[E];
+  int odd[3];                       // where a row's part starts in its first 4-byte word (the same at every stage: TS is even)
 
-  AIR_DEVICE Helper(const ScanArgs& a_, M& s, int64_t d0, int64_t g, int left, int v, int t0, int end)
-      : a(a_), sm(s), tid(threadIdx.x - kScan), tok(tid / S::HT), c(tid % S::HT * E),
-        live(tok < S::TS ? max(0, min(E, left - c)) : 0), vec(v & 1), vec_bc(v & 2), t1(end), tf(t0 + tok), ring(0) {
+  AIR_DEVICE Helper(const ScanArgs& a_, M& s, int64_t d0, int64_t g, int left, bool v, int t0, int end)
+      : a(a_), sm(s), tid(threadIdx.x - S::SCAN), tok(tid / S::HT), c(tid % S::HT * E),
+        live(tok < S::TS ? max(0, min(E, left - c)) : 0), vec_bc(v), t1(end), tf(t0 + tok), ring(0) {
     const int64_t d = d0 + c;
     x = static_cast<const T*>(a.x) + (int64_t)tf * a.xs + d;
     dt = static_cast<const T*>(a.dt) + (int64_t)tf * a.ds + d;
     z = a.z ? static_cast<const T*>(a.z) + (int64_t)tf * a.zs + d : nullptr;
     out = static_cast<T*>(a.out) + (int64_t)tf * a.os + d;
+    const T* rows[3] = {x, dt, z};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) odd[i] = VEC || sizeof(T) == 4 ? 0 : reinterpret_cast<uintptr_t>(rows[i]) >> 1 & 1;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       bias[i] = a.dt_bias && i < live ? a.dt_bias[d + i] : 0.f;
@@ -178,7 +186,7 @@ struct Helper {
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {  // four states of a token of B (the first half of the groups) or C
-      const int i = tid + kHelp * j, at = i % (M::BC / 2) * 4, n = at % S::NP;
+      const int i = tid + S::HELP * j, at = i % (M::BC / 2) * 4, n = at % S::NP;
       const bool is_c = i >= M::BC / 2;
       tb[j] = t0 + at / S::NP;
       bc_stride[j] = is_c ? a.cs_t : a.bs_t;
@@ -186,26 +194,41 @@ struct Helper {
       has_bc[j] = n < a.N;
     }
   }
-  AIR_DEVICE void row(T* dst, const T* p, const void* any, bool in) {
-    if (vec) copy_async<E * (int)sizeof(T)>(dst, in ? p : any, in);
+  AIR_DEVICE void row(int which, const T* p, const void* any, bool in) {
+    T* dst = sm.rows[ring][which][tid];
+    if constexpr (VEC) copy_async<E * (int)sizeof(T)>(dst, in ? p : any, in);
     else {
+      // word by word: those that hold one of the row's elements, so nothing past the row's own words is read
+      constexpr int per = 4 / sizeof(T);
 #pragma unroll
-      for (int i = 0; i < E; ++i) dst[i] = in && i < live ? p[i] : from_f<T>(0.f);
+      for (int j = 0; j < E / per + per - 1; ++j) {
+        const bool some = in && j * per - odd[which] < live;
+        copy_async<4>(dst + j * per, some ? p - odd[which] + j * per : any, some);
+      }
     }
   }
-  // The next stage's rows, complete for this helper after arrived() with at most kAhead - 1 stages fetched after it
+  // E elements of a fetched row; what is not there is zero
+  AIR_DEVICE void read(int slot, int which, float* f) const {
+    const T* p = sm.rows[slot][which][tid];
+    if constexpr (VEC) load_v<T, E>(p, f);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = i < live ? to_f(p[odd[which] + i]) : 0.f;
+    }
+  }
+  // The next stage's rows, complete for this helper after arrived() with kAhead - 1 stages fetched after it
   AIR_DEVICE void fetch() {
     const bool in = tf < t1 && live > 0;
-    row(sm.rows[ring][0][tid], x, a.x, in);
-    row(sm.rows[ring][1][tid], dt, a.dt, in);
-    if (!FIRST && a.z) row(sm.rows[ring][2][tid], z, a.z, in);
+    row(0, x, a.x, in);
+    row(1, dt, a.dt, in);
+    if (!FIRST && a.z) row(2, z, a.z, in);
     tf += S::TS;
     x += S::TS * a.xs;
     dt += S::TS * a.ds;
     z += S::TS * a.zs;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int i = tid + kHelp * j;
+      const int i = tid + S::HELP * j;
       if (i >= (FIRST ? M::BC / 2 : M::BC)) continue;
       const bool in_ = tb[j] < t1 && has_bc[j];
       if (vec_bc) copy_async<4 * (int)sizeof(T)>(sm.raw_bc[ring][i], in_ ? bc[j] : a.B, in_);
@@ -225,10 +248,10 @@ struct Helper {
   AIR_DEVICE void prepare(int k, bool in) {
     const int slot = k % kRing;
     float xv[E], dv[E];
-    load_v<T, E>(sm.rows[slot][0][tid], xv);
-    load_v<T, E>(sm.rows[slot][1][tid], dv);
+    read(slot, 0, xv);
+    read(slot, 1, dv);
 #pragma unroll
-    for (int i = 0; i < E && (S::HT * S::TS == kHelp || tok < S::TS); i += 2) {
+    for (int i = 0; i < E && (S::HT * S::TS == S::HELP || tok < S::TS); i += 2) {
       float v = dv[i] + bias[i], w = dv[i + 1] + bias[i + 1];
       if (a.softplus) unpack2(softplus2(v, w), v, w);
       if (!in) v = w = 0.f;
@@ -236,7 +259,7 @@ struct Helper {
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int i = tid + kHelp * j;
+      const int i = tid + S::HELP * j;
       if (i >= (FIRST ? M::BC / 2 : M::BC)) continue;
       float f[4];
       load_v<T, 4>(sm.raw_bc[slot][i], f);
@@ -253,8 +276,8 @@ struct Helper {
     if (live <= 0 || !(mask >> tok & 1)) return;
     const int slot = k % kRing;
     float y[E], f[E], g[E];
-    if (a.skip) load_v<T, E>(sm.rows[slot][0][tid], f);
-    if (a.z) load_v<T, E>(sm.rows[slot][2][tid], g);
+    if (a.skip) read(slot, 0, f);
+    if (a.z) read(slot, 2, g);
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
       f2 sum = 0ull;
@@ -267,7 +290,7 @@ struct Helper {
       if (a.z) sum = mul2(sum, silu2(pack2(g[i], g[i + 1])));
       unpack2(sum, y[i], y[i + 1]);
     }
-    if (vec) store_v<T, E>(o, y);
+    if constexpr (VEC) store_v<T, E>(o, y);
     else {
 #pragma unroll
       for (int i = 0; i < E; ++i)
@@ -385,8 +408,8 @@ AIR_DEVICE bool starts_from(const SeqArgs& a, int n, int64_t& slot) {
   return s.init;
 }
 
-template <typename T, int L, bool FIRST>
-__global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_constant__ ScanArgs a, const __grid_constant__ TileArgs ta, int vec) {
+template <typename T, int L, bool FIRST, bool VEC>
+__global__ void __launch_bounds__(Shape<L>::THREADS, Shape<L>::BLOCKS) scan_tiles_kernel(const __grid_constant__ ScanArgs a, const __grid_constant__ TileArgs ta, bool vec_bc) {
   using S = Shape<L>;
   extern __shared__ __align__(16) uint8_t raw_smem[];
   Smem<T, L>& sm = *reinterpret_cast<Smem<T, L>*>(raw_smem);
@@ -409,13 +432,13 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
   const int stages = idle ? 0 : (t1 - t0 + S::TS - 1) / S::TS;
   const int64_t row = (int64_t)a.D * a.N;
 
-  if (threadIdx.x >= kScan) {
-    Helper<T, L, FIRST> w(a, sm, d0, grp, left, vec, t0, t1);
+  if (threadIdx.x >= S::SCAN) {
+    Helper<T, L, FIRST, VEC> w(a, sm, d0, grp, left, vec_bc, t0, t1);
     auto next = [&](int k) {                                 // stage k's buffers
       if (k > 0) w.fetch();
       w.arrived();
       w.prepare(k, t0 + k * S::TS + w.tok < t1);
-      give(prepared(k));
+      give<S::THREADS>(prepared(k));
     };
     if (stages > 0) {
 #pragma unroll
@@ -425,13 +448,13 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
     }
     if (!FIRST && a.seq.S > 0) {
       // offsets and rows that are not sound are reported once, empty sequences without a state start one of zeros
-      for (int n = tile * kHelp + w.tid; n < a.seq.N; n += ta.tiles * kHelp) {
+      for (int n = tile * S::HELP + w.tid; n < a.seq.N; n += ta.tiles * S::HELP) {
         const SeqRange s = seq_range(a.seq, n, blk == 0);
         if (a.seq.cu && s.slot >= 0 && s.t0 == s.t1 && !s.init)
           for (int64_t i = d0 * a.N; i < (d0 + min(left, S::CH)) * a.N; ++i) a.state[s.slot * row + i] = 0.f;
       }
     } else if (!FIRST && blk == 0) {
-      for (int n = tile * kHelp + w.tid; n < a.seq.N; n += ta.tiles * kHelp) seq_range(a.seq, n);
+      for (int n = tile * S::HELP + w.tid; n < a.seq.N; n += ta.tiles * S::HELP) seq_range(a.seq, n);
     }
     for (int k = 0; k < stages; ++k) {
       const int t = t0 + k * S::TS;
@@ -440,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
         mask = tokens_inside<1>(a.seq, t);
         seg = segment_at(a.seq, min(t + S::TS, a.seq.T - 1));
       }
-      take(scanned(k));
+      take<S::THREADS>(scanned(k));
       if (!FIRST) w.finish(k, mask & (t + S::TS <= t1 ? ~0u : (1u << (t1 - t)) - 1));
       if (k + 2 < stages) next(k + 2);
     }
@@ -492,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
   float total[2] = {0.f, 0.f}, low[2] = {0.f, 0.f};          // the sum of delta and what its roundings lost
   for (int k = 0; k < stages; ++k) {
     const int t = t0 + k * S::TS;
-    take(prepared(k));
+    take<S::THREADS>(prepared(k));
     f2 sum2 = 0ull;
     if (FIRST || t + S::TS <= seg.hi) {
       w.template stage<!FIRST>(k & 1, sum2);
@@ -516,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tiles_kernel(const __grid_co
         total[s_] = n;
       }
     }
-    give(scanned(k));
+    give<S::THREADS>(scanned(k));
   }
   if (FIRST) {
     w.store(ta.h + tile * row, al);
@@ -536,47 +559,57 @@ int channel_blocks(const ScanArgs& a) {
 
 int lanes_of(int N) { return N <= 8 ? 4 : N <= 16 ? 8 : N <= 32 ? 16 : 32; }
 
-template <typename T, int L>
-const char* launch(const ScanArgs& a, const ScanPlan& p, float* ws, cudaStream_t st) {
+template <typename T, int L, bool VEC>
+const char* launch(const ScanArgs& a, const ScanPlan& p, float* ws, bool vec_bc, cudaStream_t st) {
   using S = Shape<L>;
   const int64_t row = (int64_t)a.D * a.N;
   TileArgs ta{p.tiles, p.tile, channel_blocks<L>(a), ws, ws + p.tiles * row, ws + 2 * p.tiles * row};
   const int64_t blocks = (int64_t)ta.blocks_g * a.G;
   if (blocks * p.tiles >= (1ll << 31)) return "selective_scan: too many channels and tokens for one call";
+  constexpr int bytes = sizeof(Smem<T, L>);
+  static unsigned long long done1 = 0, done2 = 0;
+  if (!set_max_smem_per_device(scan_tiles_kernel<T, L, true, VEC>, bytes, done1) ||
+      !set_max_smem_per_device(scan_tiles_kernel<T, L, false, VEC>, bytes, done2))
+    return "selective_scan: the device has too little shared memory";
+  if (p.tiles > 1) scan_tiles_kernel<T, L, true, VEC><<<(unsigned)(blocks * (p.tiles - 1)), S::THREADS, bytes, st>>>(a, ta, vec_bc);
+  scan_tiles_kernel<T, L, false, VEC><<<(unsigned)(blocks * p.tiles), S::THREADS, bytes, st>>>(a, ta, vec_bc);
+  return nullptr;
+}
+
+template <typename T, int L>
+const char* launch(const ScanArgs& a, const ScanPlan& p, float* ws, cudaStream_t st) {
   auto ok = [](const void* q, int64_t stride, int bytes) {
     return reinterpret_cast<uintptr_t>(q) % bytes == 0 && stride * (int64_t)sizeof(T) % bytes == 0;
   };
-  const bool rows = a.D / a.G % 8 == 0 && ok(a.x, a.xs, 16) && ok(a.dt, a.ds, 16) && ok(a.out, a.os, 16) && (!a.z || ok(a.z, a.zs, 16));
-  constexpr int four = 4 * sizeof(T);
+  constexpr int part = Shape<L>::E * sizeof(T) > 16 ? 16 : Shape<L>::E * sizeof(T), four = 4 * sizeof(T);
+  const bool rows = a.D / a.G % Shape<L>::E == 0 && ok(a.x, a.xs, part) && ok(a.dt, a.ds, part) && ok(a.out, a.os, part) &&
+                    (!a.z || ok(a.z, a.zs, part));
   const bool bc = a.N % 4 == 0 && ok(a.B, a.bs_t, four) && ok(a.C, a.cs_t, four) && (a.G == 1 || (ok(a.B, a.bs_g, four) && ok(a.C, a.cs_g, four)));
-  const int vec = rows + 2 * bc;
-  constexpr int bytes = sizeof(Smem<T, L>);
-  static unsigned long long done1 = 0, done2 = 0;
-  if (!set_max_smem_per_device(scan_tiles_kernel<T, L, true>, bytes, done1) ||
-      !set_max_smem_per_device(scan_tiles_kernel<T, L, false>, bytes, done2))
-    return "selective_scan: the device has too little shared memory";
-  if (p.tiles > 1) scan_tiles_kernel<T, L, true><<<(unsigned)(blocks * (p.tiles - 1)), kThreads, bytes, st>>>(a, ta, vec);
-  scan_tiles_kernel<T, L, false><<<(unsigned)(blocks * p.tiles), kThreads, bytes, st>>>(a, ta, vec);
-  return nullptr;
+  return rows ? launch<T, L, true>(a, p, ws, bc, st) : launch<T, L, false>(a, p, ws, bc, st);
 }
 
 }  // namespace
 
 ScanPlan scan_plan(const ScanArgs& a, int sms) {
   const int L = lanes_of(a.N);
-  const int64_t per_group = a.D / a.G, ch = 512 / L;
+  const int64_t per_group = a.D / a.G, ch = L == 4 ? Shape<4>::CH : L == 8 ? Shape<8>::CH : L == 16 ? Shape<16>::CH : Shape<32>::CH;
   const int64_t blocks = (per_group + ch - 1) / ch * a.G;
-  // Blocks of a wave run at one speed per SM. A cut adds a first pass of 0.8 of the work over what crosses tiles: all of
-  // a long sequence, less of short ones.
+  // Time of one token with c blocks on the busiest SM: two at once take 1.5 times as long as one (82 against 54 ns with 16
+  // states); blocks of 256 + 256 threads have an SM to themselves and count as two. A cut adds a first pass of 0.65 of the
+  // work over what crosses tiles: all of a long sequence, less of short ones.
+  const bool pairs = L <= 16;
+  auto speed = [&](int64_t n) {
+    const int64_t c = (n + sms - 1) / sms;
+    return pairs ? c / 2 * 1.5 + c % 2 : c * 1.5;
+  };
   ScanPlan best{1, a.seq.T, 0};
-  double cost = (double)a.seq.T * ((blocks + sms - 1) / sms);
+  double cost = a.seq.T * speed(blocks);
   for (int64_t n = 2; n <= 64 && a.seq.T / n >= 64; ++n) {
     const int64_t tile = ((a.seq.T + n - 1) / n + 15) / 16 * 16;
     const int64_t tiles = (a.seq.T + tile - 1) / tile;
     if (tiles < 2) break;
     const double crossing = std::min(1.0, (double)tiles / std::max(1, a.seq.N));
-    const double c = tile * (double)((blocks * tiles + sms - 1) / sms) +
-                     0.8 * crossing * tile * (double)((blocks * (tiles - 1) + sms - 1) / sms) + 24.0 + tiles;
+    const double c = tile * speed(blocks * tiles) + 0.65 * crossing * tile * speed(blocks * (tiles - 1)) + 48.0 + tiles;
     if (c < cost) {
       cost = c;
       best = {(int)tiles, (int)tile, (int64_t)tiles * a.D * (2 * a.N + 1)};
