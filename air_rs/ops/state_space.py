@@ -104,13 +104,12 @@ def block_norm(y: torch.Tensor, weight: torch.Tensor | None, eps: float, *, resi
         raise ValueError(f"block_norm: gate_act must be one of {', '.join(GATES)}, not {gate_act!r}")
     if resid_out is None:
         resid_out = residual
-    if out is None and (weight is not None or residual is None):
-        out = torch.empty(y.shape, dtype=torch.bfloat16, device=y.device)
     row = scale if isinstance(scale, torch.Tensor) else None
-    require_ext().block_norm(y, weight, eps, residual, post_weight, gate, GATES[gate_act],
-                             1.0 if row is not None else float(scale), row, w_offset, out, resid_out)
+    made, _ = require_ext().block_norm(y, weight, eps, residual, post_weight, gate, GATES[gate_act],
+                                       1.0 if row is not None else float(scale), row, w_offset, out,
+                                       out is None and (weight is not None or residual is None), resid_out)
     count_launch()
-    return out, resid_out
+    return made if out is None else out, resid_out
 
 
 class TokenLogprobs(NamedTuple):

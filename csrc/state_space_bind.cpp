@@ -1,8 +1,6 @@
 // torch <-> kernel adapter of the state-space decoder's operators: causal convolution and selective scan (prompts and
 // single tokens), block norm, token log probabilities. Shapes, types, strides and aliasing are checked before devices,
 // so every refusal but that of a wrong device is the same for CPU tensors.
-#include <cstring>
-
 #include "bind_util.h"
 #include "state_space.h"
 
@@ -12,11 +10,16 @@ namespace {
 
 // What a call was given, for the checks that concern all operands.
 struct Operands {
+  struct Operand {
+    const Tensor* t;
+    const char* what;
+  };
   const char* op;
-  std::vector<std::pair<Tensor, const char*>> all;
+  Operand all[16];
+  int n = 0;
 
   explicit Operands(const char* name) : op(name) {}
-  void add(const Tensor& t, const char* what) { all.emplace_back(t, what); }
+  void add(const Tensor& t, const char* what) { all[n++] = {&t, what}; }
 
   // [rows, cols] bf16 or f32 with contiguous rows (`type`: the type it must have)
   void rows(const Tensor& t, const char* what, int64_t n, int64_t d, c10::optional<at::ScalarType> type = c10::nullopt) {
@@ -30,13 +33,15 @@ struct Operands {
     TORCH_CHECK(type.has_value() ? is == *type : is == at::kBFloat16 || is == at::kFloat, op, ": ", what, " must be ",
                 type.has_value() ? toString(*type) : "BFloat16 or Float");
   }
-  const float* floats(const optional<Tensor>& t, const char* what, at::IntArrayRef shape) {
-    if (!t.has_value()) return nullptr;
-    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->sizes() == shape, op, ": ", what,
+  const float* floats(const Tensor& t, const char* what, at::IntArrayRef shape) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() && t.sizes() == shape, op, ": ", what,
                 " must be contiguous float32 of ", str(shape[0]), shape.size() > 1 ? " x " + str(shape[1]) : std::string(),
                 " values");
-    add(*t, what);
-    return t->data_ptr<float>();
+    add(t, what);
+    return t.data_ptr<float>();
+  }
+  const float* floats(const optional<Tensor>& t, const char* what, at::IntArrayRef shape) {
+    return t.has_value() ? floats(*t, what, shape) : nullptr;
   }
   const int* ints(const optional<Tensor>& t, const char* what, int64_t n) {
     if (!t.has_value()) return nullptr;
@@ -72,18 +77,18 @@ struct Operands {
     return off < wa || off + wb > ra;          // b's columns start inside a's, or reach a's next row
   }
   // `t` is written: nothing else may lie in it, but for `same`, which may be the same memory element by element.
-  void written(const Tensor& t, const char* what, const Tensor* same = nullptr) {
-    for (const auto& o : all) {
-      if (!std::strcmp(o.second, what)) continue;
-      if (same && o.first.data_ptr() == same->data_ptr() && o.first.is_same(*same) && t.data_ptr() == same->data_ptr() &&
-          t.strides() == same->strides() && t.scalar_type() == same->scalar_type()) continue;
-      TORCH_CHECK(!meet(t, o.first), op, ": ", what, " shares memory with ", o.second);
+  void written(const Tensor& t, const char* what, const Tensor* same = nullptr) const {
+    for (int i = 0; i < n; ++i) {
+      const Tensor& o = *all[i].t;
+      if (&o == &t) continue;
+      if (same && &o == same && t.data_ptr() == o.data_ptr() && t.strides() == o.strides() && t.scalar_type() == o.scalar_type()) continue;
+      TORCH_CHECK(!meet(t, o), op, ": ", what, " shares memory with ", all[i].what);
     }
   }
-  void on_device() {
-    TORCH_CHECK(all[0].first.is_cuda(), op, ": ", all[0].second, " must be a CUDA tensor");
-    for (const auto& o : all) TORCH_CHECK(o.first.device() == all[0].first.device(), op, ": ", o.second,
-                                          " must be on the device of ", all[0].second);
+  void on_device() const {
+    TORCH_CHECK(all[0].t->is_cuda(), op, ": ", all[0].what, " must be a CUDA tensor");
+    const auto device = all[0].t->device();
+    for (int i = 1; i < n; ++i) TORCH_CHECK(all[i].t->device() == device, op, ": ", all[i].what, " must be on the device of ", all[0].what);
   }
 };
 
@@ -265,9 +270,11 @@ Tensor selective_scan_step(Tensor x, Tensor dt, Tensor A, Tensor B, Tensor C, Te
   return scan("selective_scan_step", x, dt, A, B, C, skip, z, dt_bias, softplus, state, c10::nullopt, slots, c10::nullopt, out, err, 1);
 }
 
-// act: 0 SiLU, 1 sigmoid, 2 the gate itself. Writes out and resid_out where given.
-void block_norm(Tensor y, optional<Tensor> w, double eps, optional<Tensor> resid, optional<Tensor> post_w, optional<Tensor> gate,
-                int64_t act, double scale, optional<Tensor> scale_row, double w_offset, optional<Tensor> out, optional<Tensor> resid_out) {
+// act: 0 SiLU, 1 sigmoid, 2 the gate itself. `new_out`: out is made here, in bf16.
+std::tuple<optional<Tensor>, optional<Tensor>> block_norm(Tensor y, optional<Tensor> w, double eps, optional<Tensor> resid,
+                                                          optional<Tensor> post_w, optional<Tensor> gate, int64_t act, double scale,
+                                                          optional<Tensor> scale_row, double w_offset, optional<Tensor> out,
+                                                          bool new_out, optional<Tensor> resid_out) {
   const char* op = "block_norm";
   TORCH_CHECK(y.dim() == 2, op, ": y must be [tokens, dim]");
   const int64_t T = y.size(0), K = y.size(1);
@@ -312,6 +319,7 @@ void block_norm(Tensor y, optional<Tensor> w, double eps, optional<Tensor> resid
     a.r_bf16 = resid_out->scalar_type() == at::kBFloat16;
     four(*resid_out);
   }
+  if (new_out) out = at::empty({T, K}, y.options().dtype(at::kBFloat16));
   if (out.has_value()) {
     c.rows(*out, "out", T, K);
     distinct_rows(*out, op, "out");
@@ -336,6 +344,7 @@ void block_norm(Tensor y, optional<Tensor> w, double eps, optional<Tensor> resid
   const char* e = air::launch_block_norm(a, vec, at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(e == nullptr, e ? e : "");
   post(op);
+  return {out, resid_out};
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(Tensor logits, optional<Tensor> tokens, int64_t k, Tensor err) {
