@@ -51,7 +51,7 @@ struct ScanPlan {
   int tiles, tile;
   int64_t floats;
 };
-bool scan_tiles_supported(const ScanArgs& a);
+bool scan_tiles_worth(const ScanArgs& a);       // against launch_scan_tokens, by size
 ScanPlan scan_plan(const ScanArgs& a, int sms);
 const char* launch_scan_tiles(const ScanArgs& a, const ScanPlan& p, float* ws, bool f32, cudaStream_t st);
 

@@ -246,7 +246,7 @@ Tensor scan(const char* op, const Tensor& x, const Tensor& dt, const Tensor& A, 
   TORCH_CHECK(a.seq.N <= (1ll << 31) / (D / 4 + 1), op, ": too many sequences");
   const bool f32 = type == at::kFloat;
   auto st = at::cuda::getCurrentCUDAStream();
-  if (!step && air::scan_tiles_supported(a)) {
+  if (!step && air::scan_tiles_worth(a)) {
     const air::ScanPlan p = air::scan_plan(a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
     Tensor ws;                                     // from the allocator's pool of this stream
     if (p.floats) ws = at::empty({p.floats}, x.options().dtype(at::kFloat));
