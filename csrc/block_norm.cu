@@ -148,7 +148,14 @@ __global__ void __launch_bounds__(NT) block_norm_rows_kernel(const BlockNormArgs
   for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, b ^= 1) {
     fetch(t + gridDim.x, b ^ 1);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
-    float h[J][E];
+    float h[J][E], w[J][E];
+    auto load_weights = [&](const float* p, float (&f)[J][E]) {      // asked for before the reduction they wait for
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int i = E * (threadIdx.x + NT * j);
+        if (i < a.K) load_v<float, E>(p + i, f[j]);
+      }
+    };
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       if (E * (threadIdx.x + NT * j) < a.K) load_v<TY, E>(ys(b, 0)[j][threadIdx.x], h[j]);
@@ -160,16 +167,12 @@ __global__ void __launch_bounds__(NT) block_norm_rows_kernel(const BlockNormArgs
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int e = 0; e < E; ++e) ss = fmaf(h[j][e], h[j][e], ss);
+      load_weights(a.post, w);
       const float inv = sum.inv_rms(ss, a);
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int i = E * (threadIdx.x + NT * j);
-        if (i >= a.K) continue;
-        float w[E];
-        load_v<float, E>(a.post + i, w);
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e) h[j][e] *= inv * (w[e] + a.w_offset);
-      }
+        for (int e = 0; e < E; ++e) h[j][e] *= inv * (w[j][e] + a.w_offset);
     }
     float ss = 0.f;
 #pragma unroll
@@ -193,15 +196,15 @@ __global__ void __launch_bounds__(NT) block_norm_rows_kernel(const BlockNormArgs
       if (a.resid_out) store_v<TR, E>(static_cast<TR*>(a.resid_out) + t * a.ldro + i, h[j]);
     }
     if (!a.out) continue;
+    if (a.w) load_weights(a.w, w);
     const float inv = a.w ? sum.inv_rms(ss, a) : 1.f;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int i = E * (threadIdx.x + NT * j);
       if (i >= a.K) continue;
       float o[E];
-      if (a.w) load_v<float, E>(a.w + i, o);
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = a.w ? h[j][e] * inv * (o[e] + a.w_offset) : h[j][e];
+      for (int e = 0; e < E; ++e) o[e] = a.w ? h[j][e] * inv * (w[j][e] + a.w_offset) : h[j][e];
       if (a.o_bf16) store_v<__nv_bfloat16, E>(static_cast<__nv_bfloat16*>(a.out) + t * a.ldo + i, o);
       else store_v<float, E>(static_cast<float*>(a.out) + t * a.ldo + i, o);
     }
