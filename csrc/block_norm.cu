@@ -24,9 +24,8 @@ struct RowSum {
     if constexpr (NT > 32) {
       if ((threadIdx.x & 31) == 0) red[place][threadIdx.x >> 5] = v;
       __syncthreads();
-      v = 0.f;
-#pragma unroll
-      for (int w = 0; w < NT / 32; ++w) v += red[place][w];
+      const int lane = threadIdx.x & 31;
+      v = warp_sum(lane < NT / 32 ? red[place][lane] : 0.f);
       place ^= 1;
     }
     return v;
@@ -245,10 +244,10 @@ void launch(const BlockNormArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-const char* launch_block_norm(const BlockNormArgs& a, bool vec, cudaStream_t st) {
+const char* launch_block_norm(const BlockNormArgs& a, int vec, cudaStream_t st) {
   if (a.T <= 0) return nullptr;
   if (a.K < 1 || a.K > kBlockNormMaxK) return "block_norm: 1 to 32768 columns";
-#define AIR_BN_E(TY, TR) (vec ? launch<TY, TR, 4>(a, st) : launch<TY, TR, 1>(a, st))
+#define AIR_BN_E(TY, TR) (vec == 4 ? launch<TY, TR, 4>(a, st) : vec == 2 ? launch<TY, TR, 2>(a, st) : launch<TY, TR, 1>(a, st))
   if (a.y_bf16 && a.r_bf16) AIR_BN_E(__nv_bfloat16, __nv_bfloat16);
   else if (a.y_bf16) AIR_BN_E(__nv_bfloat16, float);
   else if (a.r_bf16) AIR_BN_E(float, __nv_bfloat16);

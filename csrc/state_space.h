@@ -70,7 +70,8 @@ struct BlockNormArgs {
   int act;                 // of the gate: 0 SiLU, 1 sigmoid, 2 none
 };
 constexpr int kBlockNormMaxK = 32768;
-const char* launch_block_norm(const BlockNormArgs& a, bool vec, cudaStream_t st);
+// vec = 4, 2 or 1 divides K and all rows are aligned to vec elements.
+const char* launch_block_norm(const BlockNormArgs& a, int vec, cudaStream_t st);
 
 struct TokenLogprobArgs {
   const void* logits;      // [T, V] bf16 or f32

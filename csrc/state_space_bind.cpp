@@ -286,8 +286,10 @@ std::tuple<optional<Tensor>, optional<Tensor>> block_norm(Tensor y, optional<Ten
   a.w = c.floats(w, "weight", {K});
   a.post = c.floats(post_w, "post_weight", {K});
   a.scale_row = c.floats(scale_row, "scale", {K});
-  bool vec = K % 4 == 0;
-  auto four = [&](const Tensor& t) { vec = vec && aligned(t, 4 * t.element_size()); };
+  int vec = 4;
+  auto four = [&](const Tensor& t) {
+    while (vec > 1 && (K % vec || !aligned(t, vec * t.element_size()))) vec /= 2;
+  };
   for (const auto* t : {&w, &post_w, &scale_row})
     if (t->has_value()) four(**t);
   four(y);

@@ -98,17 +98,18 @@ def test_conv_matches_the_sum(case, dtype, silu):
     init = torch.where((has.bool() & (slots >= 0))[:, None, None], pool[slots.long().clamp(min=0)], torch.zeros((), dtype=dtype))
     ref, tol, ends = _conv_ref(x[:, D:], w, bias, lens, init, silu)
     cu = _i32([0] + torch.tensor(lens).cumsum(0).tolist())
-    st = pool.cuda()
-    out = torch.full((T + 1, D + 3), 7.0, dtype=dtype, device="cuda")
-    ops.causal_conv(x.cuda()[:, D:], w.cuda(), None if bias is None else bias.cuda(), state=st, cu_seqlens=cu,
-                    slots=slots.cuda(), has_state=has.cuda(), silu=silu, out=out[:T, :D])
-    _held(out[:T, :D], ref, tol, dtype == torch.bfloat16)
-    assert bool((out[T:] == 7).all()) and bool((out[:, D:] == 7).all())
     want = pool.clone()
     for n in range(N):
         if slots[n] >= 0:
             want[slots[n]] = ends[n]
-    assert torch.equal(st.cpu(), want)
+    for pad in (3, 16, 2):                           # rows at odd places, whole 16-byte parts, and pairs
+        st = pool.cuda()
+        out = torch.full((T + 1, D + pad), 7.0, dtype=dtype, device="cuda")
+        ops.causal_conv(x.cuda()[:, D:], w.cuda(), None if bias is None else bias.cuda(), state=st, cu_seqlens=cu,
+                        slots=slots.cuda(), has_state=has.cuda(), silu=silu, out=out[:T, :D])
+        _held(out[:T, :D], ref, tol, dtype == torch.bfloat16)
+        assert bool((out[T:] == 7).all()) and bool((out[:, D:] == 7).all())
+        assert torch.equal(st.cpu(), want)
     ops.check_errors()
 
 
@@ -179,6 +180,9 @@ SCANS = [  # lens, channels, states, groups
     ([70], 96, 1, 1),
     ([3, 50], 65, 24, 1),
     ([700], 32, 8, 1),
+    ([1, 2, 1, 0, 3, 1, 1, 4, 2, 1] * 3, 40, 16, 1),
+    ([90, 300, 7, 200], 64, 16, 1),
+    ([260, 40], 48, 32, 2),
 ]
 
 
@@ -215,19 +219,20 @@ def test_scan_matches_the_recurrence(case, dtype, softplus):
         slots[2] = -1
     init = torch.where((has.bool() & (slots >= 0))[:, None, None], pool[slots.long().clamp(min=0)], torch.zeros(()))
     ref, tol, ends, etol = _scan_ref(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["bias"], softplus, lens, init)
-    st, out = pool.cuda(), torch.full((T + 1, d + 1), 7.0, dtype=dtype, device="cuda")
     b = i["B"][:, 0] if groups == 1 else i["B"]
-    ops.selective_scan(i["x"].cuda(), i["dt"].cuda(), i["A"].cuda(), b.cuda(), i["C"].cuda(), D=_dev(i["D"]), z=_dev(i["z"]),
-                       dt_bias=_dev(i["bias"]), softplus=softplus, state=st, slots=slots.cuda(), has_state=has.cuda(),
-                       cu_seqlens=_i32([0] + torch.tensor(lens).cumsum(0).tolist()), out=out[:T, :d])
-    _held(out[:T, :d], ref, tol, dtype == torch.bfloat16)
-    assert bool((out[T:] == 7).all()) and bool((out[:, d:] == 7).all())
-    st = st.cpu()
-    for k in range(N):
-        if slots[k] >= 0:
-            _held(st[slots[k]], ends[k], etol[k], False)
     free = [s for s in range(N + 2) if s not in slots.tolist()]
-    assert torch.equal(st[free], pool[free])
+    for pad in (1, 16):                              # rows at odd places, and whole 16-byte parts where d allows them
+        st, out = pool.cuda(), torch.full((T + 1, d + pad), 7.0, dtype=dtype, device="cuda")
+        ops.selective_scan(i["x"].cuda(), i["dt"].cuda(), i["A"].cuda(), b.cuda(), i["C"].cuda(), D=_dev(i["D"]), z=_dev(i["z"]),
+                           dt_bias=_dev(i["bias"]), softplus=softplus, state=st, slots=slots.cuda(), has_state=has.cuda(),
+                           cu_seqlens=_i32([0] + torch.tensor(lens).cumsum(0).tolist()), out=out[:T, :d])
+        _held(out[:T, :d], ref, tol, dtype == torch.bfloat16)
+        assert bool((out[T:] == 7).all()) and bool((out[:, d:] == 7).all())
+        st = st.cpu()
+        for k in range(N):
+            if slots[k] >= 0:
+                _held(st[slots[k]], ends[k], etol[k], False)
+        assert torch.equal(st[free], pool[free])
     ops.check_errors()
 
 
@@ -438,6 +443,12 @@ NORMS = [  # T, K, residual, post, gate, act, scale, offset, weight
     (6, 1, torch.float32, True, "rows", "silu", 1.0, 0.0, True),
     (3000, 264, torch.float32, False, "", "silu", 1.0, 0.0, True),
     (2, 6000, torch.float32, False, "", "silu", 1.0, 0.0, False),
+    (7, 2050, torch.bfloat16, True, "rows", "silu", 0.5, 1.0, True),
+    (500, 3000, torch.float32, True, "rows", "silu", "row", 1.0, True),      # more rows than blocks
+    (160, 8192, torch.bfloat16, True, "row", "sigmoid", 0.22, 0.0, True),
+    (5000, 96, torch.float32, True, "rows", "none", 1.0, 1.0, True),
+    (2500, 1000, torch.float32, False, "row", "silu", 1.0, 0.0, True),
+    (1300, 2044, torch.float32, True, "", "silu", 0.5, 0.0, False),
 ]
 
 
@@ -465,10 +476,12 @@ def test_block_norm(case, dtype):
         _held(res, rr, rtol, rt == torch.bfloat16)
         # into another buffer: the residual stays
         keep, other = _dev(resid), torch.empty(T, K, dtype=rt, device="cuda")
-        ops.block_norm(y.cuda(), _dev(w), 1e-5, residual=keep, post_weight=_dev(p), gate=_dev(gt), gate_act=act,
-                       scale=_dev(sc) if scale == "row" else scale, w_offset=off, resid_out=other)
+        out, _ = ops.block_norm(y.cuda(), _dev(w), 1e-5, residual=keep, post_weight=_dev(p), gate=_dev(gt), gate_act=act,
+                                scale=_dev(sc) if scale == "row" else scale, w_offset=off, resid_out=other)
         assert torch.equal(keep.cpu(), resid)
         _held(other, rr, rtol, rt == torch.bfloat16)
+        if weight:
+            _held(out, ref, tol, True)
 
 
 @gpu
