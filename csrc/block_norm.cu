@@ -1,10 +1,11 @@
 // The way from a block's output to the next block's input in one pass:
 //   h = y;  h = h rsqrt(mean(h^2) + eps) (post + w_offset);  h = h act(gate);
 //   r = resid + scale h;  out = r rsqrt(mean(r^2) + eps) (w + w_offset)
-// each step but the sum optional. One CTA per row with the row in registers, so y, gate and the residual are read once,
-// r and out written once and nothing else goes to memory. All steps are f32 on the unrounded values of the step before;
-// out and (in bf16) the stored residual are rounded once. Memory-bound with many rows, the latency of one or two block
-// reductions with one.
+// each step but the sum optional. A block has a row in registers, so y, gate and the residual are read once, r and out
+// written once and nothing else goes to memory. All steps are f32 on the unrounded values of the step before; out and (in
+// bf16) the stored residual are rounded once. Memory-bound with many rows: 6007 x 4096 with bf16 y and gate, f32 residual
+// and both norms takes 59 us (5.8 TB/s, floor 52.6), f32 y 69 (floor 67.6), 4094 columns 87 and 4095 135 (pairs and
+// single elements); one row 2.9 us, the latency of the loads and one or two block reductions.
 #include <algorithm>
 
 #include "state_space.cuh"
@@ -224,8 +225,8 @@ bool launch_rows(const BlockNormArgs& a, cudaStream_t st) {
 
 template <typename TY, typename TR, int E>
 void launch(const BlockNormArgs& a, cudaStream_t st) {
-  // Many rows: at 6007 x 4096 (bf16, gate, both norms; floor 52.6 us) 256 threads take 68 us, 512 82 (f32: 89 and 76), a
-  // row a block without the copies ahead 71; at 3000 x 8192 1024 threads 77, 512 89.
+  // Many rows: at 6007 x 4096 (bf16, gate, both norms) 256 threads take 59 us, 512 70 and a row a block without the copies
+  // ahead 71; at 3000 x 8192 (floor 52.5) 1024 threads 71, 512 76.
   if constexpr (E == 4) {
     if (a.K <= 512 ? launch_rows<TY, TR, 32, 4>(a, st) : a.K <= 1024 ? launch_rows<TY, TR, 64, 4>(a, st) :
         a.K <= 2048 ? launch_rows<TY, TR, 128, 4>(a, st) : a.K > 4096 ? a.K <= 8192 && launch_rows<TY, TR, 1024, 2>(a, st) :

@@ -12,9 +12,10 @@ namespace {
 
 constexpr int kTokThreads = 128;
 
-// One token after the other, for single tokens and any shape: L lanes share a channel, S states each (the states of a
-// lane are consecutive, so the lanes of a channel read its whole row of the pool). A warp works on 32 / L channels.
-// Single tokens are bound by the pool: 8 bytes a state against a dozen instructions.
+// One token after the other, for any shape: more than 64 states, calls of short sequences, single tokens whose rows are not
+// aligned. L lanes share a channel, S states each (the states of a lane are consecutive, so the lanes of a channel read its
+// whole row of the pool). A warp works on 32 / L channels. Latency-bound: 0.8 us a token with 16 states, 1.3
+// with 128, which the tiles avoid.
 template <typename T, int L, int S>
 __global__ void __launch_bounds__(kTokThreads) scan_tokens_kernel(const ScanArgs a, int blocks_d) {
   const int n = blockIdx.x / blocks_d;
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kTokThreads) scan_tokens_kernel(const ScanArgs
 }
 
 // Single tokens, `rows` of them a thread with A and the channel's parameters kept; the states of a lane are whole accesses
-// (N a multiple of 4 or 8, aligned rows). 128 x 8192 with 16 states takes 34 us at a floor of 21.9: instructions, of
+// (N a multiple of 4 or 8, aligned rows). 128 x 8192 with 16 states takes 34.5 us at a floor of 21.9: instructions, of
 // which the work of a channel (step, gate, addresses) is shared by eight states a lane (four: 46 us). Up to four rows a
 // thread (one: 57 us with four states a lane); two rows in flight cost more registers than they gain (44 us).
 template <typename T, int L, int S>

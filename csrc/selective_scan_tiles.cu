@@ -1,22 +1,26 @@
 // Selective scan of packed prompts in tiles of tokens.
 //   h = exp(delta A) h + delta x B,   y = (C . h + D x) silu(z)
 //
-// What bounds it: one exponential per token, channel and state. At 16 states an element of x costs 16 exponentials (a
-// quarter of a warp's clock each per scheduler and 4 lanes: 4 clocks) against 8 bytes of bf16 rows, so the special-function
-// and instruction pipes, not memory. The recurrence itself is one chain of multiply-adds a state: independent chains in a thread keep
-// the pipes busy, not occupancy.
+// What bounds it: one exponential per token, channel and state (a warp's exponential takes 8 clocks of its scheduler, a
+// paired multiply-add 2, both measured), against 8 bytes a token and channel: 64 channels of a token with 16 states are 33 ns
+// of an SM's exponentials and 12 ns of its share of the memory bandwidth. So the special-function, multiply-add and issue
+// slots are what counts: 8192 x 8192 x 16 bf16 takes 660 us where the exponentials alone would take 231 and the
+// bytes 82; issue slots are busy 58 % on average (67 % on the 108 SMs that have two blocks, 40 have one), the
+// multiply-add pipe 53 %.
 //
-// A block has eight scan warps and eight helper warps. L lanes share a pair of channels, each with two states of both: the
-// arithmetic runs on pairs of channels (f32x2), so the steps of a pair are one operand and B and C, stored twice, another,
-// and y of the pair comes out as one. Stage by stage of TS tokens, through two sets of buffers, the helpers turn dt and x of the
+// A block has as many scan warps as helper warps, four of each (two blocks an SM). L lanes share a pair of channels, each
+// with two states of both: the arithmetic runs on pairs of channels (f32x2), so the steps of a pair are one operand and y
+// of the pair comes out as one. Stage by stage of TS tokens, through two sets of buffers, the helpers turn dt and x of the
 // next stages into delta and delta x, and the lanes' parts of y of the last one into the output (sum, skip, gate,
-// rounding), so all global accesses are theirs: whole rows, copied asynchronously six stages ahead.
+// rounding), so all global accesses are theirs, copied asynchronously up to three stages ahead. Before the helpers, with each
+// scan warp loading its own rows, the case above took 11.9 ms; with the helpers' loads through registers 1.45.
 //
 // The tokens of all sequences lie in one row of tiles of equal length; a block walks through its tile and loads or
 // stores a state where a sequence starts or ends, so ragged batches are balanced. With few channels there are several
 // tiles: a first pass then computes what each tile's last sequence adds to the next tile (the state from zero, or from the
 // sequence's initial state, and the sum of delta), and the second pass starts from exp(A sum) times those of the tiles before.
-// That pass doubles the exponentials of sequences that cross tiles, so the host cuts no more than fills the SMs.
+// That pass adds 0.65 of the work over sequences that cross tiles, so the host cuts no more than pays (scan_plan).
+// Up to 64 states; more go token by token (selective_scan.cu).
 #include <algorithm>
 
 #include "state_space.cuh"
@@ -25,12 +29,6 @@ namespace air {
 
 namespace {
 
-#ifndef LB
-#define LB 1
-#endif
-#ifndef KG
-#define KG 4
-#endif
 // p = e - 1 where |u| is past the polynomial's interval
 AIR_DEVICE void far_decay(float& p, float u, float e) {
   asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %1;\n\tsetp.gt.f32 q, a, %2;\n\t@q add.f32 %0, %3, 0fBF800000;\n\t}"

@@ -9,7 +9,11 @@
 //
 // The alternatives need no second pass over the row: the k-th largest of the threads' maxima is at most the k-th largest
 // logit, so only the k threads whose maximum reaches it can hold one. Their elements (k / threads of the row, from L2) are
-// read again by the whole block, the few that reach the bound are collected and ordered. Memory-bound.
+// read again by the whole block, the few that reach the bound are collected and ordered. A row with fewer than k logits
+// above -1e29 is swept once more, for finite ones below.
+//
+// Memory-bound with many long rows: 2048 x 128256 bf16 takes 101 us without alternatives (5.2 TB/s, floor 80), 110 with one,
+// 131 with five where every 16th row has three tokens left and is swept twice. One row of f32 takes 6.1 us without and 10.4 with 20.
 #include <cooperative_groups.h>
 
 #include "state_space.cuh"
