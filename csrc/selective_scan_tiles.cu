@@ -205,13 +205,26 @@ struct Helper {
       }
     }
   }
-  // E elements of a fetched row; what is not there is zero
+  // E elements of a fetched row. Channels past the group's last one get whatever shares their words: nothing of theirs is kept.
   AIR_DEVICE void read(int slot, int which, float* f) const {
     const T* p = sm.rows[slot][which][tid];
-    if constexpr (VEC) load_v<T, E>(p, f);
+    if constexpr (VEC || sizeof(T) == 4) load_v<T, E>(p, f);
     else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+      uint32_t v[E / 2 + 1];
+      if constexpr (E == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(w);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(w);
+        v[0] = u.x; v[1] = u.y;
+      }
 #pragma unroll
-      for (int i = 0; i < E; ++i) f[i] = i < live ? to_f(p[odd[which] + i]) : 0.f;
+      for (int i = 0; i < E / 2; ++i) {
+        const uint32_t two = __funnelshift_r(v[i], v[i + 1], odd[which] * 16);
+        f[2 * i] = __uint_as_float(two << 16);
+        f[2 * i + 1] = __uint_as_float(two & 0xffff0000u);
+      }
     }
   }
   // The next stage's rows, complete for this helper after arrived() with kAhead - 1 stages fetched after it
@@ -289,7 +302,18 @@ struct Helper {
       unpack2(sum, y[i], y[i + 1]);
     }
     if constexpr (VEC) store_v<T, E>(o, y);
-    else {
+    else if (sizeof(T) == 2 && live == E) {              // in words as far as they are the row's own
+      const bool at_odd = reinterpret_cast<uintptr_t>(o) >> 1 & 1;
+      if (!at_odd) {
+#pragma unroll
+        for (int i = 0; i < E; i += 2) store_v<T, 2>(o + i, y + i);
+      } else {
+        o[0] = from_f<T>(y[0]);
+#pragma unroll
+        for (int i = 1; i + 1 < E; i += 2) store_v<T, 2>(o + i, y + i);
+        o[E - 1] = from_f<T>(y[E - 1]);
+      }
+    } else {
 #pragma unroll
       for (int i = 0; i < E; ++i)
         if (i < live) o[i] = from_f<T>(y[i]);
