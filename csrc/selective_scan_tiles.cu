@@ -174,9 +174,9 @@ struct Helper {
     dt = static_cast<const T*>(a.dt) + (int64_t)tf * a.ds + d;
     z = a.z ? static_cast<const T*>(a.z) + (int64_t)tf * a.zs + d : nullptr;
     out = static_cast<T*>(a.out) + (int64_t)tf * a.os + d;
-    const T* rows[3] = {x, dt, z};
-#pragma unroll
-    for (int i = 0; i < 3; ++i) odd[i] = VEC || sizeof(T) == 4 ? 0 : reinterpret_cast<uintptr_t>(rows[i]) >> 1 & 1;
+    odd[0] = odd_half(x);
+    odd[1] = odd_half(dt);
+    odd[2] = odd_half(z);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       bias[i] = a.dt_bias && i < live ? a.dt_bias[d + i] : 0.f;
@@ -195,37 +195,12 @@ struct Helper {
   AIR_DEVICE void row(int which, const T* p, const void* any, bool in) {
     T* dst = sm.rows[ring][which][tid];
     if constexpr (VEC) copy_async<E * (int)sizeof(T)>(dst, in ? p : any, in);
-    else {
-      // word by word: those that hold one of the row's elements, so nothing past the row's own words is read
-      constexpr int per = 4 / sizeof(T);
-#pragma unroll
-      for (int j = 0; j < E / per + per - 1; ++j) {
-        const bool some = in && j * per - odd[which] < live;
-        copy_async<4>(dst + j * per, some ? p - odd[which] + j * per : any, some);
-      }
-    }
+    else copy_words<T, E>(dst, p, any, odd[which], in ? live : -8);
   }
   // E elements of a fetched row. Channels past the group's last one get whatever shares their words: nothing of theirs is kept.
   AIR_DEVICE void read(int slot, int which, float* f) const {
-    const T* p = sm.rows[slot][which][tid];
-    if constexpr (VEC || sizeof(T) == 4) load_v<T, E>(p, f);
-    else {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
-      uint32_t v[E / 2 + 1];
-      if constexpr (E == 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(w);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z;
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(w);
-        v[0] = u.x; v[1] = u.y;
-      }
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const uint32_t two = __funnelshift_r(v[i], v[i + 1], odd[which] * 16);
-        f[2 * i] = __uint_as_float(two << 16);
-        f[2 * i + 1] = __uint_as_float(two & 0xffff0000u);
-      }
-    }
+    if constexpr (VEC) load_v<T, E>(sm.rows[slot][which][tid], f);
+    else read_words<T, E>(sm.rows[slot][which][tid], odd[which], f);
   }
   // The next stage's rows, complete for this helper after arrived() with kAhead - 1 stages fetched after it
   AIR_DEVICE void fetch() {
@@ -302,22 +277,7 @@ struct Helper {
       unpack2(sum, y[i], y[i + 1]);
     }
     if constexpr (VEC) store_v<T, E>(o, y);
-    else if (sizeof(T) == 2 && live == E) {              // in words as far as they are the row's own
-      const bool at_odd = reinterpret_cast<uintptr_t>(o) >> 1 & 1;
-      if (!at_odd) {
-#pragma unroll
-        for (int i = 0; i < E; i += 2) store_v<T, 2>(o + i, y + i);
-      } else {
-        o[0] = from_f<T>(y[0]);
-#pragma unroll
-        for (int i = 1; i + 1 < E; i += 2) store_v<T, 2>(o + i, y + i);
-        o[E - 1] = from_f<T>(y[E - 1]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (i < live) o[i] = from_f<T>(y[i]);
-    }
+    else store_words<T, E>(o, y, live);
   }
 };
 

@@ -105,6 +105,62 @@ AIR_DEVICE void copy_async(void* dst, const void* src, bool in) {
   }
 }
 
+// ---- E elements (2 or 4) of a row that starts anywhere, as the 4-byte words that hold them. bf16 at an odd place takes a
+// word more, of which half belongs to a neighbour: read, never written. `odd`: the first element's half of its word.
+template <typename T>
+AIR_DEVICE int odd_half(const T* p) { return sizeof(T) == 4 ? 0 : reinterpret_cast<uintptr_t>(p) >> 1 & 1; }
+// Asynchronously to dst (E + 2 elements of bf16, E of f32), for the first `live` elements; `any` is readable, zeros where
+// there is nothing to read.
+template <typename T, int E>
+AIR_DEVICE void copy_words(T* dst, const T* p, const void* any, int odd, int live) {
+  constexpr int per = 4 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < E / per + per - 1; ++j) {
+    const bool some = j * per - odd < live;
+    copy_async<4>(dst + j * per, some ? static_cast<const void*>(p - odd + j * per) : any, some);
+  }
+}
+// What copy_words put at p (aligned to 2 E elements of bf16, E of f32). Past `live` it may be a neighbour's.
+template <typename T, int E>
+AIR_DEVICE void read_words(const T* p, int odd, float* f) {
+  if constexpr (sizeof(T) == 4) load_v<T, E>(p, f);
+  else {
+    uint32_t v[E / 2 + 1];
+    if constexpr (E == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      v[0] = u.x; v[1] = u.y; v[2] = u.z;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      v[0] = u.x; v[1] = u.y;
+    }
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const uint32_t two = __funnelshift_r(v[i], v[i + 1], odd * 16);
+      f[2 * i] = __uint_as_float(two << 16);
+      f[2 * i + 1] = __uint_as_float(two & 0xffff0000u);
+    }
+  }
+}
+// The first `live` of E values to a row that starts anywhere, in words as far as they are its own.
+template <typename T, int E>
+AIR_DEVICE void store_words(T* o, const float* y, int live) {
+  if (sizeof(T) == 2 && live == E) {
+    if (!odd_half(o)) {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) store_v<T, 2>(o + i, y + i);
+    } else {
+      o[0] = from_f<T>(y[0]);
+#pragma unroll
+      for (int i = 1; i + 1 < E; i += 2) store_v<T, 2>(o + i, y + i);
+      o[E - 1] = from_f<T>(y[E - 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < live) o[i] = from_f<T>(y[i]);
+  }
+}
+
 // 1 / (1 + exp(-x)) and x / (1 + exp(-x)). Subnormals count as zero in the exponential and the reciprocal: without that
 // each of them costs three to four instructions more, for values below 2^-126.
 AIR_DEVICE float rcp_fast(float x) {
