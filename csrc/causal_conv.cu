@@ -52,7 +52,7 @@ struct Taps {
   Chan<V> w[W], b;
   AIR_DEVICE Taps(const ConvArgs& a, int d) {
     float flat[V * W], bias[V];
-    if constexpr (V * W % 4 == 0) load_v<float, V * W>(a.w + (int64_t)d * W, flat);
+    if constexpr (V > 1 && V * W % 4 == 0) load_v<float, V * W>(a.w + (int64_t)d * W, flat);
     else {
 #pragma unroll
       for (int i = 0; i < V * W; ++i) flat[i] = a.w[(int64_t)d * W + i];

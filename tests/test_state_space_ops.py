@@ -385,6 +385,51 @@ def test_other_streams_graphs_and_two_calls_at_once():
         assert all(torch.equal(p, q) for p, q in zip(o, want)) and all(torch.equal(p, q) for p, q in zip(s, s0))
 
 
+def _shifted(t):
+    """The same values one element further into a buffer: aligned to single elements only."""
+    b = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+    b[1:] = t.reshape(-1)
+    return b[1:].view(t.shape)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,d,n,W", [(40, 32, 16, 4), (90, 64, 8, 2), (7, 24, 64, 3)])
+def test_operands_at_odd_addresses(dtype, T, d, n, W):
+    i = _scan_inputs(T, T, d, n, 1, dtype)
+    i["z"] = i["z"].contiguous()
+    w, b = torch.randn(d, W, generator=_gen(1)), torch.randn(d, generator=_gen(2))
+    zeros = torch.zeros(1, W - 1, d, dtype=dtype)
+    ref, tol, ends = _conv_ref(i["x"], w, b, [T], zeros, True)
+    sref, stol, sends, setol = _scan_ref(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["bias"], True, [T], torch.zeros(1, d, n))
+    c = {k: _shifted(v.cuda()) for k, v in i.items()}
+    cs, ss = _shifted(zeros.cuda()), _shifted(torch.zeros(1, d, n, device="cuda"))
+    out = ops.causal_conv(c["x"], _shifted(w.cuda()), _shifted(b.cuda()), state=cs)
+    _held(out, ref, tol, dtype == torch.bfloat16)
+    assert torch.equal(cs.cpu(), ends)
+    kw = dict(D=c["D"], z=c["z"], dt_bias=c["bias"])
+    out = ops.selective_scan(c["x"], c["dt"], c["A"], c["B"][:, 0], c["C"], state=ss, **kw)
+    _held(out, sref, stol, dtype == torch.bfloat16)
+    _held(ss[0], sends[0], setol[0], False)
+    # the same tokens one by one
+    cs.zero_()
+    ss.zero_()
+    rows = lambda t, k: _shifted(c[k][t:t + 1])
+    for t in range(T):
+        o = ops.causal_conv_step(rows(t, "x"), _shifted(w.cuda()), cs, _shifted(b.cuda()))
+        _held(o, ref[t:t + 1], tol[t:t + 1], dtype == torch.bfloat16)
+        kw = dict(D=c["D"], z=rows(t, "z"), dt_bias=c["bias"])
+        o = ops.selective_scan_step(rows(t, "x"), rows(t, "dt"), c["A"], rows(t, "B"), rows(t, "C"), ss, **kw)
+        _held(o, sref[t:t + 1], stol[t:t + 1], dtype == torch.bfloat16)
+    _held(ss[0], sends[0], setol[0], False)
+    y, wt = c["x"], _shifted(b.cuda())
+    ref, tol, rr, rtol = _norm_ref(i["x"], b, 1e-5, i["z"].float(), b, i["dt"], "silu", 0.5, 1.0)
+    res = _shifted(i["z"].float().cuda())
+    o, r = ops.block_norm(y, wt, 1e-5, residual=res, post_weight=wt, gate=c["dt"], scale=0.5, w_offset=1.0)
+    _held(o, ref, tol, True)
+    _held(r, rr, rtol, False)
+
+
 @gpu
 def test_offsets_past_32_bits():
     rows, d, far = 3, 16, (1 << 31) // 2 + 64          # rows 2^30 elements apart: the last one past 2^31
