@@ -52,7 +52,10 @@ AIR_DEVICE float exp2_fast(float u) {
 template <typename T, int V>
 AIR_DEVICE void load_v(const T* p, float* f) {
   if constexpr (V == 1) f[0] = to_f(*p);
-  else if constexpr (sizeof(T) == 2 && V == 8) bf16x8_to_f32(*reinterpret_cast<const uint4*>(p), f);
+  else if constexpr (sizeof(T) == 2 && V % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 8) bf16x8_to_f32(*reinterpret_cast<const uint4*>(p + i), f + i);
+  }
   else if constexpr (sizeof(T) == 2 && V == 4) {
     const uint2 u = *reinterpret_cast<const uint2*>(p);
     const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
