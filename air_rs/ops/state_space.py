@@ -63,8 +63,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     x, dt and z [T, D] in bf16 or f32 (one type, any token strides, rows contiguous); A f32 [D, N], N <= 256; B and C
     [T, N] or [T, G, N] of the same type (G divides D, channel d reads group d // (D / G)); D and dt_bias f32 [D].
     ``cu_seqlens``, ``slots``, ``has_state`` and what is reported are those of :func:`causal_conv`; ``state`` is
-    f32 [S, D, N], updated in place. h, delta and the sums are f32; y is rounded once, to x's type. More than 64 states,
-    and calls of fewer than six tokens a sequence, run token by token."""
+    f32 [S, D, N], updated in place. h, delta and the sums are f32; y is rounded once, to x's type. A state that holds an
+    infinity keeps it where it decays fast and may become NaN where |delta A| <= 1/32. More than 64 states, and calls of
+    fewer than six tokens a sequence, run token by token."""
     out = require_ext().selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus, state, cu_seqlens, slots, has_state,
                                        out, _err(x) if err is None else err)
     count_launch()

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kTokThreads) scan_tokens_kernel(const ScanArgs
       const int c = q * S + i;
       const float b = c < a.N ? to_f(B[t * a.bs_t + c]) : 0.f;
       const float cc = c < a.N ? to_f(C[t * a.cs_t + c]) : 0.f;
-      h[i] = fmaf(decay_m1(delta * A[i]), h[i], fmaf(dx, b, h[i]));
+      h[i] = decayed(delta * A[i], h[i], dx, b);
       y = fmaf(cc, h[i], y);
     }
 #pragma unroll
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kTokThreads) scan_tokens_kernel(const ScanArgs
 }
 
 // Single tokens, `rows` of them a thread with A and the channel's parameters kept; the states of a lane are whole accesses
-// (N a multiple of 4 or 8, aligned rows). 128 x 8192 with 16 states takes 34.5 us at a floor of 21.9: instructions, of
+// (N a multiple of 4 or 8, aligned rows). 128 x 8192 with 16 states takes 33.6 us at a floor of 21.9: instructions, of
 // which the work of a channel (step, gate, addresses) is shared by eight states a lane (four: 46 us). Up to four rows a
 // thread (one: 57 us with four states a lane); two rows in flight cost more registers than they gain (44 us).
 template <typename T, int L, int S>
@@ -127,16 +127,16 @@ __global__ void __launch_bounds__(kTokThreads) scan_step_kernel(const ScanArgs a
       if (st) load_v<float, S>(st, h);
     }
     if (a.softplus) delta = softplus_f(delta);
-    const f2 step = dup2(delta), dx = dup2(delta * x);
+    const float dx = delta * x;
+    const f2 step = dup2(delta);
     f2 y2 = 0ull;
 #pragma unroll
     for (int i = 0; i < S / 2; ++i) {
       float u0, u1;
       unpack2(mul2(step, A[i]), u0, u1);
-      const f2 old = pack2(h[2 * i], h[2 * i + 1]);
-      const f2 now = fma2(pack2(decay_m1(u0), decay_m1(u1)), old, fma2(dx, pack2(B[2 * i], B[2 * i + 1]), old));
-      y2 = fma2(pack2(C[2 * i], C[2 * i + 1]), now, y2);
-      unpack2(now, h[2 * i], h[2 * i + 1]);
+      h[2 * i] = decayed(u0, h[2 * i], dx, B[2 * i]);
+      h[2 * i + 1] = decayed(u1, h[2 * i + 1], dx, B[2 * i + 1]);
+      y2 = fma2(pack2(C[2 * i], C[2 * i + 1]), pack2(h[2 * i], h[2 * i + 1]), y2);
     }
     float y, y_;
     unpack2(y2, y, y_);

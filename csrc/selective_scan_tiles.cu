@@ -4,7 +4,7 @@
 // What bounds it: one exponential per token, channel and state (a warp's exponential takes 8 clocks of its scheduler, a
 // paired multiply-add 2, both measured), against 8 bytes a token and channel: 64 channels of a token with 16 states are 33 ns
 // of an SM's exponentials and 12 ns of its share of the memory bandwidth. So the special-function, multiply-add and issue
-// slots are what counts: 8192 x 8192 x 16 bf16 takes 660 us where the exponentials alone would take 231 and the
+// slots are what counts: 8192 x 8192 x 16 bf16 takes 681 us where the exponentials alone would take 231 and the
 // bytes 82; issue slots are busy 58 % on average (67 % on the 108 SMs that have two blocks, 40 have one), the
 // multiply-add pipe 53 %.
 //
@@ -29,22 +29,16 @@ namespace air {
 
 namespace {
 
-// p = e - 1 where |u| is past the polynomial's interval
-AIR_DEVICE void far_decay(float& p, float u, float e) {
-  asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %1;\n\tsetp.gt.f32 q, a, %2;\n\t@q add.f32 %0, %3, 0fBF800000;\n\t}"
-      : "+f"(p) : "f"(u), "f"(kNearDecay), "f"(e));
-}
-// 2^u - 1 of M pairs (decay_m1), step by step over all of them: M independent chains, and the exponentials beside them
+// What 2^u h + in (decayed) takes of M pairs, step by step over all of them: p = 2^u - 1 beside slow decays, e = 2^u. M
+// independent chains, and the exponentials beside them.
 template <int M>
-AIR_DEVICE void decays(const f2* u, f2* p) {
+AIR_DEVICE void decays(const f2* u, f2* p, f2* e) {
   const f2 c2 = dup2(kDecay2), c1 = dup2(kDecay1), c0 = dup2(kDecay0);
-  float e[2 * M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     float ua, ub;
     unpack2(u[m], ua, ub);
-    e[2 * m] = exp2_fast(ua);
-    e[2 * m + 1] = exp2_fast(ub);
+    e[m] = pack2(exp2_fast(ua), exp2_fast(ub));
   }
 #pragma unroll
   for (int m = 0; m < M; ++m) p[m] = fma2(c2, u[m], c1);
@@ -52,15 +46,23 @@ AIR_DEVICE void decays(const f2* u, f2* p) {
   for (int m = 0; m < M; ++m) p[m] = fma2(p[m], u[m], c0);
 #pragma unroll
   for (int m = 0; m < M; ++m) p[m] = mul2(p[m], u[m]);
-#pragma unroll
-  for (int m = 0; m < M; ++m) {
-    float a, b, ua, ub;
-    unpack2(p[m], a, b);
-    unpack2(u[m], ua, ub);
-    far_decay(a, ua, e[2 * m]);
-    far_decay(b, ub, e[2 * m + 1]);
-    p[m] = pack2(a, b);
-  }
+}
+// One state of the pair: p = e past the slow decays, in += h beside them, so that the state's next value is p h + in. The sum is
+// all that waits for the token before.
+AIR_DEVICE void choose_decay(float u, float e, float h, float& p, float& in) {
+  asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %2;\n\tsetp.gt.f32 q, a, %3;\n\t@q mov.f32 %0, %4;\n\t@!q add.f32 %1, %1, %5;\n\t}"
+      : "+f"(p), "+f"(in) : "f"(u), "f"(kNearDecay), "f"(e), "f"(h));
+}
+AIR_DEVICE f2 decayed2(f2 u, f2 p, f2 e, f2 h, f2 in) {
+  float u0, u1, p0, p1, e0, e1, h0, h1, i0, i1;
+  unpack2(u, u0, u1);
+  unpack2(p, p0, p1);
+  unpack2(e, e0, e1);
+  unpack2(h, h0, h1);
+  unpack2(in, i0, i1);
+  choose_decay(u0, e0, h0, p0, i0);
+  choose_decay(u1, e1, h1, p1, i1);
+  return fma2(pack2(p0, p1), h, pack2(i0, i1));
 }
 // softplus_f of a pair
 AIR_DEVICE f2 softplus2(float a, float b) {
@@ -346,7 +348,7 @@ struct Scan {
   // through h. What the chains read, and the next tokens' steps, are loaded before. `sum`: of delta.
   template <bool OUT, int K>
   AIR_DEVICE void tokens(int buf, int i, ulonglong2* st, int next, f2& sum) {
-    f2 u[K * 2], p[K * 2], dx[K];
+    f2 u[K * 2], p[K * 2], e[K * 2], dx[K];
     float4 c[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -361,11 +363,11 @@ struct Scan {
 #pragma unroll
       for (int k = 0; k < K; ++k) st[k] = step(buf, next + k);
     }
-    decays<K * 2>(u, p);
+    decays<K * 2>(u, p, e);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      h[0] = fma2(p[k * 2], h[0], fma2(dx[k], dup2(c[k].x), h[0]));
-      h[1] = fma2(p[k * 2 + 1], h[1], fma2(dx[k], dup2(c[k].y), h[1]));
+      h[0] = decayed2(u[k * 2], p[k * 2], e[k * 2], h[0], mul2(dx[k], dup2(c[k].x)));
+      h[1] = decayed2(u[k * 2 + 1], p[k * 2 + 1], e[k * 2 + 1], h[1], mul2(dx[k], dup2(c[k].y)));
       if (OUT) *reinterpret_cast<f2*>(&sm.y[buf][i + k][part]) = fma2(dup2(c[k].w), h[1], mul2(dup2(c[k].z), h[0]));
     }
   }

@@ -196,14 +196,16 @@ AIR_DEVICE float softplus_f(float x) {
   return x != x ? x : fmaf(p, u, fmaxf(x, 0.f));
 }
 
-// 2^u - 1 for the scan's decays, u = delta A log2(e). Added as h + (2^u - 1) h, a slow decay keeps its rate: 2^u itself,
-// rounded to 24 bits, would change a rate of 2^-10 by 2^-14 of itself at every token. For |u| <= log2(e) / 32 a quadratic
-// times u (equal ripple of the relative error, computed for this interval: 3.2e-7, 4.2e-7 with the roundings), beyond it
-// the exponential less one, whose error is then at most 7.6e-6 of the rate.
+// A state's step: 2^u h + in, u = delta A log2(e). Beside slow decays, |u| <= log2(e) / 32, it is (2^u - 1) h + (h + in): so a
+// slow decay keeps its rate, where 2^u itself, rounded to 24 bits, would change a rate of 2^-10 by 2^-14 of itself at every
+// token. 2^u - 1 is a quadratic times u there (equal ripple of the relative error, computed for this interval: 3.2e-7, 4.2e-7
+// with the roundings). Beyond it 2^u h is rounded at its own size, not at that of the h it forgets; the exponential is then
+// off by at most 7.6e-6 of the rate.
 constexpr float kNearDecay = 0.0450842196f, kDecay0 = 0.693147182f, kDecay1 = 0.24024117f, kDecay2 = 0.0555041097f;
-AIR_DEVICE float decay_m1(float u) {
-  const float e = exp2_fast(u), p = fmaf(fmaf(kDecay2, u, kDecay1), u, kDecay0);
-  return fabsf(u) <= kNearDecay ? p * u : e - 1.f;
+AIR_DEVICE float decayed(float u, float h, float dx, float b) {
+  const float p = fmaf(fmaf(kDecay2, u, kDecay1), u, kDecay0) * u;
+  const bool slow = fabsf(u) <= kNearDecay;
+  return fmaf(slow ? p : exp2_fast(u), h, fmaf(dx, b, slow ? h : 0.f));
 }
 
 struct SeqRange {

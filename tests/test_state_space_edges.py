@@ -1,0 +1,126 @@
+"""Where the state-space operators round: states that a token forgets, growing states across cuts, rows of logits with one
+sure token; and launch forms that only larger calls take.
+
+u = 2^-24. An exponential 2^x is off by at most 4 u relatively; the decay less one of a slow state (|delta A| <= 1/32) by
+7.1 u of itself.
+"""
+import math
+
+import pytest
+import torch
+
+from air_rs import ops
+from test_state_space_ops import TYPES, U, _dev, _gen, _held, _i32, _scan_inputs, _silu
+
+gpu = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------- selective scan
+def _scan_bound(x, dt, A, B, C, D, z, bias, softplus, lens, init):
+    """-> out, its tolerance, states, their tolerance. Every rounding is relative to what is rounded: the old state counts
+    as far as the token keeps it, and whole only beside slow decays, where it is added to the token's input first."""
+    T, d = x.shape
+    per = torch.arange(d) // (d // B.shape[1])
+    v = dt.double() + (bias.double() if bias is not None else 0)
+    ev = U * (dt.double().abs() + (bias.double().abs() if bias is not None else 0))
+    if softplus:
+        delta = v.clamp(min=0) + torch.log1p(torch.exp(-v.abs()))
+        ed = delta * (2 * v.abs() * U + 10 * U) + ev * torch.sigmoid(v) + ev * delta
+    else:
+        delta, ed = v, ev
+    A, x64 = A.double(), x.double()
+    out, tol = torch.zeros(T, d, dtype=torch.float64), torch.zeros(T, d, dtype=torch.float64)
+    ends, tols, t = [], [], 0
+    for n, L in enumerate(lens):
+        h, e = init[n].double().clone(), torch.zeros(d, A.shape[1], dtype=torch.float64)
+        for _ in range(L):
+            g = delta[t][:, None] * A
+            a, b, c = torch.exp(g), B[t].double()[per], C[t].double()[per]
+            inp = (delta[t] * x64[t])[:, None] * b
+            eg = (ed[t] + 3 * U * delta[t].abs())[:, None] * A.abs()
+            slow, fast = g.abs() < 0.0313, g.abs() > 0.0312                 # both may hold beside 1/32
+            own = torch.maximum(7.1 * U * torch.expm1(g).abs() * slow, (4 * U * a + 2.0 ** -126) * fast)
+            e = a * e + (a * eg + own) * h.abs() + U * (h.abs() + inp.abs()) * slow + 3 * U * inp.abs() + \
+                (ed[t] * x64[t].abs())[:, None] * b.abs()
+            h = a * h + inp
+            e = 1.001 * (e + U * h.abs())
+            out[t] = (h * c).sum(-1)
+            tol[t] = (e * c.abs()).sum(-1) + (A.shape[1] + 3) * U * (h * c).abs().sum(-1)
+            t += 1
+        ends.append(h)
+        tols.append(e)
+    if D is not None:
+        out, tol = out + D.double() * x64, tol + 2 * U * ((D.double() * x64).abs() + out.abs())
+    if z is not None:
+        s = _silu(z.double())
+        out, tol = out * s, tol * s.abs() * 1.001 + (out * s).abs() * (2 * z.double().abs() + 12) * U
+    return out, tol, torch.stack(ends), torch.stack(tols)
+
+
+FORGETS = [  # lens, channels, states, groups: sequence by sequence, tiles of every width, tiles that cut a sequence
+    ([3, 1, 4, 5], 32, 16, 1),
+    ([9], 12, 130, 1),
+    ([40, 17], 32, 8, 1),
+    ([40, 17], 33, 16, 1),
+    ([19, 40], 32, 24, 2),
+    ([40, 17], 24, 64, 1),
+    ([700, 60], 64, 16, 1),
+    ([300, 230], 37, 8, 1),
+    ([300, 230], 40, 32, 1),
+    ([300, 230], 32, 64, 2),
+    ([260, 300], 24, 40, 1),
+]
+
+
+def _forgetting(seed, T, d, n, groups, dtype):
+    """Slow steps, and at every seventh token one that forgets all before it: 20 to 60 decay times, with a small input."""
+    i = _scan_inputs(seed, T, d, n, groups, dtype)
+    i["A"] = -(1 + torch.rand(d, n, generator=_gen(seed)))
+    i["dt"] = (0.002 * i["dt"].float().abs()).to(dtype)
+    i["dt"][5::7] = (20 + 10 * torch.rand(T, d, generator=_gen(seed + 1)))[5::7].to(dtype)
+    i["dt"][0] = 25.0
+    i["x"][5::7] = (1e-3 * i["x"].float())[5::7].to(dtype)
+    i["x"][0] *= 1e-3
+    return i
+
+
+@gpu
+@pytest.mark.parametrize("case", range(len(FORGETS)))
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scan_forgets_large_states(case, dtype):
+    """The state after a token that forgets is as exact as its own input, however large the state was before."""
+    lens, d, n, groups = FORGETS[case]
+    T, N = sum(lens), len(lens)
+    i = _forgetting(case, T, d, n, groups, dtype)
+    pool = 1e4 * torch.randn(N, d, n, generator=_gen(90 + case))
+    ref, tol, ends, etol = _scan_bound(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], None, None, False, lens, pool)
+    st = pool.cuda()
+    out = ops.selective_scan(*(i[k].cuda() for k in ("x", "dt", "A", "B", "C")), D=i["D"].cuda(), softplus=False, state=st,
+                             has_state=_i32([1] * N), cu_seqlens=_i32([0] + torch.tensor(lens).cumsum(0).tolist()))
+    _held(out, ref, tol, dtype == torch.bfloat16)
+    _held(st, ends, etol, False)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,n", [(32, 16), (24, 8), (10, 5), (8, 64), (6, 200)])
+def test_scan_step_forgets_large_states(dtype, d, n):
+    i = _forgetting(d, 8, d, n, 1, dtype)              # rows 0 and 5 forget
+    pool = 1e4 * torch.randn(8, d, n, generator=_gen(d))
+    ref, tol, ends, etol = _scan_bound(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], None, None, False, [1] * 8, pool)
+    st = pool.cuda()
+    c = {k: _dev(v) for k, v in i.items()}
+    out = ops.selective_scan_step(c["x"], c["dt"], c["A"], c["B"], c["C"], st, D=c["D"], softplus=False)
+    _held(out, ref, tol, dtype == torch.bfloat16)
+    _held(st, ends, etol, False)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 40])
+def test_scan_keeps_infinite_states_of_fast_decays(T):
+    d, n = 16, 16
+    i = {k: _dev(v) for k, v in _scan_inputs(0, T, d, n, 1, torch.float32, gate=False).items()}
+    st = torch.full((1, d, n), math.inf, device="cuda")
+    ops.selective_scan(i["x"], torch.ones_like(i["dt"]), torch.full_like(i["A"], -1.0), i["B"], i["C"], softplus=False, state=st,
+                       has_state=_i32([1]))
+    assert bool((st == math.inf).all())
