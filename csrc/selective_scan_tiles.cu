@@ -386,6 +386,13 @@ struct Scan {
   }
 };
 
+// 2^u h in two steps: with positive rates (or negative steps) 2^u may pass f32 while the product does not, and nothing grows
+// to nothing.
+AIR_DEVICE float grown(float u, float h) {
+  const float half = exp2f(0.5f * u);
+  return h == 0.f ? 0.f : h * half * half;
+}
+
 AIR_DEVICE bool starts_from(const SeqArgs& a, int n, int64_t& slot) {
   const SeqRange s = seq_range(a, n, false);
   slot = s.slot;
@@ -478,7 +485,9 @@ __global__ void __launch_bounds__(Shape<L>::THREADS, Shape<L>::BLOCKS) scan_tile
         for (int i = 0; i < 2; ++i) {
           float u, v;
           unpack2(mul2(w.A[i], pack2(sum[0], sum[1])), u, v);
-          acc[i] = fma2(pack2(exp2f(u), exp2f(v)), w.h[i], acc[i]);
+          float a, b;
+          unpack2(w.h[i], a, b);
+          acc[i] = add2(pack2(grown(u, a), grown(v, b)), acc[i]);
         }
 #pragma unroll
         for (int s_ = 0; s_ < 2; ++s_)

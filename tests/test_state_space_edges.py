@@ -124,3 +124,29 @@ def test_scan_keeps_infinite_states_of_fast_decays(T):
     ops.selective_scan(i["x"], torch.ones_like(i["dt"]), torch.full_like(i["A"], -1.0), i["B"], i["C"], softplus=False, state=st,
                        has_state=_i32([1]))
     assert bool((st == math.inf).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_growing_states_across_cuts(dtype):
+    """Positive rates: a stretch of tokens may multiply a state by more than f32 holds while the state itself fits."""
+    T, d, n = 512, 16, 16                              # cut into tiles of 64 tokens
+    i = _scan_inputs(0, T, d, n, 1, dtype, gate=False)
+    i["A"] = 1.5 + 0.1 * torch.rand(d, n, generator=_gen(1))
+    i["x"][:-5] = 0
+    tile = torch.arange(T) // 64
+    i["dt"] = torch.where(tile % 2 == 0, 1.0, -1.0)[:, None].expand(T, d).contiguous().to(dtype)
+    for start in (0.0, 1e-32):                         # at most e^102 times that
+        pool = torch.full((1, d, n), start)
+        ref, tol, ends, etol = _scan_bound(i["x"], i["dt"], i["A"], i["B"], i["C"], None, None, None, False, [T], pool)
+        st = pool.cuda()
+        out = ops.selective_scan(*(i[k].cuda() for k in ("x", "dt", "A", "B", "C")), softplus=False, state=st, has_state=_i32([1]))
+        _held(out, ref, tol, dtype == torch.bfloat16)
+        _held(st, ends, etol, False)
+    # rates that no product of f32 holds, and nothing to grow
+    i["dt"].fill_(4.0)
+    ref, tol, ends, etol = _scan_bound(i["x"], i["dt"], i["A"], i["B"], i["C"], None, None, None, False, [T], torch.zeros(1, d, n))
+    st = torch.zeros(1, d, n, device="cuda")
+    out = ops.selective_scan(*(i[k].cuda() for k in ("x", "dt", "A", "B", "C")), softplus=False, state=st)
+    _held(out, ref, tol, dtype == torch.bfloat16)
+    _held(st, ends, etol, False)
