@@ -128,7 +128,7 @@ struct Sums {
   float ref, s, e;                         // s = sum exp(d), e = sum d exp(d) for d = x - ref
   AIR_DEVICE void move(float to) {         // to >= ref
     const float d = ref - to, f = ref == -INFINITY ? 0.f : exp2f(d * kLog2e);
-    e = ref == -INFINITY ? 0.f : f * fmaf(d, s, e);
+    e = f == 0.f ? 0.f : f * fmaf(d, s, e);      // d s may pass f32 where nothing is left
     s *= f;
     ref = to;
   }

@@ -150,3 +150,20 @@ def test_growing_states_across_cuts(dtype):
     out = ops.selective_scan(*(i[k].cuda() for k in ("x", "dt", "A", "B", "C")), softplus=False, state=st)
     _held(out, ref, tol, dtype == torch.bfloat16)
     _held(st, ends, etol, False)
+
+
+# ---------------------------------------------------------------------------------- token log probabilities
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V", [(12, 97), (12, 70001), (500, 40000)])
+def test_entropy_of_rows_with_a_huge_logit(dtype, T, V):
+    """One logit so far above the others that it is certain: entropy zero, also where differences pass the type's range."""
+    x = 3 * torch.randn(T, V, generator=_gen(T)).cuda()
+    top = torch.tensor([torch.finfo(dtype).max, 1e36, 1e35, 3e38], device="cuda")[torch.arange(T, device="cuda") % 4]
+    at = torch.randint(0, V, (T,), generator=_gen(V)).cuda()
+    x[torch.arange(T, device="cuda"), at] = top
+    x[1::3, at[0]] = torch.minimum(x[1::3, at[0]], torch.tensor(torch.finfo(dtype).min, device="cuda"))
+    x[torch.arange(T, device="cuda"), at] = top
+    r = ops.token_logprobs(x.to(dtype), at.int(), top=2)
+    assert bool((r.entropy == 0).all()) and bool((r.logprobs == 0).all())
+    assert torch.equal(r.top_ids[:, 0], at.int()) and bool((r.top_logprobs[:, 0] == 0).all())
