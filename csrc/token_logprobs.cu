@@ -3,17 +3,19 @@
 // and the k most likely tokens (ties: the lowest index first).
 //
 // A block (or a cluster of blocks, with few rows) streams its row in 16-byte accesses. Each thread keeps s = sum exp(d) and
-// e = sum d exp(d) for d = x - ref and moves its reference only when a logit passes it by more than 16, so the exponential
-// and four paired operations are what two elements cost; sums are f32, joined around the row's maximum:
-// entropy = log s - e / s. Infinities below count as -1e30, whose exponential is an exact zero.
+// e = sum d exp(d) for d = x - ref, ref being its largest logit so far: four vectors are summed by themselves around the new
+// maximum, then the sums before are moved there and added, so the exponential and four paired operations are what two
+// elements cost, and a favourite's term, next to which small ones round, meets only a vector's worth of them and then
+// sums. The threads' sums are f32, joined around the row's maximum: entropy = log s - e / s. Infinities below count as
+// -1e30, whose exponential is an exact zero.
 //
 // The alternatives need no second pass over the row: the k-th largest of the threads' maxima is at most the k-th largest
 // logit, so only the k threads whose maximum reaches it can hold one. Their elements (k / threads of the row, from L2) are
 // read again by the whole block, the few that reach the bound are collected and ordered. A row with fewer than k logits
 // above -1e29 is swept once more, for finite ones below.
 //
-// Memory-bound with many long rows: 2048 x 128256 bf16 takes 101 us without alternatives (5.2 TB/s, floor 80), 110 with one,
-// 131 with five where every 16th row has three tokens left and is swept twice. One row of f32 takes 6.1 us without and 10.4 with 20.
+// Memory-bound with many long rows: 2048 x 128256 bf16 takes 94 us without alternatives (5.6 TB/s, floor 80), 103 with one,
+// 122 with five where every 16th row has three tokens left and is swept twice. One row of f32 takes 6.1 us without and 10.4 with 20.
 #include <cooperative_groups.h>
 
 #include "state_space.cuh"
@@ -26,7 +28,6 @@ namespace cg = cooperative_groups;
 
 constexpr float kMasked = -1e30f;          // stands for -inf in the sums
 constexpr float kAllLow = -1e29f;          // a row whose maximum is below takes the plain path
-constexpr float kMargin = 16.f;
 
 using Key = unsigned long long;
 // Order of the alternatives as one number: the value's bits mapped to rising unsigned ones, then the index inverted.
@@ -240,10 +241,19 @@ AIR_DEVICE void collect(LpSmem<T, NT>& sm, const Row<T>& row, int k, int items, 
   for (int w0 = threadIdx.x; w0 < items; w0 += NT * U) {
     Vec<T> v[U];
     int i[U];
+    bool whole = true;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       i[u] = w0 + u * NT < items ? at(w0 + u * NT) : -1;
-      if (i[u] >= 0) v[u] = row(i[u]);
+      whole &= i[u] > 0 && i[u] < row.vectors - 1;
+    }
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u].load(row.base + (int64_t)i[u] * E);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i[u] >= 0) v[u] = row(i[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -284,39 +294,45 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const TokenLogprobAr
   const int per = (row.vectors + CS - 1) / CS;
   const int v0 = min(row.vectors, rank * per), v1 = min(row.vectors, v0 + per);
 
-  float ref = -INFINITY, top = -INFINITY;
-  f2 s2 = 0ull, e2 = 0ull, back = 0ull;              // the sums in two halves; -ref twice
+  float ref = kMasked;                               // the largest logit so far
+  f2 s2 = 0ull, e2 = 0ull;                           // the sums in two halves
   auto join = [&]() {
     float s0, s1, e0, e1;
     unpack2(s2, s0, s1);
     unpack2(e2, e0, e1);
     return Sums{ref, s0 + s1, e0 + e1};
   };
-  auto add = [&](V& v) {
-    v.clamp();
-    const float m = v.max();
-    top = fmaxf(top, m);
-    if (m > ref + kMargin || ref == -INFINITY) {
-      Sums r = join();
-      r.move(m);
-      ref = m;
-      s2 = pack2(r.s, 0.f);
-      e2 = pack2(r.e, 0.f);
-      back = dup2(-m);
-    }
-    float f[E];
-    v.get(f);
+  auto add = [&](V (&v)[U]) {
+    float to = ref;
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const f2 d = add2(pack2(f[i], f[i + 1]), back);
-      float u0, u1;
-      unpack2(mul2(d, dup2(kLog2e)), u0, u1);
-      const f2 p = pack2(exp2_fast(u0), exp2_fast(u1));
-      s2 = add2(s2, p);
-      e2 = fma2(d, p, e2);
+    for (int j = 0; j < U; ++j) {
+      v[j].clamp();
+      to = fmaxf(to, v[j].max());
     }
+    f2 gs = 0ull, ge = 0ull;
+    const f2 back = dup2(-to);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float f[E];
+      v[j].get(f);
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        const f2 d = add2(pack2(f[i], f[i + 1]), back);
+        float u0, u1;
+        unpack2(mul2(d, dup2(kLog2e)), u0, u1);
+        const f2 p = pack2(exp2_fast(u0), exp2_fast(u1));
+        gs = add2(gs, p);
+        ge = fma2(d, p, ge);
+      }
+    }
+    const float d = fmaxf(ref - to, -1000.f);        // far enough to be nothing, and d s stays in f32
+    const f2 f = dup2(exp2_fast(d * kLog2e));
+    e2 = fma2(f, fma2(dup2(d), s2, e2), ge);
+    s2 = fma2(f, s2, gs);
+    ref = to;
   };
-  // whole vectors, several in flight, then the two at the row's ends, which may hold fewer elements
+  // whole vectors, several in flight; then what is left of them with one of the two at the row's ends, which may hold fewer
+  // elements
   const int w0 = v0 + (v0 == 0), w1 = v1 - (v1 == row.vectors && v1 > w0);
   const T* p = row.base + (int64_t)(w0 + threadIdx.x) * E;
   int i = w0 + threadIdx.x;
@@ -324,20 +340,18 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const TokenLogprobAr
     V v[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) v[j].load(p + j * NT * E);
+    add(v);
+  }
+  const int end = threadIdx.x == 0 && w0 > v0 && v1 > v0 ? v0 : threadIdx.x == NT - 1 && w1 < v1 ? w1 : -1;
+  if (i < w1 || end >= 0) {
+    V v[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) add(v[j]);
-  }
-  for (; i < w1; i += NT, p += NT * E) {
-    V v;
-    v.load(p);
-    add(v);
-  }
-  if (threadIdx.x == 0 && w0 > v0 && v1 > v0) {
-    V v = row(v0);
-    add(v);
-  }
-  if (threadIdx.x == NT - 1 && w1 < v1) {
-    V v = row(w1);
+    for (int j = 0; j < U - 1; ++j) {
+      if (i + j * NT < w1) v[j].load(p + j * NT * E);
+      else v[j].load_part(p, 0, 0);
+    }
+    if (end >= 0) v[U - 1] = row(end);
+    else v[U - 1].load_part(p, 0, 0);
     add(v);
   }
 
@@ -345,7 +359,7 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const TokenLogprobAr
   {
     const Sums w = warp_join(join());
     if ((threadIdx.x & 31) == 0) sm.warp[threadIdx.x >> 5] = w;
-    sm.maxima[threadIdx.x] = top;
+    sm.maxima[threadIdx.x] = ref;
     if (threadIdx.x == 0) sm.n_chosen = sm.count = 0;
   }
   __syncthreads();
@@ -362,7 +376,7 @@ __global__ void __launch_bounds__(NT) token_logprobs_kernel(const TokenLogprobAr
   // ---- the block's k largest
   if (a.k) {
     const float bound = sm.bound;
-    if (top >= bound) sm.chosen[atomicAdd(&sm.n_chosen, 1)] = (short)threadIdx.x;
+    if (ref >= bound) sm.chosen[atomicAdd(&sm.n_chosen, 1)] = (short)threadIdx.x;
     __syncthreads();
     const int each = (w1 - w0 + NT - 1) / NT + 1;    // a thread's vectors; the last place is for one of the row's ends
     collect<T, NT>(sm, row, a.k, sm.n_chosen * each,

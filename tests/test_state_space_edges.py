@@ -167,3 +167,52 @@ def test_entropy_of_rows_with_a_huge_logit(dtype, T, V):
     r = ops.token_logprobs(x.to(dtype), at.int(), top=2)
     assert bool((r.entropy == 0).all()) and bool((r.logprobs == 0).all())
     assert torch.equal(r.top_ids[:, 0], at.int()) and bool((r.top_logprobs[:, 0] == 0).all())
+
+
+def _lp_bound(logits, tokens, top):
+    """Holds a call against 64 bits, on the device. Exponentials are of d = x - (the largest so far), off by (3 |d| + 4) u,
+    but the largest logit's is exactly one: what is relative to the other terms only counts for their share of the sum. R
+    counts roundings of the sums: 16 adds of four vectors, one for each of a thread's groups of four (4096 logits a block
+    or more) and 16 of the halves, lanes, warps and blocks; where the maximum moves, the terms before it take a factor that is
+    off by 4 u, at most once a group and ten times in the joins."""
+    r = ops.token_logprobs(logits, tokens, top=top)
+    V = logits.shape[1]
+    R = 16 + (V / 4096 + 2) + 16
+    small = 4 + 4 * (V / 4096 + 12)
+    for lo in range(0, logits.shape[0], 256):
+        rows = slice(lo, lo + 256)
+        x = logits[rows].double()
+        m = x.amax(-1, keepdim=True)
+        dist = m - x
+        s = torch.exp(-dist).sum(-1)
+        p, ls = torch.exp(-dist) / s[:, None], torch.log(s)
+        spread = (p * dist).sum(-1)
+        rel = (3 * spread + small * (p * (dist > 0)).sum(-1) + R) * U
+        lp = -dist - ls[:, None]
+        near = lambda at, v: rel[:, None] + U * (2 * ls[:, None] + dist.gather(1, at) + v.abs())
+        tok = tokens[rows].long()[:, None]
+        want = lp.gather(1, tok)
+        _held(r.logprobs[rows], want[:, 0].cpu(), near(tok, want)[:, 0].cpu(), False)
+        ent = ls + spread
+        te = rel * (1 + spread) + (p * dist * (3 * dist + 1 + small)).sum(-1) * U + R * U * spread + U * (2 * ls + 2 * spread + ent)
+        _held(r.entropy[rows], ent.cpu(), te.cpu(), False)
+        if top:
+            order = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top]
+            assert torch.equal(r.top_ids[rows].long(), order)
+            want = lp.gather(1, order)
+            _held(r.top_logprobs[rows], want.cpu(), near(order, want).cpu(), False)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1, 450])
+def test_entropy_of_sure_rows(dtype, T):
+    """A favourite 11 to 16 above everything else: its exponential must not swallow the small ones."""
+    V = 128000
+    x = torch.zeros(T, V)
+    x[::2] = torch.randn(len(x[::2]), V, generator=_gen(T))
+    at = torch.randint(0, V, (T,), generator=_gen(1))
+    x[torch.arange(T), at] = 11 + 4.9 * torch.rand(T, generator=_gen(2))
+    _lp_bound(x.to(dtype).cuda(), at.int().cuda(), 1)
+    x[:, 0] = 12.0                                     # and one that comes first
+    _lp_bound(x.to(dtype).cuda(), at.int().cuda(), 0)
