@@ -851,13 +851,16 @@ class Engine:
 
     def token_scores(self, ids: list[int], add_bos: bool | None = None, top: int = 0):
         """:meth:`token_logprobs` with the entropy at each position and its ``top`` most likely tokens (at most 32), as
-        ``ops.TokenLogprobs`` of CPU tensors."""
+        ``ops.TokenLogprobs`` of CPU tensors. IndexError for an id outside the vocabulary."""
         from .. import ops
         if not 0 <= top <= 32:
             raise ValueError(f"token_scores: 0 to 32 alternatives, not {top}")
         bos = self.add_bos if add_bos is None else add_bos
         ids = ([self.cfg.bos_token_id] if bos else []) + list(ids)
         T = len(ids)
+        for t in ids:
+            if not 0 <= t < self.cfg.vocab_size:
+                raise IndexError(f"token_scores: token id {t} is outside the vocabulary of {self.cfg.vocab_size}")
         if T < 2:
             return ops.TokenLogprobs(torch.empty(0), torch.empty(0), torch.empty(0, top), torch.empty(0, top, dtype=torch.int32))
         if self.runner is None:
@@ -889,8 +892,9 @@ class Engine:
                             torch.zeros(T, dtype=torch.int32, device=dev), tab.to(dev),
                             torch.arange(T - 1, dtype=torch.int64, device=dev), None, None, None, None,
                             None, return_logits=True)
-            r = ops.token_logprobs(lg, tok[1:], top=top)
-            return ops.TokenLogprobs(*(t.cpu() for t in r))
+            r = ops.TokenLogprobs(*(t.cpu() for t in ops.token_logprobs(lg, tok[1:], top=top, err=rn.err)))
+            rn.check_errors()
+            return r
         finally:
             self.seqs.free_sequence(seq)
 

@@ -216,3 +216,51 @@ def test_entropy_of_sure_rows(dtype, T):
     _lp_bound(x.to(dtype).cuda(), at.int().cuda(), 1)
     x[:, 0] = 12.0                                     # and one that comes first
     _lp_bound(x.to(dtype).cuda(), at.int().cuda(), 0)
+
+
+# ---------------------------------------------------------------------------------- the engine's scores
+def _engine(device):
+    from air_rs.gguf import GGMLType
+    from air_rs.models.config import tiny_llama
+    from air_rs.models.random_init import random_tensors
+    from air_rs.models.reference import OracleModel
+    from air_rs.runtime.builder import build_runner
+    from air_rs.runtime.engine import Engine
+    cfg = tiny_llama()
+    recs = list(random_tensors(cfg, GGMLType.Q8_0, seed=0, device="cpu"))
+    if device == "cpu":
+        return Engine(cfg, None, oracle=OracleModel(cfg, {n: (r, q, s) for n, r, q, s in recs}))
+    return Engine(cfg, build_runner(cfg, iter(recs), device="cuda", max_batch=8, max_model_len=256, num_blocks=64))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_engine_scores_no_id_outside_the_vocabulary(device):
+    eng = _engine(device)
+    V, ids = eng.cfg.vocab_size, [5, 6, 7, 8]
+    scores = eng.token_logprobs(ids)
+    for bad in (-1, V, V + 100, -V):
+        for at in range(len(ids)):
+            wrong = ids[:at] + [bad] + ids[at + 1:]
+            with pytest.raises(IndexError, match="vocabulary"):
+                eng.token_logprobs(wrong)
+            with pytest.raises(IndexError, match="vocabulary"):
+                eng.token_scores(wrong, top=2)
+    with pytest.raises(IndexError, match="vocabulary"):
+        eng.token_scores([V], add_bos=False)
+    assert eng.token_logprobs(ids) == scores            # nothing is left of the refused calls
+    if device == "cuda":
+        from air_rs.runtime.engine import SamplingParams
+        out = eng.generate_ids([ids], SamplingParams(max_tokens=3, temperature=0.0, ignore_eos=True))
+        assert len(out[0]) == 3 and int(eng.runner.err) == 0
+        ops.check_errors()
+    assert eng.token_logprobs([0, V - 1], add_bos=False)[0] < 0
+
+
+@gpu
+def test_engine_scores_read_the_runners_errors():
+    eng = _engine("cuda")
+    eng.runner.err.fill_(1)                             # as a kernel of the scored forward would
+    with pytest.raises(RuntimeError, match="error code 1"):
+        eng.token_scores([5, 6, 7])
+    assert len(eng.token_logprobs([5, 6, 7], add_bos=False)) == 2
+    assert eng.seqs.allocator.num_used_blocks() == 0
