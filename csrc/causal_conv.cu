@@ -8,8 +8,9 @@
 // Sequences: the first W - 1 tokens and the state row, read and replaced by the same threads, so no block reads a row
 // that another writes. x is read once but for W - 1 rows a run. Memory-bound: two element sizes of traffic for
 // 2 W + 5 operations and two special functions; the arithmetic runs on pairs of channels (f32x2).
-// 16384 x 8192 bf16 with four taps takes 100 us (5.4 TB/s, floor 82; f32 8192 x 8192 87 us), and rows that
-// are not whole 16-byte parts, which go element by element or in pairs, 187 to 197 us.
+// 16384 x 8192 bf16 with two, three and four taps takes 87, 92 and 100 us (5.4 TB/s and more, floor 82; f32 8192 x 8192 85, 86
+// and 87 us). Rows that are not whole 16-byte parts go in pairs or element by element: 163, 166 and 195 us in pairs, 182 to 193
+// in single elements.
 #include "state_space.cuh"
 
 namespace air {

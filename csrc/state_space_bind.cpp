@@ -163,7 +163,8 @@ Tensor conv(const char* op, const Tensor& x, const Tensor& w, const optional<Ten
   a.D = (int)D;
   a.W = (int)W;
   a.silu = silu;
-  int vec = !aligned(w, 16) ? 1 : x.scalar_type() == at::kFloat ? 4 : 8;
+  // a thread's taps start at a multiple of vec W floats: w need only start at 16 bytes
+  int vec = reinterpret_cast<uintptr_t>(a.w) % 16 ? 1 : x.scalar_type() == at::kFloat ? 4 : 8;
   auto rows = [&](const Tensor& t) {
     while (vec > 1 && (D % vec || !aligned(t, vec * t.element_size()))) vec /= 2;
   };

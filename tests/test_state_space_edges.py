@@ -264,3 +264,29 @@ def test_engine_scores_read_the_runners_errors():
         eng.token_scores([5, 6, 7])
     assert len(eng.token_logprobs([5, 6, 7], add_bos=False)) == 2
     assert eng.seqs.allocator.num_used_blocks() == 0
+
+
+# ---------------------------------------------------------------------------------- causal convolution
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("step", [False, True])
+def test_few_taps_read_whole_rows(dtype, step):
+    """Two and three taps take no longer than four: their rows are as whole, and they compute less."""
+    d = 8192
+    x = torch.randn(4096 if step else 8192, d, device="cuda").to(dtype)
+    out = torch.empty_like(x)
+
+    def us(W):
+        w, st = torch.randn(d, W, device="cuda"), torch.zeros(x.shape[0], W - 1, d, dtype=dtype, device="cuda")
+        times = []
+        for _ in range(9):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ops.causal_conv_step(x, w, st, out=out) if step else ops.causal_conv(x, w, out=out)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 1e3)
+        return sorted(times)[4]
+    four = us(4)
+    for W in (2, 3):
+        assert us(W) <= 1.3 * four
