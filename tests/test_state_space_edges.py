@@ -290,3 +290,61 @@ def test_few_taps_read_whole_rows(dtype, step):
     four = us(4)
     for W in (2, 3):
         assert us(W) <= 1.3 * four
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,vectors", [(1100, 640), (1100, 1500), (1000, 1500), (30, 4100), (150, 4100), (300, 4100), (420, 4100), (600, 4100)])
+@pytest.mark.parametrize("top", [0, 7])
+def test_token_logprobs_blocks_of_every_size(dtype, T, vectors, top):
+    """Blocks of 64, 128, 256 and 512 threads and clusters of 8, 4 and 2, rows of odd lengths that start anywhere."""
+    V = vectors * (8 if dtype == torch.bfloat16 else 4) - 3
+    g = torch.Generator(device="cuda").manual_seed(T + vectors)
+    x = (4 * torch.randn(T, V + 5, generator=g, device="cuda")).to(dtype)[:, 2:V + 2]
+    tok = torch.randint(0, V, (T,), generator=g, device="cuda").int()
+    tok[::3] = x.float().argmax(-1)[::3].int()
+    _lp_bound(x, tok, top)
+
+
+# ---------------------------------------------------------------------------------- forms of larger calls
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,d,n", [(75, 8192, 16), (21, 8192, 64), (41, 8190, 24), (161, 4096, 8)])
+def test_scan_step_with_several_rows_a_thread(dtype, B, d, n):
+    i = _scan_inputs(B, B, d, n, 1, dtype)
+    g = _gen(B)
+    pool = torch.randn(B + 2, d, n, generator=g)
+    slots = torch.randperm(B + 2, generator=g)[:B].int()
+    slots[2], slots[B - 1] = -1, -1
+    live = slots >= 0
+    init = pool[slots.long().clamp(min=0)]
+    ref, tol, ends, etol = _scan_bound(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["bias"], True, [1] * B, init)
+    c = {k: _dev(v) for k, v in i.items()}
+    st = pool.cuda()
+    out = ops.selective_scan_step(c["x"], c["dt"], c["A"], c["B"], c["C"], st, D=c["D"], z=c["z"], dt_bias=c["bias"], slots=slots.cuda())
+    _held(out[live.cuda()], ref[live], tol[live], dtype == torch.bfloat16)
+    assert bool((out[~live.cuda()] == 0).all())
+    st = st.cpu()
+    _held(st[slots[live].long()], ends[live], etol[live], False)
+    free = [s for s in range(B + 2) if s not in slots.tolist()]
+    assert torch.equal(st[free], pool[free])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,d,n,groups", [([300, 0, 200, 77], 32, 64, 1), ([150, 400], 37, 40, 1), ([513], 48, 64, 2), ([70, 330], 22, 33, 1)])
+def test_scan_cuts_prompts_with_many_states(dtype, lens, d, n, groups):
+    """33 to 64 states, sequences that cross the ends of tiles, with and without an initial state, rows at odd places too."""
+    T, N = sum(lens), len(lens)
+    i = _scan_inputs(T, T, d, n, groups, dtype)
+    pool = torch.randn(N, d, n, generator=_gen(T))
+    for has in ([1] * N, [k % 2 for k in range(N)]):
+        init = pool * torch.tensor(has)[:, None, None]
+        ref, tol, ends, etol = _scan_bound(i["x"], i["dt"], i["A"], i["B"], i["C"], i["D"], i["z"], i["bias"], True, lens, init)
+        for pad in (1, 16):
+            st, out = pool.cuda(), torch.full((T, d + pad), 7.0, dtype=dtype, device="cuda")
+            ops.selective_scan(*(i[k].cuda() for k in ("x", "dt", "A", "B", "C")), D=i["D"].cuda(), z=i["z"].cuda(), dt_bias=i["bias"].cuda(),
+                               state=st, has_state=_i32(has), cu_seqlens=_i32([0] + torch.tensor(lens).cumsum(0).tolist()), out=out[:, :d])
+            _held(out[:, :d], ref, tol, dtype == torch.bfloat16)
+            assert bool((out[:, d:] == 7).all())
+            _held(st, ends, etol, False)
