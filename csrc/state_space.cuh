@@ -219,7 +219,7 @@ AIR_DEVICE SeqRange seq_range(const SeqArgs& a, int n, bool report = true) {
   SeqRange s;
   s.t0 = a.cu ? a.cu[n] : a.step ? n : 0;
   s.t1 = a.cu ? a.cu[n + 1] : a.step ? n + 1 : a.T;
-  s.slot = a.S > 0 ? (a.slots ? (int64_t)a.slots[n] : (int64_t)n) : -1;
+  s.slot = a.slots ? (int64_t)a.slots[n] : a.S > 0 ? (int64_t)n : -1;
   if (s.t0 < 0 || s.t1 < s.t0 || s.t1 > a.T) {
     if (report) set_error(a.err, kErrBounds);
     s.t0 = s.t1 = 0;

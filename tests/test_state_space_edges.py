@@ -348,3 +348,20 @@ def test_scan_cuts_prompts_with_many_states(dtype, lens, d, n, groups):
             _held(out[:, :d], ref, tol, dtype == torch.bfloat16)
             assert bool((out[:, d:] == 7).all())
             _held(st, ends, etol, False)
+
+
+# ---------------------------------------------------------------------------------- state rows
+@gpu
+@pytest.mark.parametrize("T", [2, 40])
+def test_rows_of_an_empty_pool_are_reported(T):
+    """A pool without rows has no row 0: reported, and as if without a state."""
+    d = 16
+    i = {k: _dev(v) for k, v in _scan_inputs(0, T, d, 16, 1, torch.float32, gate=False).items()}
+    args, w = (i["x"], i["dt"], i["A"], i["B"], i["C"]), torch.randn(d, 4, generator=_gen(0)).cuda()
+    none = dict(conv=torch.empty(0, 3, d, device="cuda"), scan=torch.empty(0, d, 16, device="cuda"))
+    for slot, code in ((0, 1), (3, 1), (-1, 0)):
+        err = torch.zeros(2, dtype=torch.int32, device="cuda")
+        kw = dict(slots=_i32([slot]), has_state=_i32([1]))
+        assert torch.equal(ops.causal_conv(i["x"], w, state=none["conv"], err=err[:1], **kw), ops.causal_conv(i["x"], w))
+        assert torch.equal(ops.selective_scan(*args, state=none["scan"], err=err[1:], **kw), ops.selective_scan(*args))
+        assert err.tolist() == [code, code]
