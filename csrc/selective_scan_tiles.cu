@@ -4,9 +4,8 @@
 // What bounds it: one exponential per token, channel and state (a warp's exponential takes 8 clocks of its scheduler, a
 // paired multiply-add 2, both measured), against 8 bytes a token and channel: 64 channels of a token with 16 states are 33 ns
 // of an SM's exponentials and 12 ns of its share of the memory bandwidth. So the special-function, multiply-add and issue
-// slots are what counts: 8192 x 8192 x 16 bf16 takes 681 us where the exponentials alone would take 231 and the
-// bytes 82; issue slots are busy 58 % on average (67 % on the 108 SMs that have two blocks, 40 have one), the
-// multiply-add pipe 53 %.
+// slots are what counts: 8192 x 8192 x 16 bf16 takes 657 us where the exponentials alone would take 231 and the
+// bytes 82; issue slots are busy 61 % on average (108 SMs have two blocks, 40 have one), the multiply-add pipe 51 %.
 //
 // A block has as many scan warps as helper warps, four of each (two blocks an SM). L lanes share a pair of channels, each
 // with two states of both: the arithmetic runs on pairs of channels (f32x2), so the steps of a pair are one operand and y
@@ -29,7 +28,7 @@ namespace air {
 
 namespace {
 
-// What 2^u h + in (decayed) takes of M pairs, step by step over all of them: p = 2^u - 1 beside slow decays, e = 2^u. M
+// What 2^u h + in (decayed) takes of M pairs, step by step over all of them: e = 2^u and p = (2^u - 1) / u beside slow decays. M
 // independent chains, and the exponentials beside them.
 template <int M>
 AIR_DEVICE void decays(const f2* u, f2* p, f2* e) {
@@ -44,25 +43,23 @@ AIR_DEVICE void decays(const f2* u, f2* p, f2* e) {
   for (int m = 0; m < M; ++m) p[m] = fma2(c2, u[m], c1);
 #pragma unroll
   for (int m = 0; m < M; ++m) p[m] = fma2(p[m], u[m], c0);
-#pragma unroll
-  for (int m = 0; m < M; ++m) p[m] = mul2(p[m], u[m]);
 }
-// One state of the pair: p = e past the slow decays, in += h beside them, so that the state's next value is p h + in. The sum is
-// all that waits for the token before.
-AIR_DEVICE void choose_decay(float u, float e, float h, float& p, float& in) {
-  asm("{\n\t.reg .pred q;\n\t.reg .f32 a;\n\tabs.f32 a, %2;\n\tsetp.gt.f32 q, a, %3;\n\t@q mov.f32 %0, %4;\n\t@!q add.f32 %1, %1, %5;\n\t}"
-      : "+f"(p), "+f"(in) : "f"(u), "f"(kNearDecay), "f"(e), "f"(h));
+// One state of the pair: what multiplies h, and what of h is added beside it. (Adding h to the token's input under a
+// predicate, a shorter chain through h, takes 681 us where this takes 657, and 810 for 841 at 16384 x 4096, one block an SM.)
+AIR_DEVICE void choose_decay(float u, float p, float h, float& e, float& kept) {
+  const bool slow = fabsf(u) <= kNearDecay;
+  e = slow ? p * u : e;
+  kept = slow ? h : 0.f;
 }
-AIR_DEVICE f2 decayed2(f2 u, f2 p, f2 e, f2 h, f2 in) {
-  float u0, u1, p0, p1, e0, e1, h0, h1, i0, i1;
+AIR_DEVICE f2 decayed2(f2 u, f2 p, f2 e, f2 h, f2 dx, f2 b) {
+  float u0, u1, p0, p1, e0, e1, h0, h1, k0, k1;
   unpack2(u, u0, u1);
   unpack2(p, p0, p1);
   unpack2(e, e0, e1);
   unpack2(h, h0, h1);
-  unpack2(in, i0, i1);
-  choose_decay(u0, e0, h0, p0, i0);
-  choose_decay(u1, e1, h1, p1, i1);
-  return fma2(pack2(p0, p1), h, pack2(i0, i1));
+  choose_decay(u0, p0, h0, e0, k0);
+  choose_decay(u1, p1, h1, e1, k1);
+  return fma2(pack2(e0, e1), h, fma2(dx, b, pack2(k0, k1)));
 }
 // softplus_f of a pair
 AIR_DEVICE f2 softplus2(float a, float b) {
@@ -366,8 +363,8 @@ struct Scan {
     decays<K * 2>(u, p, e);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      h[0] = decayed2(u[k * 2], p[k * 2], e[k * 2], h[0], mul2(dx[k], dup2(c[k].x)));
-      h[1] = decayed2(u[k * 2 + 1], p[k * 2 + 1], e[k * 2 + 1], h[1], mul2(dx[k], dup2(c[k].y)));
+      h[0] = decayed2(u[k * 2], p[k * 2], e[k * 2], h[0], dx[k], dup2(c[k].x));
+      h[1] = decayed2(u[k * 2 + 1], p[k * 2 + 1], e[k * 2 + 1], h[1], dx[k], dup2(c[k].y));
       if (OUT) *reinterpret_cast<f2*>(&sm.y[buf][i + k][part]) = fma2(dup2(c[k].w), h[1], mul2(dup2(c[k].z), h[0]));
     }
   }
