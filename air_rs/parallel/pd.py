@@ -276,6 +276,20 @@ class TcpKvConnector:
                 with self._cv:
                     self._errors.append(e)
                     self._cv.notify_all()
+                self._discard(conn)
+
+    @staticmethod
+    def _discard(conn, seconds: float = 1.0):
+        """Takes the rest of a refused stream: closing over unread bytes resets the connection, and a sender still at its
+        frame would see that instead of the end of its call."""
+        deadline = time.monotonic() + seconds
+        try:
+            while (left := deadline - time.monotonic()) > 0:
+                conn.settimeout(left)
+                if not conn.recv(1 << 16):
+                    return
+        except OSError:
+            pass
 
     def send_blocks(self, seq_id: int, blocks: list[KvBlock], target, timeout: float = 2.0,
                     corrupt: bool = False, features: int = 0) -> int:
