@@ -65,7 +65,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     ``cu_seqlens``, ``slots``, ``has_state`` and what is reported are those of :func:`causal_conv`; ``state`` is
     f32 [S, D, N], updated in place. h, delta and the sums are f32; y is rounded once, to x's type. A state that holds an
     infinity keeps it where it decays fast and may become NaN where |delta A| <= 1/32. More than 64 states, and calls of
-    fewer than six tokens a sequence, run token by token."""
+    fewer than six tokens a sequence on average, run token by token (about a microsecond for each token of the longest
+    sequence): single tokens that are batched with a long prompt belong in a call of :func:`selective_scan_step`."""
     out = require_ext().selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus, state, cu_seqlens, slots, has_state,
                                        out, _err(x) if err is None else err)
     count_launch()

@@ -88,7 +88,7 @@ AIR_DEVICE int scanned(int k) { return 3 + (k & 1); }
 template <int L>
 struct Shape {
   // Threads that scan, and as many helpers. Two blocks an SM of 128 + 128, or, where many lanes share a pair and a block of
-  // that size would have few channels to share B and C, one of 256 + 256 (8000 x 2048 with 64 states: 607 against 765 us).
+  // that size would have few channels to share B and C, one of 256 + 256 (8000 x 2048 with 64 states: 590 against 758 us).
   static constexpr int SCAN = L <= 16 ? 128 : 256, HELP = SCAN, THREADS = SCAN + HELP, BLOCKS = 256 / SCAN;
   static constexpr int CH = 2 * SCAN / L, CP = CH / 2;   // channels a block, and pairs
   static constexpr int TS = L <= 4 ? 8 : 16;             // tokens a stage
@@ -609,8 +609,10 @@ ScanPlan scan_plan(const ScanArgs& a, int sms) {
 }
 
 // A sequence's start and end cost a walk through a tile 1.2 us (offsets, then the state, one after the other), so calls of
-// short sequences go sequence by sequence: 4000 tokens of 4096 channels in sequences of 4 take 849 us here and 662 there,
-// in sequences of 8 533 and 591, of 16 370 and 556; 64 sequences of one token 80 and 20.
+// short sequences go sequence by sequence: 4000 tokens of 4096 channels in sequences of 4 take 643 us here and 663 there,
+// in sequences of 8 425 and 596, of 16 312 and 567; 64 sequences of one token 60 and 18. The lengths are on the device: a call
+// whose mean is below the limit pays for a long sequence among short ones (4000 tokens with 1000 sequences of one:
+// 816 and 5750 us).
 bool scan_tiles_worth(const ScanArgs& a) { return a.N <= 64 && a.seq.T >= 6ll * a.seq.N; }
 
 const char* launch_scan_tiles(const ScanArgs& a, const ScanPlan& p, float* ws, bool f32, cudaStream_t st) {

@@ -15,7 +15,7 @@
 // above -1e29 is swept once more, for finite ones below.
 //
 // Memory-bound with many long rows: 2048 x 128256 bf16 takes 94 us without alternatives (5.6 TB/s, floor 80), 103 with one,
-// 122 with five where every 16th row has three tokens left and is swept twice. One row of f32 takes 6.1 us without and 10.4 with 20.
+// 122 with five where every 16th row has three tokens left and is swept twice. One row of f32 takes 6.1 us without and 10.5 with 20.
 #include <cooperative_groups.h>
 
 #include "state_space.cuh"
@@ -448,10 +448,10 @@ void launch(const TokenLogprobArgs& a, cudaStream_t st) {
 
 template <typename T>
 void choose(const TokenLogprobArgs& a, cudaStream_t st) {
-  // Blocks of 256 threads fill the device at five an SM. Rows that leave room are cut among clusters of up to 8 blocks (1 row
-  // of 128256: 9.8 us against 16.4 by one block; 100 rows: 19 against 38), or taken by larger blocks (400 rows: 46
-  // against 53). Many short rows leave most threads of a block idle in the selection: 20000 x 5000 takes 101 us
-  // with 64 threads, 128 with 128 and 233 with 256, 4000 x 16000 takes 64, 56 and 70; 300 x 10000 20, 13 and 10.
+  // Blocks of 256 threads fill the device at four or five an SM. Rows that leave room are cut among clusters of up to 8 blocks (1
+  // row of 128256: 10.5 us against 18.4 by one block; 100 rows: 16 against 27), or taken by larger blocks (400 rows: 39.7
+  // against 40.3). Many short rows leave most threads of a block idle in the selection: 20000 x 5000 takes 85 us
+  // with 64 threads, 112 with 128 and 199 with 256, 4000 x 16000 takes 50, 48 and 64; 300 x 10000 10.1, 8.2 and 8.8.
   const int64_t room = 148 * 5, vectors = a.V / Vec<T>::E;
   if (vectors <= 1024 && a.T > 1024) launch<T, 64, 1>(a, st);
   else if (vectors <= 2048 && a.T > 1024) launch<T, 128, 1>(a, st);
