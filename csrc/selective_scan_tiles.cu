@@ -44,22 +44,26 @@ AIR_DEVICE void decays(const f2* u, f2* p, f2* e) {
 #pragma unroll
   for (int m = 0; m < M; ++m) p[m] = fma2(p[m], u[m], c0);
 }
-// One state of the pair: what multiplies h, and what of h is added beside it. (Adding h to the token's input under a
-// predicate, a shorter chain through h, takes 681 us where this takes 657, and 810 for 841 at 16384 x 4096, one block an SM.)
-AIR_DEVICE void choose_decay(float u, float p, float h, float& e, float& kept) {
+// One state of the pair, by one comparison: what multiplies h, and what of h is added. SELECT: h or zero, which the token's input
+// is then added to in the same instruction. Otherwise the sum of h and `in`, the input by itself, whose product does not
+// wait for the token before: an instruction more, a step less in the chain through h.
+template <bool SELECT>
+AIR_DEVICE void choose_decay(float u, float p, float h, float& e, float& in) {
   const bool slow = fabsf(u) <= kNearDecay;
   e = slow ? p * u : e;
-  kept = slow ? h : 0.f;
+  in = SELECT ? (slow ? h : 0.f) : slow ? in + h : in;
 }
+template <bool SELECT>
 AIR_DEVICE f2 decayed2(f2 u, f2 p, f2 e, f2 h, f2 dx, f2 b) {
-  float u0, u1, p0, p1, e0, e1, h0, h1, k0, k1;
+  float u0, u1, p0, p1, e0, e1, h0, h1, i0, i1;
   unpack2(u, u0, u1);
   unpack2(p, p0, p1);
   unpack2(e, e0, e1);
   unpack2(h, h0, h1);
-  choose_decay(u0, p0, h0, e0, k0);
-  choose_decay(u1, p1, h1, e1, k1);
-  return fma2(pack2(e0, e1), h, fma2(dx, b, pack2(k0, k1)));
+  if (!SELECT) unpack2(mul2(dx, b), i0, i1);
+  choose_decay<SELECT>(u0, p0, h0, e0, i0);
+  choose_decay<SELECT>(u1, p1, h1, e1, i1);
+  return fma2(pack2(e0, e1), h, SELECT ? fma2(dx, b, pack2(i0, i1)) : pack2(i0, i1));
 }
 // softplus_f of a pair
 AIR_DEVICE f2 softplus2(float a, float b) {
@@ -281,7 +285,7 @@ struct Helper {
 };
 
 // ---- scan warps: two states of two channels a lane, as pairs over the channels
-template <typename T, int L>
+template <typename T, int L, bool SELECT>
 struct Scan {
   using S = Shape<L>;
   const ScanArgs& a;
@@ -363,8 +367,8 @@ struct Scan {
     decays<K * 2>(u, p, e);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      h[0] = decayed2(u[k * 2], p[k * 2], e[k * 2], h[0], dx[k], dup2(c[k].x));
-      h[1] = decayed2(u[k * 2 + 1], p[k * 2 + 1], e[k * 2 + 1], h[1], dx[k], dup2(c[k].y));
+      h[0] = decayed2<SELECT>(u[k * 2], p[k * 2], e[k * 2], h[0], dx[k], dup2(c[k].x));
+      h[1] = decayed2<SELECT>(u[k * 2 + 1], p[k * 2 + 1], e[k * 2 + 1], h[1], dx[k], dup2(c[k].y));
       if (OUT) *reinterpret_cast<f2*>(&sm.y[buf][i + k][part]) = fma2(dup2(c[k].w), h[1], mul2(dup2(c[k].z), h[0]));
     }
   }
@@ -396,7 +400,7 @@ AIR_DEVICE bool starts_from(const SeqArgs& a, int n, int64_t& slot) {
   return s.init;
 }
 
-template <typename T, int L, bool FIRST, bool VEC>
+template <typename T, int L, bool FIRST, bool VEC, bool SELECT>
 __global__ void __launch_bounds__(Shape<L>::THREADS, Shape<L>::BLOCKS) scan_tiles_kernel(const __grid_constant__ ScanArgs a, const __grid_constant__ TileArgs ta, bool vec_bc) {
   using S = Shape<L>;
   extern __shared__ __align__(16) uint8_t raw_smem[];
@@ -458,7 +462,7 @@ __global__ void __launch_bounds__(Shape<L>::THREADS, Shape<L>::BLOCKS) scan_tile
     return;
   }
 
-  Scan<T, L> w(a, sm, d0, left);
+  Scan<T, L, SELECT> w(a, sm, d0, left);
   const bool al = a.N % 2 == 0;                              // scratch is aligned
   auto enter = [&](int t) {                                  // the state before token t of seg
     w.zero();
@@ -557,12 +561,21 @@ const char* launch(const ScanArgs& a, const ScanPlan& p, float* ws, bool vec_bc,
   const int64_t blocks = (int64_t)ta.blocks_g * a.G;
   if (blocks * p.tiles >= (1ll << 31)) return "selective_scan: too many channels and tokens for one call";
   constexpr int bytes = sizeof(Smem<T, L>);
-  static unsigned long long done1 = 0, done2 = 0;
-  if (!set_max_smem_per_device(scan_tiles_kernel<T, L, true, VEC>, bytes, done1) ||
-      !set_max_smem_per_device(scan_tiles_kernel<T, L, false, VEC>, bytes, done2))
+  static unsigned long long done1 = 0, done2 = 0, done3 = 0;
+  constexpr auto first = scan_tiles_kernel<T, L, true, VEC, false>;
+  if (p.tiles > 1) {
+    if (!set_max_smem_per_device(first, bytes, done1)) return "selective_scan: the device has too little shared memory";
+    first<<<(unsigned)(blocks * (p.tiles - 1)), S::THREADS, bytes, st>>>(a, ta, vec_bc);
+  }
+  // The form of the decay's sum (choose_decay). Eight scan warps on an SM hide its chain, so the shorter form pays: 8192 x
+  // 8192 takes 657 us with it and 681 without, 8000 x 2048 with 64 states 590 and 608; with one block an SM 16384 x 4096 takes 840 us
+  // with it and 809 without, 8000 x 2048 with 24 states 413 and 389. Up to 8 states it never paid (4000 x 4096: 186 and 184).
+  constexpr bool always = L == 32, never = L == 4;
+  constexpr auto shorter = scan_tiles_kernel<T, L, false, VEC, !never>, other = scan_tiles_kernel<T, L, false, VEC, always>;
+  const bool pays = always || (!never && p.pairs);
+  if (!set_max_smem_per_device(pays ? shorter : other, bytes, pays ? done2 : done3))
     return "selective_scan: the device has too little shared memory";
-  if (p.tiles > 1) scan_tiles_kernel<T, L, true, VEC><<<(unsigned)(blocks * (p.tiles - 1)), S::THREADS, bytes, st>>>(a, ta, vec_bc);
-  scan_tiles_kernel<T, L, false, VEC><<<(unsigned)(blocks * p.tiles), S::THREADS, bytes, st>>>(a, ta, vec_bc);
+  (pays ? shorter : other)<<<(unsigned)(blocks * p.tiles), S::THREADS, bytes, st>>>(a, ta, vec_bc);
   return nullptr;
 }
 
@@ -592,7 +605,7 @@ ScanPlan scan_plan(const ScanArgs& a, int sms) {
     const int64_t c = (n + sms - 1) / sms;
     return pairs ? c / 2 * 1.5 + c % 2 : c * 1.5;
   };
-  ScanPlan best{1, a.seq.T, 0};
+  ScanPlan best{1, a.seq.T, false, 0};
   double cost = a.seq.T * speed(blocks);
   for (int64_t n = 2; n <= 64 && a.seq.T / n >= 64; ++n) {
     const int64_t tile = ((a.seq.T + n - 1) / n + 15) / 16 * 16;
@@ -602,9 +615,10 @@ ScanPlan scan_plan(const ScanArgs& a, int sms) {
     const double c = tile * speed(blocks * tiles) + 0.65 * crossing * tile * speed(blocks * (tiles - 1)) + 48.0 + tiles;
     if (c < cost) {
       cost = c;
-      best = {(int)tiles, (int)tile, (int64_t)tiles * a.D * (2 * a.N + 1)};
+      best = {(int)tiles, (int)tile, false, (int64_t)tiles * a.D * (2 * a.N + 1)};
     }
   }
+  best.pairs = blocks * best.tiles > sms;
   return best;
 }
 

@@ -46,9 +46,11 @@ constexpr int kScanMaxStates = 256;
 // Sequences token by token, a few threads per channel: any shape.
 void launch_scan_tokens(const ScanArgs& a, bool f32, cudaStream_t st);
 
-// Prompts in tiles of tokens, at most 64 states: the number of tiles, their tokens and the floats of scratch.
+// Prompts in tiles of tokens, at most 64 states: the number of tiles, their tokens, whether SMs have two blocks each and the
+// floats of scratch.
 struct ScanPlan {
   int tiles, tile;
+  bool pairs;
   int64_t floats;
 };
 bool scan_tiles_worth(const ScanArgs& a);       // against launch_scan_tokens, by size

@@ -57,7 +57,7 @@ def _scan_bound(x, dt, A, B, C, D, z, bias, softplus, lens, init):
     return out, tol, torch.stack(ends), torch.stack(tols)
 
 
-FORGETS = [  # lens, channels, states, groups: sequence by sequence, tiles of every width, tiles that cut a sequence
+FORGETS = [  # lens, channels, states, groups: sequence by sequence, tiles of every width, tiles that cut a sequence, two blocks an SM
     ([3, 1, 4, 5], 32, 16, 1),
     ([9], 12, 130, 1),
     ([40, 17], 32, 8, 1),
@@ -69,6 +69,8 @@ FORGETS = [  # lens, channels, states, groups: sequence by sequence, tiles of ev
     ([300, 230], 40, 32, 1),
     ([300, 230], 32, 64, 2),
     ([260, 300], 24, 40, 1),
+    ([25, 14], 5001, 16, 1),
+    ([14, 25], 2512, 24, 1),
 ]
 
 
